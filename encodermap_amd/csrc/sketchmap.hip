@@ -581,11 +581,12 @@ typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));   // (HIP's uint
 template <int LT, bool FASTSIG, int NCH>
 // (leading scalars: what the tile decode and the first operand loads need, preloaded into scalar registers at wave launch --
 //  -amdgpu-kernarg-preload-count; 56 bytes, the struct follows)
-__global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(LT > 8 ? 3 : 8, LT > 8 ? 3 : 8))) void sk_tile_f16_kernel(
+__global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(LT > 8 ? 3 : NCH == 0 ? 6 : 8, LT > 8 ? 3 : NCH == 0 ? 6 : 8))) void sk_tile_f16_kernel(
     const uint16_t* p_planes, long p_plane_stride, int p_xcd_nbg, int p_nbc, int p_symm, int p_deal_world, int p_deal_rank, int p_row0, int p_B,
     int p_split_B, int p_split_ld, int p_kmode_ksplit, const SkArgs a) {
   // (the compiler sizes its register budget for the occupancy a 64-KB LDS would allow; gfx950 has 160 KB, so the target
-  //  is stated: 8 tiles resident per CU: <= 64 VGPRs, <= 20 KB LDS)
+  //  is stated: 8 tiles resident per CU: <= 64 VGPRs, <= 20 KB LDS; a run-time number of chunks needs 78 VGPRs: 6 per CU -- held to 64 it
+  //  spills inside the chunk loop, and the ADC step takes 0.165 ms instead of 0.098)
   constexpr int T = 64;
   constexpr int LMAX = LT ? LT : 4;
   // LT = 8: latent widths 5 .. 8 (run-time width, zero padded).  Every consumer plans latents beyond four columns on the 32-tile

@@ -175,7 +175,8 @@ __global__ __launch_bounds__(NTC) void wide_layer_kernel(const WideArgs a) {
                 d = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah[s], wp[p & 1][s][1], d, 0, 0, 0);
                 d = __builtin_amdgcn_mfma_f32_16x16x32_f16(al[s], wp[p & 1][s][0], d, 0, 0, 0);
                 d = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah[s], wp[p & 1][s][0], d, 0, 0, 0);
-                acc[p] = d * rsa[s] + acc[p];
+#pragma unroll   // (per element: without packed float instructions a whole-vector multiply-add costs hundreds of spilled registers)
+                for (int e = 0; e < 4; ++e) acc[p][e] = fmaf(d[e], rsa[s][e], acc[p][e]);
               }
             }
           }

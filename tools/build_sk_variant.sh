@@ -8,7 +8,7 @@ root=$(cd "$(dirname "$0")/.." && pwd)
 mkdir -p "$root/$(dirname "$out")"
 obj=$(mktemp /tmp/emx_sketchmap.XXXXXX.o)
 trap 'rm -f "$obj"' EXIT
-hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -ffp-contract=on -mllvm -amdgpu-kernarg-preload-count=16 -I"$root/include" -I"$root/encodermap_amd/csrc" $extra \
+hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -ffp-contract=on -mllvm -amdgpu-kernarg-preload-count=16 -Xclang -target-feature -Xclang -packed-fp32-ops -I"$root/include" -I"$root/encodermap_amd/csrc" $extra \
   -c "$root/encodermap_amd/csrc/sketchmap.hip" -o "$obj"
 others=$(ls "$root"/build/obj/*.o | grep -v '/sketchmap.o$')
 hipcc --offload-arch=gfx950 -shared -fPIC $others "$obj" -o "$root/$out"

@@ -11,7 +11,7 @@ mkdir -p "$work/encodermap_amd" "$root/$(dirname "$out")"
 cp -r "$root/encodermap_amd/csrc" "$work/encodermap_amd/csrc"
 cp -r "$root/include" "$work/include"
 if [ -n "$patch_file" ] && [ "$patch_file" != "-" ]; then (cd "$work" && patch -p1 < "$root/$patch_file"); fi
-flags="--offload-arch=gfx950 -O3 -std=c++17 -fPIC -ffp-contract=on -mllvm -amdgpu-kernarg-preload-count=16 -I$work/include -I$work/encodermap_amd/csrc $extra"
+flags="--offload-arch=gfx950 -O3 -std=c++17 -fPIC -ffp-contract=on -mllvm -amdgpu-kernarg-preload-count=16 -Xclang -target-feature -Xclang -packed-fp32-ops -I$work/include -I$work/encodermap_amd/csrc $extra"
 objs=""
 for src in "$work"/encodermap_amd/csrc/*.hip; do
   obj="$work/$(basename "${src%.hip}").o"

@@ -14,7 +14,7 @@ def main():
     src = sys.argv[1]
     flt = sys.argv[2] if len(sys.argv) > 2 and not sys.argv[2].startswith("-") else ""
     extra = sys.argv[3:] if flt else sys.argv[2:]
-    cmd = ["hipcc", "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=on", "-mllvm", "-amdgpu-kernarg-preload-count=16",
+    cmd = ["hipcc", "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=on", "-mllvm", "-amdgpu-kernarg-preload-count=16", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
            "-I" + os.path.join(ROOT, "include"), "-I" + os.path.dirname(os.path.abspath(src)), "-I" + os.path.join(ROOT, "encodermap_amd", "csrc"), *extra,
            "--cuda-device-only", "-c", src, "-o", "/dev/null",
            "-Rpass-analysis=kernel-resource-usage"]
