@@ -97,6 +97,9 @@ SIGNATURES = {
     "emx_mlp_aop_bytes": (_sz, [_p, _i]),
     "emx_mlp_forward": (_i, [_p, _p, _p, _i, _i, _p, _i, _i, _i, _p, _p, _i, _p]),
     "emx_mlp_infer": (_i, [_p, _p, _i, _i, _p, _l, _f, _l, _p, _l, _f, _p]),
+    "emx_layernorm_fwd": (_i, [_p, _i, _l, _i, _l, _p, _p, _f, _p, _l, _p, _p, _p]),
+    "emx_layernorm_ws_floats": (_sz, [_l, _i]),
+    "emx_layernorm_bwd": (_i, [_p, _l, _p, _l, _i, _l, _i, _p, _p, _p, _p, _l, _p, _p, _p, _sz, _p]),
     "emx_p2p_handle_bytes": (_i, []),
     "emx_p2p_create": (_i, [_i, _i, _l, _i, C.POINTER(_p), _p]),
     "emx_p2p_connect": (_i, [_p, _p]),
@@ -812,6 +815,80 @@ def mlp_wgrad_adam_local(plan: MlpPlan, row_begin, row_end, ws, finish: "FinishD
 
 
 # ---- ADC path ---------------------------------------------------------------------------------------------------
+_ELEMENT_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}   # EMX_F32, EMX_F16, EMX_BF16
+
+
+def _element_type(t, what) -> int:
+    code = _ELEMENT_TYPES.get(t.dtype)
+    if code is None:
+        raise EmxError(f"{what}: float32, float16 or bfloat16 expected, got {t.dtype}")
+    return code
+
+
+def _like(t, ref, what) -> None:
+    """``t`` on the device of ``ref``, and a device of the GPU's"""
+    if not t.is_cuda or t.device != ref.device:
+        raise EmxError(f"{what}: a tensor on {ref.device} expected (a GPU), got {t.device}")
+
+
+def _rows(t, ref, what) -> int:
+    """the row stride of a [rows, D] tensor like ``ref`` (its device, type and shape) whose columns lie side by side"""
+    _like(t, ref, what)
+    if t.dtype != ref.dtype or t.shape != ref.shape or t.dim() != 2:
+        raise EmxError(f"{what}: {ref.dtype} [rows, D] like the input's {tuple(ref.shape)} expected, got {t.dtype} {tuple(t.shape)}")
+    stride, col = t.stride()
+    if col != 1 and t.shape[1] > 1:
+        raise EmxError(f"{what}: the columns of a row have to lie side by side, got strides {t.stride()}")
+    return stride
+
+
+def _vector(t, n, ref, what):
+    """the address of a contiguous float32 vector of n elements (None: NULL)"""
+    if t is None:
+        return None
+    _like(t, ref, what)
+    if t.dtype != torch.float32 or t.numel() != n or not t.is_contiguous():
+        raise EmxError(f"{what}: {n} contiguous float32 values expected, got {t.dtype} {tuple(t.shape)}, strides {t.stride()}")
+    return t.data_ptr()
+
+
+def _on_device(device, fn, what, *args) -> None:
+    """``fn(*args, stream)`` on torch's current stream of ``device``, whichever device is current"""
+    if device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return _check(fn(*args, _stream()), what)
+    _check(fn(*args, _stream()), what)
+
+
+def layernorm_fwd(x, gamma, beta, eps, y, mean=None, rstd=None):
+    """y = layer norm of the rows of ``x`` [n, D] (float32 / float16 / bfloat16, rows of any stride); ``gamma`` / ``beta`` float32 [D] or
+    None, ``mean`` / ``rstd`` float32 [n] are kept for ``layernorm_bwd`` (None: not kept).  ``y`` may be ``x``."""
+    code = _element_type(x, "x")
+    ldx, ldy = _rows(x, x, "x"), _rows(y, x, "y")
+    n, D = x.shape
+    _on_device(x.device, load().emx_layernorm_fwd, "emx_layernorm_fwd", x.data_ptr(), code, n, D, ldx, _vector(gamma, D, x, "gamma"),
+               _vector(beta, D, x, "beta"), float(eps), y.data_ptr(), ldy, _vector(mean, n, x, "mean"), _vector(rstd, n, x, "rstd"))
+
+
+def layernorm_ws_floats(n_rows, D) -> int:
+    return int(load().emx_layernorm_ws_floats(int(n_rows), int(D)))
+
+
+def layernorm_bwd(dy, x, gamma, mean, rstd, dx, dgamma, dbeta, ws=None):
+    """The gradients of ``layernorm_fwd``: ``dx`` like ``x`` (may be ``dy`` or ``x``), ``dgamma`` / ``dbeta`` float32 [D], overwritten; None:
+    not wanted.  ``ws``: ``layernorm_ws_floats(n, D)`` float32 of scratch (needed for dgamma / dbeta)."""
+    code = _element_type(x, "x")
+    ldx, ld_dy = _rows(x, x, "x"), _rows(dy, x, "dy")
+    ld_dx = _rows(dx, x, "dx") if dx is not None else 0
+    n, D = x.shape
+    if ws is not None:
+        _vector(ws, ws.numel(), x, "ws")
+    _on_device(x.device, load().emx_layernorm_bwd, "emx_layernorm_bwd", dy.data_ptr(), ld_dy, x.data_ptr(), ldx, code, n, D,
+               _vector(gamma, D, x, "gamma"), _vector(mean, n, x, "mean"), _vector(rstd, n, x, "rstd"),
+               None if dx is None else dx.data_ptr(), ld_dx, _vector(dgamma, D, x, "dgamma"), _vector(dbeta, D, x, "dbeta"),
+               None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel())
+
+
 def colmean(x, out):
     B, n = x.shape
     _check(load().emx_colmean(_ptr(x), B, n, x.stride(0), _ptr(out), _stream()), "emx_colmean")

@@ -569,6 +569,30 @@ int emx_mlp_wgrad_adam_local(const emx_mlp_desc* desc, float* params, int64_t n_
                              uint32_t* sync, emx_stream_t stream);
 
 /* ------------------------------------------------------------------------------------------------ *
+ * Layer norm over the last axis, forward and backward (csrc/layernorm.hip): normalised layers between the Dense launches above.  The
+ * reference's networks have none; a user of its Keras API gets it as tf.keras.layers.LayerNormalization around a Dense layer
+ * (models.py:3179-3220 builds the stack), whose arithmetic this is:
+ *   mean = 1/D sum x;  rstd = 1 / sqrt(1/D sum (x - mean)^2 + eps);  y = (x - mean) rstd gamma + beta
+ *   t = dy gamma, h = (x - mean) rstd:  dx = rstd (t - 1/D sum t - h 1/D sum t h);  dgamma = sum_rows dy h;  dbeta = sum_rows dy
+ *   x, y, dy, dx: n_rows rows of D values of type `dtype` (EMX_F32 / EMX_F16 / EMX_BF16, one type for all of a call), row strides in
+ *   elements, no alignment asked for beyond the element's.  Inputs may have any stride >= 0 (0: one row for all), outputs >= D.
+ *   gamma, beta, mean, rstd, dgamma, dbeta: float32.  gamma / beta NULL: ones / zeros.  mean / rstd NULL (forward): not kept.
+ *   dx, dgamma, dbeta NULL: not wanted.  dgamma and dbeta are overwritten, not added to; without rows they are zero.
+ *   y may be x, dx may be dy or x (same pointer, same stride); any other overlap of their address ranges is refused.
+ *   A row with an infinity or a NaN gives NaN in its own results (and in dgamma / dbeta); eps = 0 gives NaN for a constant row.
+ *   ws: emx_layernorm_ws_floats(n_rows, D) floats of scratch (may be NULL where dgamma and dbeta are); its contents mean nothing
+ *   between calls, calls that may run at the same time need one each.
+ * ------------------------------------------------------------------------------------------------ */
+enum { EMX_F32 = 0, EMX_F16 = 1, EMX_BF16 = 2 };
+#define EMX_LAYERNORM_MAX_D (1 << 28)
+int emx_layernorm_fwd(const void* x, int dtype, int64_t n_rows, int D, int64_t ldx, const float* gamma, const float* beta, float eps, void* y,
+                      int64_t ldy, float* mean, float* rstd, emx_stream_t stream);
+size_t emx_layernorm_ws_floats(int64_t n_rows, int D);
+int emx_layernorm_bwd(const void* dy, int64_t ld_dy, const void* x, int64_t ldx, int dtype, int64_t n_rows, int D, const float* gamma,
+                      const float* mean, const float* rstd, void* dx, int64_t ld_dx, float* dgamma, float* dbeta, float* ws, size_t ws_floats,
+                      emx_stream_t stream);
+
+/* ------------------------------------------------------------------------------------------------ *
  * ADC path (AngleDihedralCartesianEncoderMap): back-mapping and per-frame pair distances
  * ------------------------------------------------------------------------------------------------ */
 /* K8  column mean over the batch: out[k] = mean_b x[b,k]     MeanAngles / mean bond lengths, layers.py:971,1153-1161 */
