@@ -36,20 +36,257 @@ struct BwdArgs {
   int D, n_parts;
 };
 
-// the sum over all threads of a block, in every thread
+// the sum over groups of N lanes of a wave, in every lane (all lanes active): cross-lane moves inside rows of 16, lane swaps beyond
+template <int N>
+__device__ __forceinline__ float lanes_sum(float v) {
+  v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0xB1, 0xF, 0xF, true));    // lane ^ 1
+  v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x4E, 0xF, 0xF, true));    // lane ^ 2
+  v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x141, 0xF, 0xF, true));   // half mirror: quad ^ 1
+  if constexpr (N > 8) v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x140, 0xF, 0xF, true));   // mirror
+  if constexpr (N > 16) v = sum_xor16(v);
+  if constexpr (N > 32) v = sum_xor32(v);
+  return v;
+}
+
+// the sum over the TPR threads that share a row, in each of them.  More than a wave: one slot per wave in `area`, which the caller
+// gives each sum of a row anew (three in turn), so that one barrier is enough
+template <int TPR>
+__device__ __forceinline__ float row_sum(float v, float* area) {
+  if constexpr (TPR <= 64) return lanes_sum<TPR>(v);
+  v = wave_sum(v);
+  if ((threadIdx.x & 63) == 0) area[threadIdx.x >> 6] = v;
+  __syncthreads();
+  float s = 0.f;
+#pragma unroll
+  for (int i = 0; i < TPR / 64; ++i) s += area[i];
+  return s;
+}
 template <int N>
 __device__ __forceinline__ float block_all_sum(float v, float* smem /* N / 64 floats */) {
-  v = wave_sum(v);
-  if constexpr (N > 64) {
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    __syncthreads();   // (the area may still be read from the sum before)
-    if (lane == 0) smem[w] = v;
-    __syncthreads();
-    v = 0.f;
+  __syncthreads();   // (the area may still be read from the sum before)
+  return row_sum<N>(v, smem);
+}
+
+// 16 bytes of a row; the address is a multiple of the element's size only
+template <typename T>
+struct Lane {
+  static constexpr int V = 16 / sizeof(T);
+  typedef T vec __attribute__((ext_vector_type(16 / sizeof(T))));
+  typedef T loose __attribute__((ext_vector_type(16 / sizeof(T)), aligned(sizeof(T))));
+  static __device__ __forceinline__ vec load(const T* p, int left /* elements of the row from p on */) {
+    if (left >= V) return *reinterpret_cast<const loose*>(p);
+    vec v;
 #pragma unroll
-    for (int i = 0; i < N / 64; ++i) v += smem[i];
+    for (int e = 0; e < V; ++e) v[e] = e < left ? p[e] : (T)0.f;
+    return v;
   }
-  return v;
+  static __device__ __forceinline__ void store(T* p, const vec v, int left) {
+    if (left >= V) {
+      *reinterpret_cast<loose*>(p) = v;
+    } else {
+#pragma unroll
+      for (int e = 0; e < V; ++e)
+        if (e < left) p[e] = v[e];
+    }
+  }
+};
+template <int V>
+__device__ __forceinline__ void load_weights(const float* w, float other, int col, int D, float (&out)[V]) {
+#pragma unroll
+  for (int q = 0; q < V / 4; ++q) {
+    typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
+    if (w != nullptr && col + 4 * q + 4 <= D) {
+      const f4 v = *reinterpret_cast<const f4*>(w + col + 4 * q);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) out[4 * q + e] = v[e];
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) out[4 * q + e] = (w != nullptr && col + 4 * q + e < D) ? w[col + 4 * q + e] : other;
+    }
+  }
+}
+
+// ---- rows that fit into registers: TPR threads hold a row, thread t its vectors t, t + TPR, ... (NV of them); each thread works on U
+// rows at a time, whose loads are all requested before the first is used
+template <typename T, int TPR, int NV, int U>
+__global__ __launch_bounds__(TPR > NT ? TPR : NT) void ln_fwd_kernel(const FwdArgs a) {
+  constexpr int V = Lane<T>::V, G = (TPR > NT ? TPR : NT) / TPR;
+  __shared__ float sm[3][TPR > 64 ? TPR / 64 : 1];
+  const int t = threadIdx.x % TPR, g = threadIdx.x / TPR;
+  const float inv = 1.f / (float)a.D;
+  const int step = TPR * V, first = t * V;
+  typename Lane<T>::vec raw[U][NV];
+  const long r0 = ((long)blockIdx.x * U) * G + g;
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const T* x = (const T*)a.x + min(r0 + u * G, a.n_rows - 1) * a.ldx;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int col = first + i * step;
+      if (col < a.D) raw[u][i] = Lane<T>::load(x + col, a.D - col);
+    }
+  }
+  float ga[NV == 1 ? V : 1], be[NV == 1 ? V : 1];
+  if constexpr (NV == 1) {
+    load_weights<V>(a.gamma, 1.f, first, a.D, ga);
+    load_weights<V>(a.beta, 0.f, first, a.D, be);
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const long r = r0 + u * G;
+    float v[NV][V];
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int left = a.D - (first + i * step);
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        v[i][e] = e < left ? (float)raw[u][i][e] : 0.f;
+        s += v[i][e];
+      }
+    }
+    const float mu = row_sum<TPR>(s, sm[0]) * inv;
+    s = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int left = a.D - (first + i * step);
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        v[i][e] -= mu;
+        s = e < left ? fmaf(v[i][e], v[i][e], s) : s;
+      }
+    }
+    const float rs = 1.f / sqrtf(fmaf(row_sum<TPR>(s, sm[1]), inv, a.eps));
+    if (r < a.n_rows) {
+      T* y = (T*)a.y + r * a.ldy;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int col = first + i * step;
+        if (col < a.D) {
+          float gi[V], bi[V];
+          if constexpr (NV > 1) {
+            load_weights<V>(a.gamma, 1.f, col, a.D, gi);
+            load_weights<V>(a.beta, 0.f, col, a.D, bi);
+          }
+          typename Lane<T>::vec o;
+#pragma unroll
+          for (int e = 0; e < V; ++e) o[e] = (T)fmaf(v[i][e] * rs, NV == 1 ? ga[NV == 1 ? e : 0] : gi[e], NV == 1 ? be[NV == 1 ? e : 0] : bi[e]);
+          Lane<T>::store(y + col, o, a.D - col);
+        }
+      }
+      if (t == 0) {
+        if (a.mean) a.mean[r] = mu;
+        if (a.rstd) a.rstd[r] = rs;
+      }
+    }
+  }
+}
+
+// ---- backward, rows that fit into registers: workgroup p walks the rows of part p, G at a time, TPR threads to a row; a thread keeps the
+// sums of ITS columns over the part's rows, the G groups' are added through LDS at the end.  The next rows' loads travel under this row's sums.
+template <typename T, int TPR, int NV>
+__global__ __launch_bounds__(TPR > NT ? TPR : NT) void ln_bwd_kernel(const BwdArgs a) {
+  constexpr int V = Lane<T>::V, NB = TPR > NT ? TPR : NT, G = NB / TPR;
+  constexpr int CW = TPR * V;                                // columns of one vector of all threads of a row
+  __shared__ float sm[2][2][TPR > 64 ? TPR / 64 : 1];
+  __shared__ float fold[G > 1 ? G * CW : 1];
+  const int t = threadIdx.x % TPR, g = threadIdx.x / TPR;
+  const float inv = 1.f / (float)a.D;
+  const long r0 = blockIdx.x * a.rows_per_part, r1 = min(r0 + a.rows_per_part, a.n_rows);
+  float dg[NV][V], db[NV][V], gam[NV][V];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    load_weights<V>(a.gamma, 1.f, t * V + i * CW, a.D, gam[i]);
+#pragma unroll
+    for (int e = 0; e < V; ++e) dg[i][e] = db[i][e] = 0.f;
+  }
+  typename Lane<T>::vec rx[NV], rd[NV];
+  float nmu = 0.f, nrs = 0.f;
+  auto request = [&](const long row) __attribute__((always_inline)) {
+    const long r = min(row, a.n_rows - 1);
+    const T *x = (const T*)a.x + r * a.ldx, *dy = (const T*)a.dy + r * a.ld_dy;
+    nmu = a.mean[r], nrs = a.rstd[r];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int col = t * V + i * CW;
+      if (col < a.D) {
+        rx[i] = Lane<T>::load(x + col, a.D - col);
+        rd[i] = Lane<T>::load(dy + col, a.D - col);
+      }
+    }
+  };
+  if (r0 < r1) request(r0 + g);
+  int flip = 0;
+  for (long rb = r0; rb < r1; rb += G, flip ^= 1) {
+    const long r = rb + g;
+    const float mu = nmu, rs = nrs;
+    float h[NV][V], d[NV][V];
+    float s = 0.f, q = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int left = a.D - (t * V + i * CW);
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        h[i][e] = e < left ? ((float)rx[i][e] - mu) * rs : 0.f;
+        d[i][e] = e < left ? (float)rd[i][e] : 0.f;
+      }
+    }
+    if (rb + G < r1) request(r + G);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        if (r < r1) {   // (uniform over the threads of a row; the rows behind the part's end are another part's, or none)
+          dg[i][e] = fmaf(d[i][e], h[i][e], dg[i][e]);
+          db[i][e] += d[i][e];
+        }
+        d[i][e] *= gam[i][e];
+        s += d[i][e];
+        q = fmaf(d[i][e], h[i][e], q);
+      }
+    }
+    if (a.dx == nullptr) continue;
+    s = row_sum<TPR>(s, sm[flip][0]) * inv;
+    q = row_sum<TPR>(q, sm[flip][1]) * inv;
+    if (r < r1) {
+      T* dx = (T*)a.dx + r * a.ld_dx;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int col = t * V + i * CW;
+        if (col < a.D) {
+          typename Lane<T>::vec o;
+#pragma unroll
+          for (int e = 0; e < V; ++e) o[e] = (T)(rs * (d[i][e] - fmaf(h[i][e], q, s)));
+          Lane<T>::store(dx + col, o, a.D - col);
+        }
+      }
+    }
+  }
+  if (a.part == nullptr) return;
+  float* out = a.part + (long)blockIdx.x * 2 * a.D;
+#pragma unroll
+  for (int which = 0; which < 2; ++which) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      if constexpr (G > 1) {
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < V; ++e) fold[g * CW + t * V + e] = which ? db[i][e] : dg[i][e];
+        __syncthreads();
+        for (int c = threadIdx.x; c < CW; c += NB) {
+          float s = 0.f;
+#pragma unroll
+          for (int k = 0; k < G; ++k) s += fold[k * CW + c];
+          if (i * CW + c < a.D) out[(long)which * a.D + i * CW + c] = s;
+        }
+      } else {
+        const int col = t * V + i * CW;
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+          if (col + e < a.D) out[(long)which * a.D + col + e] = which ? db[i][e] : dg[i][e];
+      }
+    }
+  }
 }
 
 // ---- rows of any length: one workgroup per row, the row is walked once per sum
@@ -119,22 +356,34 @@ __global__ __launch_bounds__(NT) void ln_part_kernel(const BwdArgs a) {
   p[a.D + j] = db;
 }
 
-// out[e] = sum over the parts of column e, for the 2 D columns (dgamma | dbeta)
-__global__ __launch_bounds__(NT) void ln_sum_kernel(const float* __restrict__ part, int n_parts, int D, float* __restrict__ dgamma,
-                                                    float* __restrict__ dbeta) {
-  const long e = (long)blockIdx.x * NT + threadIdx.x;
-  if (e >= 2l * D) return;
+// out[e] = sum over the parts of column e, for the 2 D columns (dgamma | dbeta): 32 columns and 32 shares of the parts per workgroup
+constexpr int SUM_NT = 1024;
+__global__ __launch_bounds__(SUM_NT) void ln_sum_kernel(const float* __restrict__ part, int n_parts, int D, float* __restrict__ dgamma,
+                                                        float* __restrict__ dbeta) {
+  __shared__ float sm[32][33];
+  const int c = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const long e = (long)blockIdx.x * 32 + c, E = 2l * D;
   float s = 0.f;
-  for (int p = 0; p < n_parts; ++p) s += part[(long)p * 2 * D + e];
-  float* out = e < D ? dgamma : dbeta;
-  if (out) out[e < D ? e : e - D] = s;
+  if (e < E) {
+#pragma unroll 8
+    for (int p = w; p < n_parts; p += 32) s += part[(long)p * E + e];
+  }
+  sm[w][c] = s;
+  __syncthreads();
+  if (w == 0 && e < E) {
+    float v = 0.f;
+#pragma unroll
+    for (int k = 0; k < 32; ++k) v += sm[k][c];
+    float* out = e < D ? dgamma : dbeta;
+    if (out) out[e < D ? e : e - D] = v;
+  }
 }
 
 // The parts of a backward pass: consecutive rows each.
 int parts_of(long n_rows, int D) {
   if (n_rows <= 0) return 0;
-  const long cap = std::min(512l, std::max(32l, (4l << 20) / D));
-  return (int)std::min((n_rows + 15) / 16, cap);
+  const long cap = std::min(1024l, std::max(32l, (4l << 20) / D));
+  return (int)std::min((n_rows + 7) / 8, cap);
 }
 
 bool known_type(int dtype) { return dtype == EMX_F32 || dtype == EMX_F16 || dtype == EMX_BF16; }
@@ -155,6 +404,49 @@ int by_type(int dtype, F f) {
   return f(0.f);
 }
 
+template <typename T, int TPR, int NV, int U>
+void start_fwd(const FwdArgs& a, hipStream_t st) {
+  constexpr int NB = TPR > NT ? TPR : NT;
+  const long rows = (long)(NB / TPR) * U;
+  hipLaunchKernelGGL((ln_fwd_kernel<T, TPR, NV, U>), dim3((unsigned)((a.n_rows + rows - 1) / rows)), dim3(NB), 0, st, a);
+}
+template <typename T>
+void launch_fwd(const FwdArgs& a, hipStream_t st) {
+  int nv = (a.D + Lane<T>::V - 1) / Lane<T>::V;   // 16-byte vectors of a row
+  if (a.n_rows >= (1l << 31)) nv = 1 << 30;   // (more workgroups than a launch has: the form whose workgroups walk)
+  if (nv <= 8) return start_fwd<T, 8, 1, 4>(a, st);
+  if (nv <= 16) return start_fwd<T, 16, 1, 4>(a, st);
+  if (nv <= 32) return start_fwd<T, 32, 1, 4>(a, st);
+  if (nv <= 64) return start_fwd<T, 64, 1, 4>(a, st);
+  if (nv <= 128) return start_fwd<T, 64, 2, 2>(a, st);
+  if (nv <= 256) return start_fwd<T, 64, 4, 1>(a, st);
+  if (nv <= 512) return start_fwd<T, 256, 2, 1>(a, st);
+  if (nv <= 1024) return start_fwd<T, 256, 4, 1>(a, st);
+  if (nv <= 2048) return start_fwd<T, 1024, 2, 1>(a, st);
+  if (nv <= 4096) return start_fwd<T, 1024, 4, 1>(a, st);
+  hipLaunchKernelGGL(ln_fwd_long_kernel<T>, dim3((unsigned)std::min<long>(a.n_rows, 1 << 20)), dim3(NT), 0, st, a);
+}
+template <typename T, int TPR, int NV>
+bool start_bwd(const BwdArgs& a, hipStream_t st) {
+  hipLaunchKernelGGL((ln_bwd_kernel<T, TPR, NV>), dim3(a.n_parts), dim3(TPR > NT ? TPR : NT), 0, st, a);
+  return true;
+}
+// false: the row is too long for the registers
+template <typename T>
+bool launch_bwd(const BwdArgs& a, hipStream_t st) {
+  const int nv = (a.D + Lane<T>::V - 1) / Lane<T>::V;
+  if (nv <= 8) return start_bwd<T, 8, 1>(a, st);
+  if (nv <= 16) return start_bwd<T, 16, 1>(a, st);
+  if (nv <= 32) return start_bwd<T, 32, 1>(a, st);
+  if (nv <= 64) return start_bwd<T, 64, 1>(a, st);
+  if (nv <= 128) return start_bwd<T, 64, 2>(a, st);
+  if (nv <= 256) return start_bwd<T, 256, 1>(a, st);
+  if (nv <= 512) return start_bwd<T, 256, 2>(a, st);
+  if (nv <= 1024) return start_bwd<T, 512, 2>(a, st);
+  if (nv <= 2048) return start_bwd<T, 1024, 2>(a, st);
+  return false;
+}
+
 }  // namespace
 
 extern "C" {
@@ -172,7 +464,7 @@ int emx_layernorm_fwd(const void* x, int dtype, int64_t n_rows, int D, int64_t l
   EMX_REQUIRE(disjoint_or_same(x, ldx, y, ldy, n_rows, D, size_of(dtype)), "%s: x and y overlap without being the same rows", who);
   const FwdArgs a{x, y, gamma, beta, mean, rstd, n_rows, ldx, ldy, D, eps};
   return by_type(dtype, [&](auto t) {
-    hipLaunchKernelGGL(ln_fwd_long_kernel<decltype(t)>, dim3((unsigned)std::min<int64_t>(n_rows, 1 << 20)), dim3(NT), 0, (hipStream_t)stream, a);
+    launch_fwd<decltype(t)>(a, (hipStream_t)stream);
     return check_launch(who);
   });
 }
@@ -203,6 +495,7 @@ int emx_layernorm_bwd(const void* dy, int64_t ld_dy, const void* x, int64_t ldx,
     const BwdArgs a{dy, x, dx, gamma, mean, rstd, sums ? ws : nullptr, n_rows, ld_dy, ldx, ld_dx, (n_rows + parts - 1) / parts, D, parts};
     const int rc = by_type(dtype, [&](auto t) {
       using T = decltype(t);
+      if (launch_bwd<T>(a, st)) return check_launch(who);
       if (sums) {   // (first: dx may lie where dy or x does)
         hipLaunchKernelGGL(ln_part_kernel<T>, dim3((D + NT - 1) / NT, parts), dim3(NT), 0, st, a);
         const int r = check_launch(who);
@@ -217,7 +510,7 @@ int emx_layernorm_bwd(const void* dy, int64_t ld_dy, const void* x, int64_t ldx,
     if (rc) return rc;
   }
   if (!sums) return EMX_OK;
-  hipLaunchKernelGGL(ln_sum_kernel, dim3((unsigned)((2l * D + NT - 1) / NT)), dim3(NT), 0, st, ws, parts, D, dgamma, dbeta);
+  hipLaunchKernelGGL(ln_sum_kernel, dim3((unsigned)((2l * D + 31) / 32)), dim3(SUM_NT), 0, st, ws, parts, D, dgamma, dbeta);
   return check_launch(who);
 }
 
