@@ -100,6 +100,9 @@ SIGNATURES = {
     "emx_layernorm_fwd": (_i, [_p, _i, _l, _i, _l, _p, _p, _f, _p, _l, _p, _p, _p]),
     "emx_layernorm_ws_floats": (_sz, [_l, _i]),
     "emx_layernorm_bwd": (_i, [_p, _l, _p, _l, _i, _l, _i, _p, _p, _p, _p, _l, _p, _p, _p, _sz, _p]),
+    "emx_orthogonalize_ws_bytes": (_sz, [_p, _i]),
+    "emx_orthogonalize": (_i, [_p, _i, _p, _p, _i, _i, _f, _p, _sz, _p]),
+    "emx_muon_step": (_i, [_p, _i, _p, _p, _i, _l, _p, _f, _f, _i, _f, _i, _f, _p, _sz, _p]),
     "emx_p2p_handle_bytes": (_i, []),
     "emx_p2p_create": (_i, [_i, _i, _l, _i, C.POINTER(_p), _p]),
     "emx_p2p_connect": (_i, [_p, _p]),
@@ -887,6 +890,74 @@ def layernorm_bwd(dy, x, gamma, mean, rstd, dx, dgamma, dbeta, ws=None):
                _vector(gamma, D, x, "gamma"), _vector(mean, n, x, "mean"), _vector(rstd, n, x, "rstd"),
                None if dx is None else dx.data_ptr(), ld_dx, _vector(dgamma, D, x, "dgamma"), _vector(dbeta, D, x, "dbeta"),
                None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel())
+
+
+class Matrix(C.Structure):
+    """Mirror of ``emx_matrix``."""
+
+    _fields_ = [("offset", _l), ("ld", _l), ("rows", _i), ("cols", _i), ("scale", _f)]
+
+
+class MatrixPlan:
+    """The matrices of flat buffers that ``orthogonalize`` / ``muon_step`` work on, and the launches' scratch.
+
+    ``mats``: (offset, rows, cols, row stride, scale of the update) per matrix, offsets in elements.  One plan serves one call at a time
+    (calls on different streams that may overlap need a plan each)."""
+
+    def __init__(self, mats, device="cuda"):
+        self.n = len(mats)
+        self.mats = (Matrix * max(self.n, 1))()
+        self.end = 0            # elements a buffer needs to hold
+        for entry, (offset, rows, cols, ld, scale) in zip(self.mats, mats):
+            entry.offset, entry.ld, entry.rows, entry.cols, entry.scale = int(offset), int(ld), int(rows), int(cols), float(scale)
+            if rows > 0 and cols > 0:
+                self.end = max(self.end, offset + (rows - 1) * (ld if rows > 1 else 0) + cols)
+        nbytes = int(load().emx_orthogonalize_ws_bytes(self.mats, self.n))
+        if nbytes == 0:
+            raise EmxError(f"MatrixPlan: {load().emx_last_error().decode()}")
+        self.ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        self._args = (C.addressof(self.mats), self.n)
+        self._ws_args = (self.ws.data_ptr(), nbytes)
+
+    @classmethod
+    def of_layers(cls, layers, device="cuda"):
+        """The kernels of Dense layers (``NetLayout.layers``: [n_in, n_out] at ``w_off``); scale sqrt(max(1, n_out / n_in)), which gives the update
+        of every layer the same effect on its output's root mean square."""
+        return cls([(l.w_off, l.n_in, l.n_out, l.n_out, max(1.0, l.n_out / l.n_in) ** 0.5) for l in layers], device)
+
+    def _flat(self, t, what, slices=1, stride=0) -> int:
+        """the address of a contiguous buffer that holds every matrix (``slices`` times, ``stride`` apart)"""
+        _like(t, self.ws, what)
+        if not t.is_contiguous():
+            raise EmxError(f"{what}: a contiguous buffer expected, got strides {t.stride()}")
+        if t.numel() < self.end + (slices - 1) * stride:
+            raise EmxError(f"{what}: {t.numel()} elements, the matrices reach to {self.end + (slices - 1) * stride}")
+        return t.data_ptr()
+
+
+def orthogonalize(plan: MatrixPlan, g, out, steps: int = 5, eps: float = 1e-7):
+    """The matrices of ``out`` <- those of ``g`` orthogonalised (include/emx.h: emx_orthogonalize); flat buffers of one type (float32 / float16 /
+    bfloat16) and any shape; ``out`` may be ``g``."""
+    code = _element_type(g, "g")
+    if out.dtype != g.dtype:
+        raise EmxError(f"out: {g.dtype} like g expected, got {out.dtype}")
+    _on_device(plan.ws.device, load().emx_orthogonalize, "emx_orthogonalize", *plan._args, plan._flat(g, "g"), plan._flat(out, "out"), code, int(steps),
+               float(eps), *plan._ws_args)
+
+
+def muon_step(plan: MatrixPlan, w, g, momentum_buffer, lr, momentum: float = 0.95, nesterov: bool = True, weight_decay: float = 0.0, steps: int = 5,
+              eps: float = 1e-7):
+    """One optimizer step on the matrices of the flat float32 buffers ``w`` and ``momentum_buffer`` (both updated).  ``g``: the gradient, or --
+    [n_slices, n] -- parts whose sum it is (what ``mlp_wgrad`` leaves).  Biases and everything else between the matrices stay as they are."""
+    for t, what in ((w, "w"), (g, "g"), (momentum_buffer, "momentum_buffer")):
+        if t.dtype != torch.float32:
+            raise EmxError(f"{what}: float32 expected, got {t.dtype}")
+    slices, stride = g.shape if g.dim() == 2 else (1, 0)
+    if slices > 1 and stride < plan.end:
+        raise EmxError(f"g: slices of {stride} elements, the matrices reach to {plan.end}")
+    _on_device(plan.ws.device, load().emx_muon_step, "emx_muon_step", *plan._args, plan._flat(w, "w"), plan._flat(g, "g", slices, stride), slices, stride,
+               plan._flat(momentum_buffer, "momentum_buffer"), float(lr), float(momentum), int(bool(nesterov)), float(weight_decay), int(steps), float(eps),
+               *plan._ws_args)
 
 
 def colmean(x, out):

@@ -1,0 +1,430 @@
+// Orthogonalised matrix updates (gfx950): the matrices of a flat buffer driven towards their nearest (semi-)orthogonal ones by an odd
+// polynomial iteration -- matrix products only -- and the optimizer step that uses them.
+//
+//   X_0 = G / (|G|_F + eps)    (G transposed where it has more rows than columns, so that X is M x N with M <= N)
+//   A = X X^T,  P = a I + b A + c A^2,  X <- P X       `steps` times; (a, b, c) = (3.4445, -4.7750, 2.0315)
+//
+// A singular value s of X goes to s (a + b s^2 + c s^4): that polynomial maps [0, 1] into [0, 1.2024] and [0, 1.2024] into itself, and
+// multiplies the small ones by up to 3.4, so after five steps those above ~1e-2 lie around one.  Hence the bounds every stored value
+// obeys, whatever G is: |X| <= 1.21, |A| <= 1.45, |P| <= 3.45.
+//
+// Arithmetic: as the dense layers', every float32 product is THREE f16 matrix instructions on operands split into two f16 planes (hi = f16(v),
+// lo = f16(v - hi): 22 bits), accumulated in float32.  The bounds above make ONE fixed scale of 2^14 enough for X, A and P (|P| 2^14 <= 56.5e3
+// < 65504; what is lost below is 2^-24 2^-14 of the matrix' norm).  The norm is summed in 64 bits: an error of its scale is the one that
+// the iteration turns into an error of every singular value.
+//
+// Layout of an operand (X, X^T, A, P): blocks of 32 rows x 32 k; a block is two K-steps of 16, each a hi and a lo PIECE of 1 KB -- what one
+// v_mfma_f32_32x32x16_f16 reads: lane l holds row l % 32, k = 8 (l / 32) .. + 7.  The accumulators of such an instruction -- lane l: column
+// l % 32, rows 8 q + 4 (l / 32) + r -- are four consecutive k of an operand whose ROWS are the product's columns: a product writes its
+// transpose in operand layout straight from registers.  M and N are padded to 32 with zeros, which stay zero.
+#include <algorithm>
+#include <cstdint>
+#include <vector>
+
+#include "emx_common.h"
+
+namespace {
+
+using namespace emx;
+
+constexpr int NT = 256;
+constexpr int MAX_TABLE = 64;                 // matrices of one launch
+constexpr int MAX_PARTS = 256;                // shares of a matrix' sum of squares
+constexpr float CA = 3.4445f, CB = -4.7750f, CC = 2.0315f;
+constexpr float SC = 16384.f, RSC = 1.f / 16384.f;
+constexpr int BLK = 4096;                     // bytes of an operand's 32 x 32 block
+
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef _Float16 half4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+struct Mat {
+  long off, ld;      // first element and row stride in the flat tensors
+  long ws;           // the matrix' scratch, from the workspace's begin
+  int rows, cols;
+  float scale;       // of the update
+  int begin;         // the launch's first workgroup for this matrix
+};
+struct Table {
+  int n;
+  Mat m[MAX_TABLE];
+};
+
+// the scratch of one matrix
+struct Scratch {
+  int M, N, Mb, Nb;
+  bool turned;
+  char *x, *t0, *t1, *a, *p;
+  double* part;
+  __host__ __device__ Scratch(int rows, int cols, char* base) {
+    turned = rows > cols;
+    M = turned ? cols : rows, N = turned ? rows : cols;
+    Mb = (M + 31) / 32, Nb = (N + 31) / 32;
+    const long xn = (long)Mb * Nb * BLK, an = (long)Mb * Mb * BLK;
+    part = reinterpret_cast<double*>(base);
+    x = base + MAX_PARTS * 8;
+    t0 = x + xn, t1 = t0 + xn, a = t1 + xn, p = a + an;
+  }
+  __host__ static size_t bytes(int rows, int cols) {
+    const Scratch s(rows, cols, nullptr);
+    return MAX_PARTS * 8 + ((size_t)3 * s.Mb * s.Nb + (size_t)2 * s.Mb * s.Mb) * BLK;
+  }
+};
+__host__ __device__ inline int parts_of(long n) { return (int)(n <= 4096l * MAX_PARTS ? (n + 4095) / 4096 : MAX_PARTS); }
+
+// the matrix a workgroup belongs to, and its number inside it
+__device__ __forceinline__ int find(const Table& t, int block, int& inside) {
+  int lo = 0, hi = t.n - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (t.m[mid].begin <= block) lo = mid;
+    else hi = mid - 1;
+  }
+  inside = block - t.m[lo].begin;
+  return lo;
+}
+
+struct StepArgs {
+  const void* g;       // gradients: flat buffer, or (slices) the parts of their sum
+  void* out;           // orthogonalize: the result's flat buffer
+  float *w, *mom;      // optimizer step
+  char* ws;
+  long slice_stride;
+  int n_slices, nesterov;
+  float beta, keep, lr, eps;    // keep = 1 - lr weight_decay
+};
+
+// ---- 1: the sum of squares in shares; the optimizer step also forms its update's direction u here
+template <typename T, bool MUON>
+__global__ __launch_bounds__(NT) void ns_norm_kernel(const Table tab, const StepArgs a) {
+  __shared__ double sm[NT / 64];
+  int part;
+  const Mat m = tab.m[find(tab, blockIdx.x, part)];
+  const Scratch s(m.rows, m.cols, a.ws + m.ws);
+  const unsigned total = (unsigned)m.rows * m.cols, cols = m.cols;
+  const int parts = parts_of(total);
+  const unsigned chunk = (total + parts - 1) / parts;
+  const unsigned e0 = part * chunk, e1 = min(e0 + chunk, total);
+  float* const u_out = reinterpret_cast<float*>(s.t1);
+  double sum = 0.0;
+  for (unsigned e = e0 + threadIdx.x; e < e1; e += NT) {
+    const unsigned r = e / cols;
+    const long at = m.off + r * m.ld + (e - r * cols);
+    float u;
+    if constexpr (MUON) {
+      const float* g = (const float*)a.g + at;
+      float v = g[0];
+      for (int k = 1; k < a.n_slices; ++k) v += g[k * a.slice_stride];
+      const float mo = fmaf(a.beta, a.mom[at], v);
+      a.mom[at] = mo;
+      u = a.nesterov ? fmaf(a.beta, mo, v) : mo;
+      u_out[e] = u;
+    } else {
+      u = (float)((const T*)a.g)[at];
+    }
+    sum = fma((double)u, (double)u, sum);
+  }
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) sum += __shfl_xor(sum, d);
+  if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = sum;
+  __syncthreads();
+  if (threadIdx.x == 0) s.part[part] = (sm[0] + sm[1]) + (sm[2] + sm[3]);
+}
+
+// eight values of a row as the hi and lo units of an operand
+__device__ __forceinline__ void split_unit(const float (&v)[8], char* hi, char* lo) {
+  half8 h, l;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    h[e] = (_Float16)v[e];
+    l[e] = (_Float16)(v[e] - (float)h[e]);
+  }
+  *reinterpret_cast<half8*>(hi) = h;
+  *reinterpret_cast<half8*>(lo) = l;
+}
+
+// ---- 2: X_0 and its transpose as operands: a workgroup per 64 x 64 of X
+template <typename T, bool MUON>
+__global__ __launch_bounds__(NT) void ns_split_kernel(const Table tab, const StepArgs a) {
+  __shared__ float tile[64][65];
+  __shared__ double sm[NT / 64];
+  int inside;
+  const Mat m = tab.m[find(tab, blockIdx.x, inside)];
+  const Scratch s(m.rows, m.cols, a.ws + m.ws);
+  const int tid = threadIdx.x;
+  const int tn = (s.Nb + 1) / 2, ti = inside / tn, tj = inside - ti * tn;
+  double sum = tid < parts_of((long)m.rows * m.cols) ? s.part[tid] : 0.0;
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) sum += __shfl_xor(sum, d);
+  if ((tid & 63) == 0) sm[tid >> 6] = sum;
+  __syncthreads();
+  const double f = (double)SC / (sqrt((sm[0] + sm[1]) + (sm[2] + sm[3])) + (double)a.eps);
+  const float* const u_in = reinterpret_cast<const float*>(s.t1);
+  // the tile as it is stored: rows (r0 ..), columns (c0 ..) of G
+  const int r0 = 64 * (s.turned ? tj : ti), c0 = 64 * (s.turned ? ti : tj);
+  for (int e = tid; e < 64 * 64; e += NT) {
+    const int r = r0 + (e >> 6), c = c0 + (e & 63);
+    float v = 0.f;
+    if (r < m.rows && c < m.cols) v = MUON ? u_in[(long)r * m.cols + c] : (float)((const T*)a.g)[m.off + r * m.ld + c];
+    v = (float)((double)v * f);
+    tile[s.turned ? e & 63 : e >> 6][s.turned ? e >> 6 : e & 63] = v;
+  }
+  __syncthreads();
+  // 4 blocks x 2 K-steps x 64 lanes units of X, as many of X^T
+  for (int e = tid; e < 1024; e += NT) {
+    const int lane = e & 63, ks = (e >> 6) & 1, bj = (e >> 7) & 1, bi = (e >> 8) & 1, tr = e >> 9;
+    const int ib = 2 * ti + bi, jb = 2 * tj + bj;
+    if (ib >= s.Mb || jb >= s.Nb) continue;
+    const int row = lane & 31, k = 16 * ks + 8 * (lane >> 5);
+    float v[8];
+#pragma unroll
+    for (int q = 0; q < 8; ++q) v[q] = tr ? tile[32 * bi + k + q][32 * bj + row] : tile[32 * bi + row][32 * bj + k + q];
+    char* base = (tr ? s.t0 + ((long)jb * s.Mb + ib) * BLK : s.x + ((long)ib * s.Nb + jb) * BLK) + ks * 2048 + lane * 16;
+    split_unit(v, base, base + 1024);
+  }
+}
+
+// ---- 3: the products.  KIND 0: A = X X^T; 1: P = a I + b A + c A A^T; 2: X <- P X; 3: the last step's X, written out
+enum { GRAM = 0, POLY = 1, NEXT = 2, LAST = 3 };
+__device__ __forceinline__ void triangle(int t, int nb, int& ti, int& tj) {   // row-major over ti <= tj
+  ti = (int)((2.f * nb + 1.f - sqrtf((2.f * nb + 1.f) * (2.f * nb + 1.f) - 8.f * t)) * 0.5f);
+  while (ti > 0 && ti * nb - ti * (ti - 1) / 2 > t) --ti;
+  while ((ti + 1) * nb - (ti + 1) * ti / 2 <= t) ++ti;
+  tj = ti + t - (ti * nb - ti * (ti - 1) / 2);
+}
+
+template <int KIND, typename T, bool MUON>
+__global__ __launch_bounds__(NT) void ns_product_kernel(const Table tab, const StepArgs a, const int odd) {
+  int inside;
+  const Mat m = tab.m[find(tab, blockIdx.x, inside)];
+  const Scratch s(m.rows, m.cols, a.ws + m.ws);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lr = lane & 31, h = lane >> 5;
+  char *const t_in = odd ? s.t1 : s.t0, *const t_out = odd ? s.t0 : s.t1;
+  int ti, tj;
+  if constexpr (KIND <= POLY) {
+    triangle(inside, (s.Mb + 1) / 2, ti, tj);
+  } else {
+    const int tn = (s.Nb + 1) / 2;
+    ti = inside / tn, tj = inside - ti * tn;
+  }
+  const int ib = 2 * ti + (wave >> 1), jb = 2 * tj + (wave & 1);     // this wave's 32 x 32 block of the product
+  const int Jb = KIND <= POLY ? s.Mb : s.Nb, Kb = KIND == GRAM ? s.Nb : s.Mb;
+  if (ib >= s.Mb || jb >= Jb) return;
+  const char* U = (KIND == GRAM ? s.x : KIND == POLY ? s.a : s.p) + (long)ib * Kb * BLK + lane * 16;
+  const char* V = (KIND == GRAM ? s.x : KIND == POLY ? s.a : t_in) + (long)jb * Kb * BLK + lane * 16;
+  // Long sums in two levels: an accumulator takes 256 k (48 additions), then joins the sum.  (One chain over 4096 k rounds 768 times: 8e-6 of
+  // the result where float32 in blocks is off by 1e-6.)
+  f32x16 sum, acc, zero;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) sum[i] = zero[i] = 0.f;
+  for (int k0 = 0; k0 < 2 * Kb; k0 += 16) {
+    const int k1 = min(k0 + 16, 2 * Kb);
+    acc = zero;
+    for (int k = k0; k < k1; ++k) {
+      const half8 uh = *reinterpret_cast<const half8*>(U + k * 2048l), ul = *reinterpret_cast<const half8*>(U + k * 2048l + 1024);
+      const half8 vh = *reinterpret_cast<const half8*>(V + k * 2048l), vl = *reinterpret_cast<const half8*>(V + k * 2048l + 1024);
+      acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(uh, vl, acc, 0, 0, 0);   // small products first
+      acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(ul, vh, acc, 0, 0, 0);
+      acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(uh, vh, acc, 0, 0, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) sum[i] += acc[i];
+  }
+  acc = sum;
+  // acc[4 q + r]: row 32 ib + 8 q + 4 h + r, column 32 jb + lr
+  if constexpr (KIND == LAST) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int row = 32 * ib + 8 * (i >> 2) + 4 * h + (i & 3), col = 32 * jb + lr;
+      if (row < s.M && col < s.N) {
+        const long at = m.off + (s.turned ? col * m.ld + row : row * m.ld + col);
+        const float v = acc[i] * (RSC * RSC);
+        if constexpr (MUON) a.w[at] = fmaf(a.w[at], a.keep, -(a.lr * m.scale) * v);
+        else ((T*)a.out)[at] = (T)v;
+      }
+    }
+  } else {
+    char* const O = KIND == GRAM ? s.a : KIND == POLY ? s.p : t_out;
+    const int rows_b = KIND == NEXT ? s.Mb : s.Mb;                   // blocks along k of the transposed result
+    char* const direct = O + ((long)jb * rows_b + ib) * BLK;         // rows: the product's columns; k: its rows
+    char* const other = KIND == NEXT ? s.x + ((long)ib * s.Nb + jb) * BLK : ib != jb ? O + ((long)ib * s.Mb + jb) * BLK : nullptr;
+    const bool both = KIND == NEXT || ti != tj;                      // (a diagonal tile's four blocks are all computed)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int at = (q >> 1) * 2048 + ((q & 1) * 32 + lr) * 16 + h * 8;
+      float v[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) v[r] = acc[4 * q + r] * RSC;
+      if constexpr (KIND == POLY) {
+        const char* am = s.a + ((long)jb * s.Mb + ib) * BLK + at;    // A is symmetric: the same four of its transpose
+        const half4 ah = *reinterpret_cast<const half4*>(am), al = *reinterpret_cast<const half4*>(am + 1024);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          v[r] = fmaf(CC, v[r], CB * ((float)ah[r] + (float)al[r]));
+          if (ib == jb && 8 * q + 4 * h + r == lr && 32 * ib + lr < s.M) v[r] += CA * SC;
+        }
+      }
+      half4 hi, lo;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        hi[r] = (_Float16)v[r];
+        lo[r] = (_Float16)(v[r] - (float)hi[r]);
+      }
+      *reinterpret_cast<half4*>(direct + at) = hi;
+      *reinterpret_cast<half4*>(direct + at + 1024) = lo;
+      if (both) {
+        // rows: the product's rows; k: its columns
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int b = (lr >> 4) * 2048 + (((lr >> 3) & 1) * 32 + 8 * q + 4 * h + r) * 16 + (lr & 7) * 2;
+          *reinterpret_cast<_Float16*>(other + b) = hi[r];
+          *reinterpret_cast<_Float16*>(other + b + 1024) = lo[r];
+        }
+      }
+    }
+  }
+}
+
+// ---- host side
+int check_matrices(const char* who, const emx_matrix* mats, int n) {
+  EMX_REQUIRE(n >= 0 && (n == 0 || mats), "%s: %d matrices", who, n);
+  struct Span { int64_t a, b, ld; int cols; };
+  std::vector<Span> spans;
+  for (int i = 0; i < n; ++i) {
+    const emx_matrix& m = mats[i];
+    EMX_REQUIRE(m.rows >= 0 && m.cols >= 0 && m.offset >= 0, "%s: matrix %d: %d x %d at %lld", who, i, m.rows, m.cols, (long long)m.offset);
+    if (m.rows == 0 || m.cols == 0) continue;
+    if (m.rows > EMX_MATRIX_MAX_SIDE || m.cols > EMX_MATRIX_MAX_SIDE)
+      return fail(EMX_EUNSUPPORTED, "%s: matrix %d: %d x %d (at most %d a side)", who, i, m.rows, m.cols, EMX_MATRIX_MAX_SIDE);
+    EMX_REQUIRE(m.rows == 1 || m.ld >= m.cols, "%s: matrix %d: row stride %lld of %d columns", who, i, (long long)m.ld, m.cols);
+    EMX_REQUIRE(m.rows == 1 || m.ld <= (int64_t)1 << 40, "%s: matrix %d: row stride %lld", who, i, (long long)m.ld);
+    spans.push_back({m.offset, m.offset + (m.rows == 1 ? 0 : (m.rows - 1) * m.ld) + m.cols, m.rows == 1 ? 0 : m.ld, m.cols});
+  }
+  // every element is updated by ONE matrix: spans apart, or columns side by side in rows of the same length
+  std::sort(spans.begin(), spans.end(), [](const Span& x, const Span& y) { return x.a < y.a; });
+  for (size_t i = 0; i < spans.size(); ++i)
+    for (size_t j = i + 1; j < spans.size() && spans[j].a < spans[i].b; ++j) {
+      const Span &x = spans[i], &y = spans[j];
+      const int64_t ld = x.ld ? x.ld : y.ld, shift = ld ? (y.a - x.a) % ld : 0;
+      const bool beside = ld && (!x.ld || !y.ld || x.ld == y.ld) && shift >= x.cols && shift + y.cols <= ld;
+      EMX_REQUIRE(beside, "%s: matrices at %lld and %lld overlap", who, (long long)x.a, (long long)y.a);
+    }
+  return EMX_OK;
+}
+
+bool empty(const emx_matrix& m) { return m.rows == 0 || m.cols == 0; }
+
+// the matrices of one launch group: at most MAX_TABLE of them from index i on; returns the index behind them
+int group(const emx_matrix* mats, int n, int i, Table& t, size_t& bytes) {
+  t.n = 0, bytes = 0;
+  for (; i < n && t.n < MAX_TABLE; ++i) {
+    const emx_matrix& m = mats[i];
+    if (empty(m)) continue;
+    t.m[t.n++] = Mat{m.offset, m.rows == 1 ? m.cols : m.ld, (long)bytes, m.rows, m.cols, m.scale, 0};
+    bytes += Scratch::bytes(m.rows, m.cols);
+  }
+  return i;
+}
+
+template <typename F>
+long number(Table& t, F blocks) {   // hands out the workgroups of a launch
+  long at = 0;
+  for (int i = 0; i < t.n; ++i) {
+    t.m[i].begin = (int)at;
+    at += blocks(t.m[i], Scratch(t.m[i].rows, t.m[i].cols, nullptr));
+  }
+  return at;
+}
+
+template <typename T, bool MUON>
+int run(const char* who, const emx_matrix* mats, int n, const StepArgs& a, int steps, hipStream_t st) {
+  for (int i = 0; i < n;) {
+    Table t;
+    size_t bytes;
+    i = group(mats, n, i, t, bytes);
+    if (t.n == 0) break;
+    auto half = [](int b) { return (long)(b + 1) / 2; };
+    const auto parts = [](const Mat& m, const Scratch&) { return (long)parts_of((long)m.rows * m.cols); };
+    const auto full = [&](const Mat&, const Scratch& s) { return half(s.Mb) * half(s.Nb); };
+    const auto upper = [&](const Mat&, const Scratch& s) { return half(s.Mb) * (half(s.Mb) + 1) / 2; };
+    int rc;
+    auto go = [&](auto kernel, long blocks, auto... more) {
+      EMX_REQUIRE(blocks < (1l << 31), "%s: %ld workgroups", who, blocks);
+      hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(NT), 0, st, t, a, more...);
+      return check_launch(who);
+    };
+    if ((rc = go(ns_norm_kernel<T, MUON>, number(t, parts)))) return rc;
+    if ((rc = go(ns_split_kernel<T, MUON>, number(t, full)))) return rc;
+    for (int k = 0; k < steps; ++k) {
+      const long up = number(t, upper);
+      if ((rc = go(ns_product_kernel<GRAM, T, MUON>, up, k & 1))) return rc;
+      if ((rc = go(ns_product_kernel<POLY, T, MUON>, up, k & 1))) return rc;
+      const long all = number(t, full);
+      if ((rc = k + 1 < steps ? go(ns_product_kernel<NEXT, T, MUON>, all, k & 1) : go(ns_product_kernel<LAST, T, MUON>, all, k & 1))) return rc;
+    }
+  }
+  return EMX_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t emx_orthogonalize_ws_bytes(const emx_matrix* mats, int n_mats) {
+  if (check_matrices("emx_orthogonalize_ws_bytes", mats, n_mats)) return 0;
+  size_t most = 16;
+  for (int i = 0; i < n_mats;) {
+    Table t;
+    size_t bytes;
+    i = group(mats, n_mats, i, t, bytes);
+    most = std::max(most, bytes);
+  }
+  return most;
+}
+
+int emx_orthogonalize(const emx_matrix* mats, int n_mats, const void* g, void* out, int dtype, int steps, float eps, void* ws, size_t ws_bytes,
+                      emx_stream_t stream) {
+  const char* who = "emx_orthogonalize";
+  int rc = check_matrices(who, mats, n_mats);
+  if (rc) return rc;
+  EMX_REQUIRE(dtype == EMX_F32 || dtype == EMX_F16 || dtype == EMX_BF16, "%s: element type %d", who, dtype);
+  EMX_REQUIRE(steps >= 1 && steps <= EMX_ORTHOGONALIZE_MAX_STEPS, "%s: %d steps", who, steps);
+  EMX_REQUIRE(eps > 0.f && std::isfinite(eps), "%s: eps %g", who, (double)eps);
+  if (std::all_of(mats, mats + n_mats, empty)) return EMX_OK;
+  EMX_REQUIRE(g && out, "%s: g and out are needed", who);
+  if (!ws || ws_bytes < emx_orthogonalize_ws_bytes(mats, n_mats) || ((uintptr_t)ws & 15))
+    return fail(EMX_EWORKSPACE, "%s: workspace of %zu bytes at %p, %zu needed on a 16-byte boundary", who, ws_bytes, ws,
+                emx_orthogonalize_ws_bytes(mats, n_mats));
+  StepArgs a{};
+  a.g = g, a.out = out, a.ws = (char*)ws, a.n_slices = 1, a.eps = eps;
+  hipStream_t st = (hipStream_t)stream;
+  if (dtype == EMX_F16) return run<_Float16, false>(who, mats, n_mats, a, steps, st);
+  if (dtype == EMX_BF16) return run<__bf16, false>(who, mats, n_mats, a, steps, st);
+  return run<float, false>(who, mats, n_mats, a, steps, st);
+}
+
+int emx_muon_step(const emx_matrix* mats, int n_mats, float* w, const float* g, int n_slices, int64_t slice_stride, float* momentum, float lr,
+                  float beta, int nesterov, float weight_decay, int steps, float eps, void* ws, size_t ws_bytes, emx_stream_t stream) {
+  const char* who = "emx_muon_step";
+  int rc = check_matrices(who, mats, n_mats);
+  if (rc) return rc;
+  EMX_REQUIRE(n_slices >= 1 && (n_slices == 1 || slice_stride >= 0), "%s: %d slices, stride %lld", who, n_slices, (long long)slice_stride);
+  EMX_REQUIRE(std::isfinite(lr) && beta >= 0.f && beta < 1.f && std::isfinite(weight_decay), "%s: lr %g, momentum %g, weight decay %g", who,
+              (double)lr, (double)beta, (double)weight_decay);
+  EMX_REQUIRE(steps >= 1 && steps <= EMX_ORTHOGONALIZE_MAX_STEPS, "%s: %d steps", who, steps);
+  EMX_REQUIRE(eps > 0.f && std::isfinite(eps), "%s: eps %g", who, (double)eps);
+  for (int i = 0; i < n_mats; ++i) EMX_REQUIRE(std::isfinite(mats[i].scale), "%s: matrix %d: scale %g", who, i, (double)mats[i].scale);
+  if (std::all_of(mats, mats + n_mats, empty)) return EMX_OK;
+  EMX_REQUIRE(w && g && momentum, "%s: w, g and momentum are needed", who);
+  EMX_REQUIRE(w != g && w != momentum && momentum != g, "%s: w, g and momentum have to be three buffers", who);
+  if (!ws || ws_bytes < emx_orthogonalize_ws_bytes(mats, n_mats) || ((uintptr_t)ws & 15))
+    return fail(EMX_EWORKSPACE, "%s: workspace of %zu bytes at %p, %zu needed on a 16-byte boundary", who, ws_bytes, ws,
+                emx_orthogonalize_ws_bytes(mats, n_mats));
+  StepArgs a{};
+  a.g = g, a.w = w, a.mom = momentum, a.ws = (char*)ws, a.slice_stride = slice_stride, a.n_slices = n_slices, a.nesterov = nesterov != 0;
+  a.beta = beta, a.keep = (float)(1.0 - (double)lr * weight_decay), a.lr = lr, a.eps = eps;
+  return run<float, true>(who, mats, n_mats, a, steps, (hipStream_t)stream);
+}
+
+}  // extern "C"

@@ -593,6 +593,38 @@ int emx_layernorm_bwd(const void* dy, int64_t ld_dy, const void* x, int64_t ldx,
                       emx_stream_t stream);
 
 /* ------------------------------------------------------------------------------------------------ *
+ * Orthogonalised matrix updates (csrc/muon.hip): an optimizer for the KERNELS of a network beside emx_adam_step* above (which stays the one
+ * for biases, norms' weights and whatever is no matrix).  The reference's only optimizer is Adam (autoencoder.py:741-743).
+ *   orth(G): X = G / (|G|_F + eps); `steps` times  A = X X^T, X <- a X + (b A + c A A) X  with (a, b, c) = (3.4445, -4.7750, 2.0315)
+ *   (X^T in X's place where G has more rows than columns).  All singular values of G above ~1e-2 of its norm come out around 1 (0.68 .. 1.2).
+ *   emx_matrix: a matrix of the flat buffers the call is given: rows x cols elements from `offset` on, row stride `ld` >= cols; `scale` is
+ *     the factor of its update in emx_muon_step.  Matrices of a call may not share elements; rows or cols may be 0 (nothing is done).
+ *   emx_orthogonalize: out <- orth(g) for every matrix; g and out (EMX_F32 / EMX_F16 / EMX_BF16, the same offsets in both) may be the same
+ *     buffer.  What lies between the matrices is neither read nor written.
+ *   emx_muon_step, float32:  G = sum over n_slices of g[s * slice_stride + .] in order (the weight-gradient partials of emx_mlp_wgrad, or one
+ *     gradient);  momentum <- beta momentum + G;  U = nesterov ? G + beta momentum : momentum;  w <- w (1 - lr weight_decay) - lr scale orth(U).
+ *     0 <= beta < 1.  The operand store of the dense-layer launches is NOT rewritten: emx_mlp_mirror afterwards.
+ *   Products run on operands of 22 bits with float32 accumulation; an infinity or a NaN in a matrix makes its result NaN, a matrix of
+ *   zeros stays zero.  1 <= steps <= EMX_ORTHOGONALIZE_MAX_STEPS, sides up to EMX_MATRIX_MAX_SIDE (more: EMX_EUNSUPPORTED), eps > 0.
+ *   ws: emx_orthogonalize_ws_bytes(mats, n_mats) bytes of scratch on a 16-byte boundary (0 from that function: the matrices are refused); its
+ *   contents mean nothing between calls, calls that may run at the same time need one each.  `mats` is host memory, read during the call.
+ * ------------------------------------------------------------------------------------------------ */
+#define EMX_MATRIX_MAX_SIDE 32768
+#define EMX_ORTHOGONALIZE_MAX_STEPS 64
+typedef struct {
+  int64_t offset;
+  int64_t ld;
+  int rows;
+  int cols;
+  float scale;
+} emx_matrix;
+size_t emx_orthogonalize_ws_bytes(const emx_matrix* mats, int n_mats);
+int emx_orthogonalize(const emx_matrix* mats, int n_mats, const void* g, void* out, int dtype, int steps, float eps, void* ws, size_t ws_bytes,
+                      emx_stream_t stream);
+int emx_muon_step(const emx_matrix* mats, int n_mats, float* w, const float* g, int n_slices, int64_t slice_stride, float* momentum, float lr,
+                  float beta, int nesterov, float weight_decay, int steps, float eps, void* ws, size_t ws_bytes, emx_stream_t stream);
+
+/* ------------------------------------------------------------------------------------------------ *
  * ADC path (AngleDihedralCartesianEncoderMap): back-mapping and per-frame pair distances
  * ------------------------------------------------------------------------------------------------ */
 /* K8  column mean over the batch: out[k] = mean_b x[b,k]     MeanAngles / mean bond lengths, layers.py:971,1153-1161 */

@@ -1,0 +1,335 @@
+"""Orthogonalised updates through the C ABI against the iteration in 64 bits.
+
+Tolerance.  A product of operands split into 22 bits carries at most 2^-22 (lost by the splitting) + 2^-22 (the product of the two low planes, left out)
+of the magnitudes added, the float32 sums about as much again: 2^-20 relative per step of the iteration is what STEP below allows for its three products
+together.  An error made in X_k reaches the result at most 3.4445^(steps - k) times as large (the derivative of s (a + b s^2 + c s^4) is largest at 0), and
+|X_k|_F <= min(3.4445^k, 1.2024 sqrt(M)) as |X_0|_F <= 1.  The sum over k is the bound of the result's error in the Frobenius norm -- and of every entry's.
+A second bound is relative to the same iteration in float32 (24-bit operands, so at most 2^2 times as exact): four times its error, or 4e-6.  It takes the
+roundings of a product's terms for independent, as those of random matrices are.  In a matrix of equal entries they are ONE error n times over, and float32
+may have the luck of a small one: with s = 1, s' = a s + b s^3 + c s^5 = 0.701 is a difference of terms that add up to 10.25, A is off by up to 2^-21 and A A
+by 3 x 2^-21, so a step is off by (4.775 + 3 x 2.0315 + 10.25) 2^-21 = 1.0e-5 where four times float32's may be 7e-6.  `test_spectra` holds such matrices
+to the first bound alone, which is proved for any matrix.
+Results of 16 bits are rounded once more.
+"""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+STEP = 2.0 ** -20
+ABC = (3.4445, -4.7750, 2.0315)
+TYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from encodermap_amd import _lib
+
+    _lib.require_gpu()
+    return _lib
+
+
+def iterate(g, steps=5, eps=1e-7):
+    a, b, c = ABC
+    x = g.t() if g.shape[0] > g.shape[1] else g
+    x = x / (x.square().sum().sqrt() + eps)
+    for _ in range(steps):
+        gram = x @ x.t()
+        x = a * x + (b * gram + c * (gram @ gram)) @ x
+    return x.t() if g.shape[0] > g.shape[1] else x
+
+
+def bound(rows, cols, steps):
+    side = min(rows, cols)
+    return STEP * sum(ABC[0] ** (steps - k) * min(ABC[0] ** k, 1.2024 * math.sqrt(side)) for k in range(steps + 1))
+
+
+def check(got, g, steps=5, eps=1e-7, what="", independent=True):
+    want, single = iterate(g.double(), steps, eps), iterate(g.float(), steps, eps)
+    e = torch.finfo(got.dtype).eps / 2 if got.dtype != torch.float32 else 0.0
+    assert torch.isfinite(got).all(), what
+    err = (got.double() - want).abs()
+    rounding = e * want.abs() * (1 + 1e-2) + (torch.finfo(got.dtype).smallest_normal * e if e else 0.0)
+    limit = bound(*g.shape, steps)
+    assert (err <= rounding + limit).all(), f"{what}: an entry is off by {(err - rounding).max().item():.3g}, {limit:.3g} allowed"
+    norm = want.norm().item()
+    off, plain = (err - rounding).clamp_min(0).norm().item(), (single.double() - want).norm().item()
+    assert off <= (min(limit, max(4 * plain, 4e-6 * norm)) if independent else limit), f"{what}: {off / max(norm, 1e-300):.3g} off, float32 {plain / max(norm, 1e-300):.3g}"
+
+
+def gradient(rows, cols, seed, rank=16, floor=0.1):
+    gen = torch.Generator("cuda").manual_seed(seed)
+    r = min(rank, rows, cols)
+    u = torch.randn(rows, r, generator=gen, device="cuda") * torch.linspace(0, -3, r, device="cuda").exp()
+    return (u @ torch.randn(r, cols, generator=gen, device="cuda") / math.sqrt(r) + floor * torch.randn(rows, cols, generator=gen, device="cuda")) * 0.05
+
+
+def lay_out(shapes, pad=0, gap=3):
+    """(plan entries, length): matrices one after the other, `gap` elements between them, rows `pad` longer than they are"""
+    out, at = [], 1
+    for rows, cols in shapes:
+        out.append((at, rows, cols, cols + pad, 1.0 + 0.25 * (len(out) % 3)))
+        at += rows * (cols + pad) + gap
+    return out, at
+
+
+def views(flat, entries):
+    return [flat[at:at + (rows - 1) * ld + cols].as_strided((rows, cols), (ld, 1)) for at, rows, cols, ld, _ in entries]
+
+
+def orthogonalize(lib, shapes, kind="f32", pad=0, steps=5, seed=0, in_place=False, make=gradient, independent=True):
+    dtype = TYPES[kind]
+    entries, n = lay_out(shapes, pad)
+    flat = torch.full((n,), 0.5, device="cuda").to(dtype)
+    for i, v in enumerate(views(flat, entries)):
+        v.copy_(make(*v.shape, seed + i))
+    out = flat.clone() if in_place else torch.full((n,), 0.25, device="cuda").to(dtype)
+    before = out.clone()
+    plan = lib.MatrixPlan(entries)
+    lib.orthogonalize(plan, out if in_place else flat, out, steps=steps)
+    for shape, g, o in zip(shapes, views(flat, entries), views(out, entries)):
+        check(o, g, steps, what=f"{shape} of {len(shapes)} {kind}", independent=independent)
+    for o in views(out, entries):
+        o.fill_(3.0)
+    for o in views(before, entries):
+        o.fill_(3.0)
+    assert torch.equal(out, before)     # what lies between the matrices stays
+    return plan
+
+
+SHAPES = [(1, 1), (1, 2), (2, 1), (1, 300), (300, 1), (2, 2), (2, 128), (128, 2), (3, 5), (10, 128), (31, 33), (32, 32), (33, 31), (64, 64), (65, 130),
+          (130, 65), (96, 128), (128, 96), (128, 128), (127, 129), (129, 127), (128, 160), (200, 100), (128, 256), (257, 300), (512, 96), (1024, 128),
+          (128, 1024), (4000, 3), (333, 999), (512, 512), (700, 1500)]
+
+
+@pytest.mark.parametrize("shape", SHAPES, ids=lambda s: f"{s[0]}x{s[1]}")
+def test_one_matrix(lib, shape):
+    orthogonalize(lib, [shape], seed=sum(shape))
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("shape", [(1, 1), (2, 128), (33, 31), (64, 64), (128, 128), (130, 65), (257, 300), (1024, 128), (333, 999)], ids=lambda s: f"{s[0]}x{s[1]}")
+def test_one_matrix_of_16_bits(lib, shape, kind):
+    orthogonalize(lib, [shape], kind, seed=sum(shape))
+
+
+@pytest.mark.parametrize("kind", sorted(TYPES))
+@pytest.mark.parametrize("pad", [1, 2, 5, 8, 40])
+def test_rows_inside_wider_ones(lib, pad, kind):
+    orthogonalize(lib, [(60, 90), (128, 128), (90, 60), (200, 140), (7, 1)], kind, pad=pad, seed=pad)
+
+
+@pytest.mark.parametrize("kind", sorted(TYPES))
+def test_all_matrices_of_a_network_at_once(lib, kind):
+    orthogonalize(lib, [(128, 128), (128, 128), (128, 2), (2, 128), (128, 128), (128, 128)], kind)
+    orthogonalize(lib, [(1024, 128), (128, 128), (128, 2), (2, 128), (128, 128), (128, 1024)], kind)
+    orthogonalize(lib, [(20, 17), (300, 200), (1, 9), (129, 64), (64, 640), (500, 500)], kind)
+
+
+def test_more_matrices_than_a_launch_takes(lib):
+    orthogonalize(lib, [(5 + i % 40, 3 + i % 70) for i in range(150)] + [(140, 150)] * 3)
+
+
+@pytest.mark.parametrize("steps", [1, 2, 3, 6, 9])
+def test_numbers_of_steps(lib, steps):
+    orthogonalize(lib, [(40, 70), (128, 128), (160, 130)], steps=steps)
+
+
+@pytest.mark.parametrize("kind", sorted(TYPES))
+def test_in_place(lib, kind):
+    orthogonalize(lib, [(40, 70), (128, 128), (150, 130), (2, 300)], kind, in_place=True)
+
+
+def test_spectra(lib):
+    """a matrix of rank one, an orthogonal one, one whose rows are equal, powers of ten down a diagonal"""
+    def rank_one(r, c, seed):
+        return gradient(r, c, seed, rank=1, floor=0.0)
+
+    def same_rows(r, c, seed):
+        return torch.ones(r, 1, device="cuda") * gradient(1, c, seed)
+
+    def orthogonal(r, c, seed):
+        return torch.linalg.qr(gradient(max(r, c), max(r, c), seed).cpu())[0][:r, :c].cuda()
+
+    def diagonal(r, c, seed):
+        d = torch.zeros(r, c, device="cuda")
+        k = min(r, c)
+        d[:k, :k] = torch.diag(10.0 ** torch.linspace(0, -6, k)).cuda()
+        return d
+
+    for make in (rank_one, same_rows, orthogonal, diagonal):
+        orthogonalize(lib, [(48, 80), (128, 128), (200, 136)], make=make, independent=False)
+
+
+@pytest.mark.parametrize("factor", [1e-30, 1e-12, 1e12, 1e30])
+def test_gradients_of_any_size(lib, factor):
+    """the norm of 1e-30 or 1e30 does not leave float32 where its square would"""
+    entries, n = lay_out([(50, 70), (140, 130)])
+    flat = torch.zeros(n, device="cuda")
+    for i, v in enumerate(views(flat, entries)):
+        v.copy_(gradient(*v.shape, i) * factor)
+    out = torch.zeros(n, device="cuda")
+    eps = 1e-7 * factor
+    lib.orthogonalize(lib.MatrixPlan(entries), flat, out, eps=eps)
+    for g, o in zip(views(flat, entries), views(out, entries)):
+        check(o, (g.double() / factor).float(), eps=1e-7, what=f"x {factor}")
+
+
+def test_zeros_stay_and_what_is_not_finite_spoils_its_own_matrix(lib):
+    entries, n = lay_out([(40, 50), (140, 150), (2, 64), (40, 50), (140, 150), (2, 64), (64, 64)])
+    flat = torch.zeros(n, device="cuda")
+    vs = views(flat, entries)
+    for k, value in ((3, float("nan")), (4, float("inf")), (5, float("-inf"))):
+        vs[k].copy_(gradient(*vs[k].shape, k))
+        vs[k][1, 17] = value
+    vs[6].copy_(gradient(64, 64, 9))
+    out = torch.full((n,), 0.25, device="cuda")
+    lib.orthogonalize(lib.MatrixPlan(entries), flat, out)
+    os = views(out, entries)
+    assert all((o == 0).all() for o in os[:3]) and all(torch.isnan(o).all() for o in os[3:6])
+    check(os[6], vs[6])
+
+
+def test_same_answer_every_time_and_any_content_of_the_scratch(lib):
+    entries, n = lay_out([(128, 128), (2, 128), (300, 200), (129, 700)])
+    flat = torch.zeros(n, device="cuda")
+    for i, v in enumerate(views(flat, entries)):
+        v.copy_(gradient(*v.shape, i))
+    plan = lib.MatrixPlan(entries)
+    first = None
+    for fill in (0, 255, 127):
+        plan.ws.fill_(fill)
+        out = torch.zeros(n, device="cuda")
+        lib.orthogonalize(plan, flat, out)
+        first = out if first is None else first
+        assert torch.equal(first, out)
+
+
+def muon_case(lib, shapes, slices, nesterov, decay, seed=0, pad=0, momentum=0.95, lr=0.02, steps=5):
+    entries, n = lay_out(shapes, pad)
+    gen = torch.Generator("cuda").manual_seed(seed)
+    g = torch.randn(slices, n, generator=gen, device="cuda") * 0.01
+    for s in range(slices):
+        for i, v in enumerate(views(g[s], entries)):
+            v.copy_(gradient(*v.shape, 100 * s + i + seed))
+    m = torch.randn(n, generator=gen, device="cuda") * 0.05
+    w = torch.randn(n, generator=gen, device="cuda")
+    w0, m0 = w.clone(), m.clone()
+    plan = lib.MatrixPlan(entries)
+    lib.muon_step(plan, w, g if slices > 1 else g[0], m, lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=decay, steps=steps)
+    total = g.double().sum(0)
+    u = 2.0 ** -24
+    mags = g.abs().double().sum(0) + m0.abs().double()
+    for e, gv, wv, mv, w0v, m0v, mag in zip(entries, *[views(t, entries) for t in (total, w, m, w0, m0, mags)]):
+        m64 = momentum * m0v.double() + gv
+        assert ((mv.double() - m64).abs() <= (slices + 2) * u * mag).all(), "momentum"
+        direction = gv + momentum * m64 if nesterov else m64
+        update = iterate(direction, steps)
+        scale = lr * e[4]
+        # the direction's own error in float32, (slices + 4) u of the magnitudes, is an error of X_0 like those of `bound`
+        start = (slices + 4) * u * (2 * mag.norm() / direction.norm()).item() * ABC[0] ** steps
+        allowed = scale * (bound(e[1], e[2], steps) + start) + 4 * u * (w0v.abs().double() + scale * update.abs())
+        err = (wv.double() - ((1 - lr * decay) * w0v.double() - scale * update)).abs()
+        assert (err <= allowed).all(), f"w of {e[1:3]}: {(err / allowed).max().item():.3g} of what is allowed"
+        # and against the same in float32
+        single = iterate(direction.float(), steps).double()
+        assert err.norm() <= scale * max(4 * (single - update).norm().item(), 8e-6 * update.norm().item()) + 4 * u * (w0v.norm() + scale * update.norm()).item()
+    for t, t0 in ((w, w0), (m, m0)):
+        for v, v0 in zip(views(t, entries), views(t0, entries)):
+            v.copy_(v0)
+        assert torch.equal(t, t0)       # biases and gaps
+
+
+@pytest.mark.parametrize("nesterov", [True, False])
+@pytest.mark.parametrize("slices", [1, 2, 3, 7, 32])
+def test_muon_step(lib, slices, nesterov):
+    muon_case(lib, [(128, 128), (128, 2), (2, 128), (60, 90)], slices, nesterov, 0.0, seed=slices)
+    muon_case(lib, [(300, 200), (129, 140), (16, 16)], slices, nesterov, 0.1, seed=slices)
+
+
+def test_muon_step_on_rows_inside_wider_ones(lib):
+    muon_case(lib, [(100, 70), (150, 140), (9, 200)], 3, True, 0.05, pad=6)
+
+
+def test_muon_step_without_momentum_is_the_orthogonalised_gradient(lib):
+    entries, n = lay_out([(70, 90), (140, 135)])
+    g = torch.zeros(n, device="cuda")
+    for i, v in enumerate(views(g, entries)):
+        v.copy_(gradient(*v.shape, i))
+    plan = lib.MatrixPlan(entries)
+    out = torch.zeros(n, device="cuda")
+    lib.orthogonalize(plan, g, out)
+    w, m = torch.zeros(n, device="cuda"), torch.zeros(n, device="cuda")
+    lib.muon_step(plan, w, g, m, lr=1.0, momentum=0.0, nesterov=False)
+    for e, o, x in zip(entries, views(out, entries), views(w, entries)):
+        assert torch.allclose(x, -e[4] * o, rtol=1e-6, atol=0)
+
+
+def test_on_another_stream_and_in_graphs_that_share_the_scratch(lib):
+    entries, n = lay_out([(128, 128), (2, 128), (150, 300)])
+    gen = torch.Generator("cuda").manual_seed(3)
+    g = torch.randn(2, n, generator=gen, device="cuda")
+    w, m = torch.randn(n, generator=gen, device="cuda"), torch.randn(n, generator=gen, device="cuda")
+    w0, m0 = w.clone(), m.clone()
+    out = torch.zeros(n, device="cuda")
+    plan = lib.MatrixPlan(entries)
+
+    def step():
+        lib.muon_step(plan, w, g, m, lr=0.1)
+
+    def ortho():
+        lib.orthogonalize(plan, w, out)
+
+    def eager(times):
+        w.copy_(w0), m.copy_(m0)
+        for _ in range(times):
+            step()
+            ortho()
+        torch.cuda.synchronize()
+        return w.clone(), m.clone(), out.clone()
+
+    want = [eager(k) for k in range(1, 4)]
+    side = torch.cuda.Stream()
+    w.copy_(w0), m.copy_(m0)
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+        ortho()
+    side.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip((w, m, out), want[0]))
+    one, two = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(one):
+        step()
+    with torch.cuda.graph(two):
+        ortho()
+    w.copy_(w0), m.copy_(m0)
+    for k in range(3):
+        out.zero_()
+        one.replay()
+        two.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip((w, m, out), want[k])), k
+
+
+def test_refusals_of_the_binding(lib):
+    entries, n = lay_out([(8, 9), (30, 40)])
+    plan = lib.MatrixPlan(entries)
+    g, out = torch.zeros(n, device="cuda"), torch.zeros(n, device="cuda")
+    short = torch.zeros(plan.end - 1, device="cuda")
+    bad = [
+        lambda: lib.orthogonalize(plan, short, out), lambda: lib.orthogonalize(plan, g, short), lambda: lib.orthogonalize(plan, g.half(), out),
+        lambda: lib.orthogonalize(plan, g.double(), out.double()), lambda: lib.orthogonalize(plan, g.cpu(), out), lambda: lib.orthogonalize(plan, g, out.cpu()),
+        lambda: lib.orthogonalize(plan, torch.zeros(2 * n, device="cuda")[::2], out), lambda: lib.orthogonalize(plan, g, out, steps=0),
+        lambda: lib.orthogonalize(plan, g, out, eps=0.0),
+        lambda: lib.muon_step(plan, g, g, out, lr=0.1), lambda: lib.muon_step(plan, out, g, out, lr=0.1),
+        lambda: lib.muon_step(plan, g.half(), g, out, lr=0.1), lambda: lib.muon_step(plan, torch.zeros(n, device="cuda"), short, out, lr=0.1),
+        lambda: lib.muon_step(plan, torch.zeros(n, device="cuda"), torch.zeros(3, plan.end - 1, device="cuda"), out, lr=0.1),
+        lambda: lib.muon_step(plan, torch.zeros(n, device="cuda"), g, out, lr=0.1, momentum=1.0),
+    ]
+    for k, call in enumerate(bad):
+        with pytest.raises(lib.EmxError):
+            call()
+            raise AssertionError(f"call {k} was accepted")
+    assert (g == 0).all() and (out == 0).all()
