@@ -286,6 +286,210 @@ __global__ __launch_bounds__(NT) void ns_product_kernel(const Table tab, const S
   }
 }
 
+// ---- the same products in tiles of 256 x 128 for large matrices: four waves, 64 x 128 each.  A wave's operand of 64 rows is its own and
+// goes from global memory into registers (every piece is what a matrix instruction reads); the operand of 128 columns is shared through LDS.
+// Per 32 k a workgroup reads 48 KB for 192 matrix instructions, its LDS traffic is 80 KB: 32 and 52 bytes a clock at their full rate.
+constexpr int BT_R = 8, BT_C = 4;             // blocks of 32 a tile has: rows, columns
+// tiles of a product, in the order they are handed out: bands of 4 tile rows, column by column inside a band
+constexpr int BAND = 4;
+constexpr long BIG_TILES = 64;
+__host__ __device__ inline long band_count(int r0, int tr, int tc, bool upper) {
+  const int h = min(BAND, tr - r0);
+  if (!upper) return (long)h * tc;
+  const int nc = tc - 2 * r0;                 // columns from the diagonal on: column 2 r0 + d has min(h, d / 2 + 1) tiles
+  if (nc >= 2 * h) return h * (h + 1) + (long)(nc - 2 * h) * h;
+  const int k = nc / 2;
+  return k * (k + 1) + (nc & 1) * (k + 1);
+}
+__host__ __device__ inline long tile_count(int tr, int tc, bool upper) {
+  long n = 0;
+  for (int r0 = 0; r0 < tr && (!upper || 2 * r0 < tc); r0 += BAND) n += band_count(r0, tr, tc, upper);
+  return n;
+}
+__device__ __forceinline__ void tile_of(int t, int tr, int tc, bool upper, int& ti, int& tj) {
+  int r0 = 0;
+  for (;;) {
+    const int n = (int)band_count(r0, tr, tc, upper);
+    if (t < n || r0 + BAND >= tr) break;
+    t -= n, r0 += BAND;
+  }
+  const int h = min(BAND, tr - r0);
+  int c0 = 0;
+  if (upper) {
+    c0 = 2 * r0;
+    for (int d = 0; d < 2 * h; ++d) {
+      const int n = d / 2 + 1;
+      if (t < n) {
+        ti = r0 + t, tj = c0 + d;
+        return;
+      }
+      t -= n;
+    }
+    c0 += 2 * h;
+  }
+  tj = c0 + t / h, ti = r0 + t % h;
+}
+
+// four values of a product's transpose (v: rows 8 q + 4 h .. + 3 of column lr) as they are stored
+__device__ __forceinline__ void split_quad(const float (&v)[4], half4& hi, half4& lo) {
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    hi[r] = (_Float16)v[r];
+    lo[r] = (_Float16)(v[r] - (float)hi[r]);
+  }
+}
+
+template <int KIND, typename T, bool MUON>
+__global__ __launch_bounds__(NT, 2) void ns_big_kernel(const Table tab, const StepArgs a, const int odd, const int total) {
+  __shared__ __align__(16) char lds[2][BT_C * BLK];
+  // one eighth of the tiles to each XCD, consecutive ones: they share operands in its L2
+  const int per = (total + 7) >> 3, at = (int)(blockIdx.x & 7) * per + (int)(blockIdx.x >> 3);
+  if (at >= total) return;
+  int inside;
+  const Mat m = tab.m[find(tab, at, inside)];
+  const Scratch s(m.rows, m.cols, a.ws + m.ws);
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int lr = lane & 31, h = lane >> 5;
+  char *const t_in = odd ? s.t1 : s.t0, *const t_out = odd ? s.t0 : s.t1;
+  const int Jb = KIND <= POLY ? s.Mb : s.Nb, Kb = KIND == GRAM ? s.Nb : s.Mb;
+  int ti, tj;
+  tile_of(inside, (s.Mb + BT_R - 1) / BT_R, (Jb + BT_C - 1) / BT_C, KIND <= POLY, ti, tj);
+  const int ib0 = BT_R * ti + 2 * wave, jb0 = BT_C * tj;
+  const char* const Ub = KIND == GRAM ? s.x : KIND == POLY ? s.a : s.p;
+  const char* const Vb = KIND == GRAM ? s.x : KIND == POLY ? s.a : t_in;
+  // (blocks beyond the matrix are read from its last one and not stored)
+  const char* U[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) U[i] = Ub + (long)min(ib0 + i, s.Mb - 1) * Kb * BLK + lane * 16;
+  const char* V = Vb + (long)min(jb0 + wave, Jb - 1) * Kb * BLK + lane * 16;   // this wave's block of the shared operand
+  f32x16 acc[2][BT_C];
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < BT_C; ++j)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+  half8 u[2][2][2], v[4];                       // [K-step][block][plane]; the shared operand's next block
+  auto request_u = [&](const int ks, const long k) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      u[ks][i][0] = *reinterpret_cast<const half8*>(U[i] + k * BLK + ks * 2048);
+      u[ks][i][1] = *reinterpret_cast<const half8*>(U[i] + k * BLK + ks * 2048 + 1024);
+    }
+  };
+  auto request_v = [&](const long k) __attribute__((always_inline)) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) v[q] = *reinterpret_cast<const half8*>(V + k * BLK + q * 1024);
+  };
+  auto keep_v = [&](const int buf) __attribute__((always_inline)) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) *reinterpret_cast<half8*>(lds[buf] + wave * BLK + q * 1024 + lane * 16) = v[q];
+  };
+  request_v(0);
+  request_u(0, 0);
+  request_u(1, 0);
+  keep_v(0);
+  if (Kb > 1) request_v(1);
+  for (int k = 0; k < Kb; ++k) {
+    const int buf = k & 1;
+    __syncthreads();                            // the buffer is written, and the other one read to its end
+    if (k + 1 < Kb) keep_v(buf ^ 1);
+    if (k + 2 < Kb) request_v(k + 2);
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) {
+#pragma unroll
+      for (int j = 0; j < BT_C; ++j) {
+        const char* p = lds[buf] + j * BLK + ks * 2048 + lane * 16;
+        const half8 vh = *reinterpret_cast<const half8*>(p), vl = *reinterpret_cast<const half8*>(p + 1024);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(u[ks][i][0], vl, acc[i][j], 0, 0, 0);   // small products first
+#pragma unroll
+        for (int i = 0; i < 2; ++i) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(u[ks][i][1], vh, acc[i][j], 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(u[ks][i][0], vh, acc[i][j], 0, 0, 0);
+      }
+      if (k + 1 < Kb) request_u(ks, k + 1);     // (into the registers just used: on its way during the other K-step)
+    }
+  }
+  // acc[i][j][4 q + r]: row 32 (ib0 + i) + 8 q + 4 h + r, column 32 (jb0 + j) + lr
+  if constexpr (KIND == LAST) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int j = 0; j < BT_C; ++j)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int row = 32 * (ib0 + i) + 8 * (e >> 2) + 4 * h + (e & 3), col = 32 * (jb0 + j) + lr;
+          if (row < s.M && col < s.N) {
+            const long to = m.off + (s.turned ? col * m.ld + row : row * m.ld + col);
+            const float x = acc[i][j][e] * (RSC * RSC);
+            if constexpr (MUON) a.w[to] = fmaf(a.w[to], a.keep, -(a.lr * m.scale) * x);
+            else ((T*)a.out)[to] = (T)x;
+          }
+        }
+  } else {
+    char* const O = KIND == GRAM ? s.a : KIND == POLY ? s.p : t_out;
+    // The result in operand layout with ITS rows as rows (the transpose of what the registers hold) by two matrix instructions against a
+    // permuted identity: k-slot (h, e) of K-step ks stands for the product's row 16 ks + 4 h + (e < 4 ? e : e + 4), which is where
+    // the registers have it.
+    half8 one[2];
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) one[ks][e] = (_Float16)(lr == 16 * ks + 4 * h + (e < 4 ? e : e + 4) ? 1.f : 0.f);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+#pragma unroll
+      for (int j = 0; j < BT_C; ++j) {
+        const int ib = ib0 + i, jb = jb0 + j;
+        if (ib >= s.Mb || jb >= Jb || (KIND <= POLY && ib > jb)) continue;
+        half4 hi[4], lo[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int to = (q >> 1) * 2048 + ((q & 1) * 32 + lr) * 16 + h * 8;
+          float x[4];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) x[r] = acc[i][j][4 * q + r] * RSC;
+          if constexpr (KIND == POLY) {
+            const char* am = s.a + ((long)jb * s.Mb + ib) * BLK + to;    // A is symmetric: the same four of its transpose
+            const half4 ah = *reinterpret_cast<const half4*>(am), al = *reinterpret_cast<const half4*>(am + 1024);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              x[r] = fmaf(CC, x[r], CB * ((float)ah[r] + (float)al[r]));
+              if (ib == jb && 8 * q + 4 * h + r == lr && 32 * ib + lr < s.M) x[r] += CA * SC;
+            }
+          }
+          split_quad(x, hi[q], lo[q]);
+          char* const direct = O + ((long)jb * s.Mb + ib) * BLK + to;
+          *reinterpret_cast<half4*>(direct) = hi[q];
+          *reinterpret_cast<half4*>(direct + 1024) = lo[q];
+        }
+        if (KIND <= POLY && ib == jb) continue;
+        char* const other = KIND == NEXT ? s.x + ((long)ib * s.Nb + jb) * BLK : O + ((long)ib * s.Mb + jb) * BLK;
+#pragma unroll
+        for (int plane = 0; plane < 2; ++plane) {
+          f32x16 d;
+#pragma unroll
+          for (int e = 0; e < 16; ++e) d[e] = 0.f;
+#pragma unroll
+          for (int ks = 0; ks < 2; ++ks) {
+            const half4 p0 = plane ? lo[2 * ks] : hi[2 * ks], p1 = plane ? lo[2 * ks + 1] : hi[2 * ks + 1];
+            d = __builtin_amdgcn_mfma_f32_32x32x16_f16(half8{p0[0], p0[1], p0[2], p0[3], p1[0], p1[1], p1[2], p1[3]}, one[ks], d, 0, 0, 0);
+          }
+          // d[4 q + r]: column lr is the product's row, 8 q + 4 h + r its column
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            half4 o;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) o[r] = (_Float16)d[4 * q + r];
+            *reinterpret_cast<half4*>(other + (q >> 1) * 2048 + ((q & 1) * 32 + lr) * 16 + h * 8 + plane * 1024) = o;
+          }
+        }
+      }
+    }
+  }
+}
+
 // ---- host side
 int check_matrices(const char* who, const emx_matrix* mats, int n) {
   EMX_REQUIRE(n >= 0 && (n == 0 || mats), "%s: %d matrices", who, n);
@@ -356,12 +560,22 @@ int run(const char* who, const emx_matrix* mats, int n, const StepArgs& a, int s
     };
     if ((rc = go(ns_norm_kernel<T, MUON>, number(t, parts)))) return rc;
     if ((rc = go(ns_split_kernel<T, MUON>, number(t, full)))) return rc;
+    const auto big_upper = [&](const Mat&, const Scratch& s) { return tile_count((s.Mb + BT_R - 1) / BT_R, (s.Mb + BT_C - 1) / BT_C, true); };
+    const auto big_full = [&](const Mat&, const Scratch& s) { return tile_count((s.Mb + BT_R - 1) / BT_R, (s.Nb + BT_C - 1) / BT_C, false); };
+    const bool big = number(t, big_full) >= BIG_TILES;
+    auto product = [&](auto small_kernel, auto big_kernel, bool up, int k) {
+      if (big) {
+        const long tiles = up ? number(t, big_upper) : number(t, big_full);
+        return go(big_kernel, 8 * ((tiles + 7) / 8), k & 1, (int)tiles);
+      }
+      return go(small_kernel, up ? number(t, upper) : number(t, full), k & 1);
+    };
     for (int k = 0; k < steps; ++k) {
-      const long up = number(t, upper);
-      if ((rc = go(ns_product_kernel<GRAM, T, MUON>, up, k & 1))) return rc;
-      if ((rc = go(ns_product_kernel<POLY, T, MUON>, up, k & 1))) return rc;
-      const long all = number(t, full);
-      if ((rc = k + 1 < steps ? go(ns_product_kernel<NEXT, T, MUON>, all, k & 1) : go(ns_product_kernel<LAST, T, MUON>, all, k & 1))) return rc;
+      if ((rc = product(ns_product_kernel<GRAM, T, MUON>, ns_big_kernel<GRAM, T, MUON>, true, k))) return rc;
+      if ((rc = product(ns_product_kernel<POLY, T, MUON>, ns_big_kernel<POLY, T, MUON>, true, k))) return rc;
+      if (k + 1 < steps) rc = product(ns_product_kernel<NEXT, T, MUON>, ns_big_kernel<NEXT, T, MUON>, false, k);
+      else rc = product(ns_product_kernel<LAST, T, MUON>, ns_big_kernel<LAST, T, MUON>, false, k);
+      if (rc) return rc;
     }
   }
   return EMX_OK;
