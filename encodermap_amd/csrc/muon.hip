@@ -19,6 +19,7 @@
 // transpose in operand layout straight from registers.  M and N are padded to 32 with zeros, which stay zero.
 #include <algorithm>
 #include <cstdint>
+#include <type_traits>
 #include <vector>
 
 #include "emx_common.h"
@@ -29,7 +30,7 @@ using namespace emx;
 
 constexpr int NT = 256;
 constexpr int MAX_TABLE = 64;                 // matrices of one launch
-constexpr int MAX_PARTS = 256;                // shares of a matrix' sum of squares
+constexpr int MAX_PARTS = 1024;               // shares of a matrix' sum of squares
 constexpr float CA = 3.4445f, CB = -4.7750f, CC = 2.0315f;
 constexpr float SC = 16384.f, RSC = 1.f / 16384.f;
 constexpr int BLK = 4096;                     // bytes of an operand's 32 x 32 block
@@ -70,7 +71,8 @@ struct Scratch {
     return MAX_PARTS * 8 + ((size_t)3 * s.Mb * s.Nb + (size_t)2 * s.Mb * s.Mb) * BLK;
   }
 };
-__host__ __device__ inline int parts_of(long n) { return (int)(n <= 4096l * MAX_PARTS ? (n + 4095) / 4096 : MAX_PARTS); }
+// (1024 elements and more to a share: the optimizer step reads up to 32 gradient parts of each)
+__host__ __device__ inline int parts_of(long n) { return (int)(n <= 1024l * MAX_PARTS ? (n + 1023) / 1024 : MAX_PARTS); }
 
 // the matrix a workgroup belongs to, and its number inside it
 __device__ __forceinline__ int find(const Table& t, int block, int& inside) {
@@ -94,41 +96,95 @@ struct StepArgs {
   float beta, keep, lr, eps;    // keep = 1 - lr weight_decay
 };
 
-// ---- 1: the sum of squares in shares; the optimizer step also forms its update's direction u here
+// ---- 1: the sum of squares in shares; the optimizer step also forms its update's direction u here.  Four consecutive elements per
+// thread at a time where the rows allow it (their length is a multiple of 4), the parts of a gradient eight at a time.
+template <typename T, bool MUON, int E>
+__device__ __forceinline__ double norm_share(const Mat& m, const StepArgs& a, float* u_out, unsigned e0, unsigned e1) {
+  typedef T vec __attribute__((ext_vector_type(E), aligned(sizeof(T))));
+  typedef float fvec __attribute__((ext_vector_type(E), aligned(4)));
+  const unsigned cols = m.cols;
+  const bool flat = m.ld == (long)cols;
+  double sum = 0.0;
+#pragma unroll 2
+  for (unsigned e = e0 + E * threadIdx.x; e < e1; e += E * NT) {
+    long at = m.off + e;
+    if (!flat) {
+      const unsigned r = e / cols;
+      at = m.off + r * m.ld + (e - r * cols);
+    }
+    float u[E];
+    if constexpr (MUON) {
+      const float* g = (const float*)a.g + at;
+      fvec mo = *reinterpret_cast<const fvec*>(a.mom + at);
+      fvec v = *reinterpret_cast<const fvec*>(g);
+      int k = 1;
+      for (; k + 8 <= a.n_slices; k += 8) {
+        fvec p[8];
+#pragma unroll
+        for (int q = 0; q < 8; ++q) p[q] = *reinterpret_cast<const fvec*>(g + (k + q) * a.slice_stride);
+#pragma unroll
+        for (int q = 0; q < 8; ++q)
+#pragma unroll
+          for (int i = 0; i < E; ++i) v[i] += p[q][i];
+      }
+      for (; k < a.n_slices; ++k) {
+        const fvec p = *reinterpret_cast<const fvec*>(g + k * a.slice_stride);
+#pragma unroll
+        for (int i = 0; i < E; ++i) v[i] += p[i];
+      }
+      fvec o;
+#pragma unroll
+      for (int i = 0; i < E; ++i) {
+        mo[i] = fmaf(a.beta, mo[i], v[i]);
+        o[i] = u[i] = a.nesterov ? fmaf(a.beta, mo[i], v[i]) : mo[i];
+      }
+      *reinterpret_cast<fvec*>(a.mom + at) = mo;
+      *reinterpret_cast<fvec*>(u_out + e) = o;
+    } else {
+      const vec v = *reinterpret_cast<const vec*>((const T*)a.g + at);
+#pragma unroll
+      for (int i = 0; i < E; ++i) u[i] = (float)v[i];
+    }
+#pragma unroll
+    for (int i = 0; i < E; ++i) sum = fma((double)u[i], (double)u[i], sum);
+  }
+  return sum;
+}
+__device__ __forceinline__ double wave_sum64(double v) {
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) v += __shfl_xor(v, d);
+  return v;
+}
 template <typename T, bool MUON>
 __global__ __launch_bounds__(NT) void ns_norm_kernel(const Table tab, const StepArgs a) {
   __shared__ double sm[NT / 64];
   int part;
   const Mat m = tab.m[find(tab, blockIdx.x, part)];
   const Scratch s(m.rows, m.cols, a.ws + m.ws);
-  const unsigned total = (unsigned)m.rows * m.cols, cols = m.cols;
+  const unsigned total = (unsigned)m.rows * m.cols;
   const int parts = parts_of(total);
-  const unsigned chunk = (total + parts - 1) / parts;
-  const unsigned e0 = part * chunk, e1 = min(e0 + chunk, total);
+  const unsigned chunk = ((total + parts - 1) / parts + 3) & ~3u;
+  const unsigned e0 = min(part * chunk, total), e1 = min(e0 + chunk, total);
   float* const u_out = reinterpret_cast<float*>(s.t1);
-  double sum = 0.0;
-  for (unsigned e = e0 + threadIdx.x; e < e1; e += NT) {
-    const unsigned r = e / cols;
-    const long at = m.off + r * m.ld + (e - r * cols);
-    float u;
-    if constexpr (MUON) {
-      const float* g = (const float*)a.g + at;
-      float v = g[0];
-      for (int k = 1; k < a.n_slices; ++k) v += g[k * a.slice_stride];
-      const float mo = fmaf(a.beta, a.mom[at], v);
-      a.mom[at] = mo;
-      u = a.nesterov ? fmaf(a.beta, mo, v) : mo;
-      u_out[e] = u;
-    } else {
-      u = (float)((const T*)a.g)[at];
-    }
-    sum = fma((double)u, (double)u, sum);
-  }
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) sum += __shfl_xor(sum, d);
+  double sum = m.cols % 4 == 0 ? norm_share<T, MUON, 4>(m, a, u_out, e0, e1) : norm_share<T, MUON, 1>(m, a, u_out, e0, e1);
+  sum = wave_sum64(sum);
   if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = sum;
   __syncthreads();
   if (threadIdx.x == 0) s.part[part] = (sm[0] + sm[1]) + (sm[2] + sm[3]);
+}
+// 2^14 / (|u|_F + eps), in every thread of a workgroup of N threads
+template <int N>
+__device__ __forceinline__ double scale_of(const Mat& m, const Scratch& s, float eps, double* sm /* N / 64 */) {
+  const int parts = parts_of((long)m.rows * m.cols);
+  double sum = 0.0;
+  for (int i = threadIdx.x; i < parts; i += N) sum += s.part[i];
+  sum = wave_sum64(sum);
+  if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = sum;
+  __syncthreads();
+  sum = 0.0;
+#pragma unroll
+  for (int i = 0; i < N / 64; ++i) sum += sm[i];
+  return (double)SC / (sqrt(sum) + (double)eps);
 }
 
 // eight values of a row as the hi and lo units of an operand
@@ -153,12 +209,7 @@ __global__ __launch_bounds__(NT) void ns_split_kernel(const Table tab, const Ste
   const Scratch s(m.rows, m.cols, a.ws + m.ws);
   const int tid = threadIdx.x;
   const int tn = (s.Nb + 1) / 2, ti = inside / tn, tj = inside - ti * tn;
-  double sum = tid < parts_of((long)m.rows * m.cols) ? s.part[tid] : 0.0;
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) sum += __shfl_xor(sum, d);
-  if ((tid & 63) == 0) sm[tid >> 6] = sum;
-  __syncthreads();
-  const double f = (double)SC / (sqrt((sm[0] + sm[1]) + (sm[2] + sm[3])) + (double)a.eps);
+  const double f = scale_of<NT>(m, s, a.eps, sm);
   const float* const u_in = reinterpret_cast<const float*>(s.t1);
   // the tile as it is stored: rows (r0 ..), columns (c0 ..) of G
   const int r0 = 64 * (s.turned ? tj : ti), c0 = 64 * (s.turned ? ti : tj);
@@ -191,6 +242,61 @@ __device__ __forceinline__ void triangle(int t, int nb, int& ti, int& tj) {   //
   while (ti > 0 && ti * nb - ti * (ti - 1) / 2 > t) --ti;
   while ((ti + 1) * nb - (ti + 1) * ti / 2 <= t) ++ti;
   tj = ti + t - (ti * nb - ti * (ti - 1) / 2);
+}
+
+// A 32 x 32 block of the last X into the caller's tensors (x: row 32 ib + 8 q + 4 h + r, column 32 jb + lr, scaled by 2^28): the update of w, or
+// the result.  All of a block's reads stand in front of its writes.  A turned matrix has four consecutive elements per lane.
+template <typename T, bool MUON>
+__device__ __forceinline__ void write_block(const Mat& m, const StepArgs& a, const Scratch& s, const f32x16& x, int ib, int jb, int lr, int h) {
+  const float keep = a.keep, f = MUON ? -(a.lr * m.scale) * (RSC * RSC) : RSC * RSC;
+  const int row0 = 32 * ib + 4 * h, col = 32 * jb + lr;
+  typedef typename std::conditional<MUON, float, T>::type O;
+  O* const base = (MUON ? (O*)a.w : (O*)a.out) + m.off;
+  if (s.turned) {
+    typedef O quad __attribute__((ext_vector_type(4), aligned(sizeof(O))));
+    O* const p = base + (long)col * m.ld + row0;
+    if (col >= s.N) return;
+    quad old[4];
+    if constexpr (MUON) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        if (row0 + 8 * q + 4 <= s.M) {
+          old[q] = *reinterpret_cast<const quad*>(p + 8 * q);
+        } else {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) old[q][r] = row0 + 8 * q + r < s.M ? p[8 * q + r] : (O)0.f;
+        }
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      quad o;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) o[r] = MUON ? (O)fmaf((float)old[q][r], keep, x[4 * q + r] * f) : (O)(x[4 * q + r] * f);
+      if (row0 + 8 * q + 4 <= s.M) {
+        *reinterpret_cast<quad*>(p + 8 * q) = o;
+      } else {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (row0 + 8 * q + r < s.M) p[8 * q + r] = o[r];
+      }
+    }
+  } else {
+    O* const p = base + (long)row0 * m.ld + col;
+    O old[16];
+    if constexpr (MUON) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int d = 8 * (e >> 2) + (e & 3);
+        if (row0 + d < s.M && col < s.N) old[e] = p[d * m.ld];
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const int d = 8 * (e >> 2) + (e & 3);
+      if (row0 + d < s.M && col < s.N) p[d * m.ld] = MUON ? (O)fmaf((float)old[e], keep, x[e] * f) : (O)(x[e] * f);
+    }
+  }
 }
 
 template <int KIND, typename T, bool MUON>
@@ -234,16 +340,7 @@ __global__ __launch_bounds__(NT) void ns_product_kernel(const Table tab, const S
   acc = sum;
   // acc[4 q + r]: row 32 ib + 8 q + 4 h + r, column 32 jb + lr
   if constexpr (KIND == LAST) {
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const int row = 32 * ib + 8 * (i >> 2) + 4 * h + (i & 3), col = 32 * jb + lr;
-      if (row < s.M && col < s.N) {
-        const long at = m.off + (s.turned ? col * m.ld + row : row * m.ld + col);
-        const float v = acc[i] * (RSC * RSC);
-        if constexpr (MUON) a.w[at] = fmaf(a.w[at], a.keep, -(a.lr * m.scale) * v);
-        else ((T*)a.out)[at] = (T)v;
-      }
-    }
+    write_block<T, MUON>(m, a, s, acc, ib, jb, lr, h);
   } else {
     char* const O = KIND == GRAM ? s.a : KIND == POLY ? s.p : t_out;
     const int rows_b = KIND == NEXT ? s.Mb : s.Mb;                   // blocks along k of the transposed result
@@ -369,7 +466,10 @@ __global__ __launch_bounds__(NT, 2) void ns_big_kernel(const Table tab, const St
     for (int j = 0; j < BT_C; ++j)
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
-  half8 u[2][2][2], v[4];                       // [K-step][block][plane]; the shared operand's next block
+  // The k loop is written in the order it is to run: a GROUP is two blocks of columns of one K-step, 12 matrix instructions on four
+  // accumulators; the next group's reads of LDS stand in front of them (the compiler left to itself puts each read right before its use),
+  // and no load is conditional (the last ones are repeated), which keeps the counts of loads in flight exact.
+  half8 u[2][2][2], v[4], w[2][2][2];           // [K-step][block][plane]; the shared operand's next block; [group parity][column block][plane]
   auto request_u = [&](const int ks, const long k) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -385,48 +485,61 @@ __global__ __launch_bounds__(NT, 2) void ns_big_kernel(const Table tab, const St
 #pragma unroll
     for (int q = 0; q < 4; ++q) *reinterpret_cast<half8*>(lds[buf] + wave * BLK + q * 1024 + lane * 16) = v[q];
   };
+  auto read_w = [&](const int buf, const int g) __attribute__((always_inline)) {   // group g: K-step g >> 1, columns 2 (g & 1) ..
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int plane = 0; plane < 2; ++plane)
+        w[g & 1][j][plane] = *reinterpret_cast<const half8*>(lds[buf] + (2 * (g & 1) + j) * BLK + (g >> 1) * 2048 + plane * 1024 + lane * 16);
+  };
+  auto multiply = [&](const int g) __attribute__((always_inline)) {
+    const int ks = g >> 1, j0 = 2 * (g & 1);
+#pragma unroll
+    for (int pass = 0; pass < 3; ++pass)        // small products first
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          acc[i][j0 + j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(u[ks][i][pass == 1], w[g & 1][j][pass == 0], acc[i][j0 + j], 0, 0, 0);
+  };
   request_v(0);
-  request_u(0, 0);
-  request_u(1, 0);
   keep_v(0);
-  if (Kb > 1) request_v(1);
+  request_v(min(1, Kb - 1));                    // (in the loop's order: the waits count loads)
+  asm volatile("" ::: "memory");
+  request_u(0, 0);
+  asm volatile("" ::: "memory");
+  request_u(1, 0);
+  asm volatile("" ::: "memory");
   for (int k = 0; k < Kb; ++k) {
     const int buf = k & 1;
     __syncthreads();                            // the buffer is written, and the other one read to its end
-    if (k + 1 < Kb) keep_v(buf ^ 1);
-    if (k + 2 < Kb) request_v(k + 2);
-#pragma unroll
-    for (int ks = 0; ks < 2; ++ks) {
-#pragma unroll
-      for (int j = 0; j < BT_C; ++j) {
-        const char* p = lds[buf] + j * BLK + ks * 2048 + lane * 16;
-        const half8 vh = *reinterpret_cast<const half8*>(p), vl = *reinterpret_cast<const half8*>(p + 1024);
-#pragma unroll
-        for (int i = 0; i < 2; ++i) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(u[ks][i][0], vl, acc[i][j], 0, 0, 0);   // small products first
-#pragma unroll
-        for (int i = 0; i < 2; ++i) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(u[ks][i][1], vh, acc[i][j], 0, 0, 0);
-#pragma unroll
-        for (int i = 0; i < 2; ++i) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(u[ks][i][0], vh, acc[i][j], 0, 0, 0);
-      }
-      if (k + 1 < Kb) request_u(ks, k + 1);     // (into the registers just used: on its way during the other K-step)
-    }
+    read_w(buf, 0);
+    __builtin_amdgcn_sched_barrier(0);
+    read_w(buf, 1);
+    __builtin_amdgcn_sched_barrier(0);
+    multiply(0);
+    __builtin_amdgcn_sched_barrier(0);
+    keep_v(buf ^ 1);
+    request_v(min(k + 2, Kb - 1));
+    read_w(buf, 2);
+    __builtin_amdgcn_sched_barrier(0);
+    multiply(1);
+    __builtin_amdgcn_sched_barrier(0);
+    request_u(0, min(k + 1, Kb - 1));           // (into the registers just used: on its way during the other K-step)
+    read_w(buf, 3);
+    __builtin_amdgcn_sched_barrier(0);
+    multiply(2);
+    __builtin_amdgcn_sched_barrier(0);
+    multiply(3);
+    __builtin_amdgcn_sched_barrier(0);
+    request_u(1, min(k + 1, Kb - 1));
   }
   // acc[i][j][4 q + r]: row 32 (ib0 + i) + 8 q + 4 h + r, column 32 (jb0 + j) + lr
   if constexpr (KIND == LAST) {
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int j = 0; j < BT_C; ++j)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int row = 32 * (ib0 + i) + 8 * (e >> 2) + 4 * h + (e & 3), col = 32 * (jb0 + j) + lr;
-          if (row < s.M && col < s.N) {
-            const long to = m.off + (s.turned ? col * m.ld + row : row * m.ld + col);
-            const float x = acc[i][j][e] * (RSC * RSC);
-            if constexpr (MUON) a.w[to] = fmaf(a.w[to], a.keep, -(a.lr * m.scale) * x);
-            else ((T*)a.out)[to] = (T)x;
-          }
-        }
+      for (int j = 0; j < BT_C; ++j) write_block<T, MUON>(m, a, s, acc[i][j], ib0 + i, jb0 + j, lr, h);
   } else {
     char* const O = KIND == GRAM ? s.a : KIND == POLY ? s.p : t_out;
     // The result in operand layout with ITS rows as rows (the transpose of what the registers hold) by two matrix instructions against a
