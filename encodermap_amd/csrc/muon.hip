@@ -51,24 +51,33 @@ struct Table {
   Mat m[MAX_TABLE];
 };
 
-// the scratch of one matrix
+// The scratch of one matrix: the shares of its sum of squares, X^T twice (read and written by a step; the second also holds the optimizer step's
+// direction u at the begin) and, M > 128: X, A and P; M <= 128: the shares of A twice, 16 blocks from each workgroup.
+constexpr int LOW = 4;                        // blocks: matrices of at most 128 rows stay in the LDS of a workgroup (ns_low_kernel)
+constexpr int LOW_WGS = 32;                   // ... 128 columns each, or more where there are more than 32 x 128
 struct Scratch {
   int M, N, Mb, Nb;
   bool turned;
-  char *x, *t0, *t1, *a, *p;
+  char *t0, *t1, *x, *a, *p;
   double* part;
   __host__ __device__ Scratch(int rows, int cols, char* base) {
     turned = rows > cols;
     M = turned ? cols : rows, N = turned ? rows : cols;
     Mb = (M + 31) / 32, Nb = (N + 31) / 32;
-    const long xn = (long)Mb * Nb * BLK, an = (long)Mb * Mb * BLK;
+    const long xn = (long)Mb * Nb * BLK, an = low() ? (long)low_wgs() * 16 * BLK : (long)Mb * Mb * BLK;
     part = reinterpret_cast<double*>(base);
-    x = base + MAX_PARTS * 8;
-    t0 = x + xn, t1 = t0 + xn, a = t1 + xn, p = a + an;
+    t0 = base + MAX_PARTS * 8, t1 = t0 + xn;
+    x = t1 + xn;
+    a = low() ? x : x + xn;
+    p = a + an;
   }
+  __host__ __device__ bool low() const { return Mb <= LOW; }
+  __host__ __device__ int strips() const { return (Nb + 3) / 4; }     // of 128 columns
+  __host__ __device__ int low_wgs() const { return strips() < LOW_WGS ? strips() : LOW_WGS; }
   __host__ static size_t bytes(int rows, int cols) {
     const Scratch s(rows, cols, nullptr);
-    return MAX_PARTS * 8 + ((size_t)3 * s.Mb * s.Nb + (size_t)2 * s.Mb * s.Mb) * BLK;
+    const size_t xn = (size_t)s.Mb * s.Nb;
+    return MAX_PARTS * 8 + (s.low() ? 2 * xn + 2 * (size_t)s.low_wgs() * 16 : 3 * xn + 2 * (size_t)s.Mb * s.Mb) * BLK;
   }
 };
 // (1024 elements and more to a share: the optimizer step reads up to 32 gradient parts of each)
@@ -436,6 +445,53 @@ __device__ __forceinline__ void split_quad(const float (&v)[4], half4& hi, half4
   }
 }
 
+// A permuted identity that turns a block by two matrix instructions: k-slot (h, e) of K-step ks stands for the block's row
+// 16 ks + 4 h + (e < 4 ? e : e + 4), which is where the accumulators of a product have it.
+__device__ __forceinline__ void identity(half8 (&one)[2], int lr, int h) {
+#pragma unroll
+  for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) one[ks][e] = (_Float16)(lr == 16 * ks + 4 * h + (e < 4 ? e : e + 4) ? 1.f : 0.f);
+}
+// a block of values (scaled) as operand planes: its transpose as it lies in the registers ...
+__device__ __forceinline__ void put_direct(char* block, const f32x16& x, int lr, int h) {
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const float v[4] = {x[4 * q], x[4 * q + 1], x[4 * q + 2], x[4 * q + 3]};
+    half4 hi, lo;
+    split_quad(v, hi, lo);
+    char* const to = block + (q >> 1) * 2048 + ((q & 1) * 32 + lr) * 16 + h * 8;
+    *reinterpret_cast<half4*>(to) = hi;
+    *reinterpret_cast<half4*>(to + 1024) = lo;
+  }
+}
+// ... and the block itself, turned by matrix instructions
+__device__ __forceinline__ void put_turned(char* block, const f32x16& x, const half8 (&one)[2], int lr, int h) {
+  half4 hi[4], lo[4];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const float v[4] = {x[4 * q], x[4 * q + 1], x[4 * q + 2], x[4 * q + 3]};
+    split_quad(v, hi[q], lo[q]);
+  }
+#pragma unroll
+  for (int plane = 0; plane < 2; ++plane) {
+    f32x16 d;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) d[e] = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) {
+      const half4 p0 = plane ? lo[2 * ks] : hi[2 * ks], p1 = plane ? lo[2 * ks + 1] : hi[2 * ks + 1];
+      d = __builtin_amdgcn_mfma_f32_32x32x16_f16(half8{p0[0], p0[1], p0[2], p0[3], p1[0], p1[1], p1[2], p1[3]}, one[ks], d, 0, 0, 0);
+    }
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      half4 o;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) o[r] = (_Float16)d[4 * q + r];
+      *reinterpret_cast<half4*>(block + (q >> 1) * 2048 + ((q & 1) * 32 + lr) * 16 + h * 8 + plane * 1024) = o;
+    }
+  }
+}
 template <int KIND, typename T, bool MUON>
 __global__ __launch_bounds__(NT, 2) void ns_big_kernel(const Table tab, const StepArgs a, const int odd, const int total) {
   __shared__ __align__(16) char lds[2][BT_C * BLK];
@@ -542,65 +598,253 @@ __global__ __launch_bounds__(NT, 2) void ns_big_kernel(const Table tab, const St
       for (int j = 0; j < BT_C; ++j) write_block<T, MUON>(m, a, s, acc[i][j], ib0 + i, jb0 + j, lr, h);
   } else {
     char* const O = KIND == GRAM ? s.a : KIND == POLY ? s.p : t_out;
-    // The result in operand layout with ITS rows as rows (the transpose of what the registers hold) by two matrix instructions against a
-    // permuted identity: k-slot (h, e) of K-step ks stands for the product's row 16 ks + 4 h + (e < 4 ? e : e + 4), which is where
-    // the registers have it.
     half8 one[2];
-#pragma unroll
-    for (int ks = 0; ks < 2; ++ks)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) one[ks][e] = (_Float16)(lr == 16 * ks + 4 * h + (e < 4 ? e : e + 4) ? 1.f : 0.f);
+    identity(one, lr, h);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
 #pragma unroll
       for (int j = 0; j < BT_C; ++j) {
         const int ib = ib0 + i, jb = jb0 + j;
         if (ib >= s.Mb || jb >= Jb || (KIND <= POLY && ib > jb)) continue;
-        half4 hi[4], lo[4];
+        f32x16 x;
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int to = (q >> 1) * 2048 + ((q & 1) * 32 + lr) * 16 + h * 8;
-          float x[4];
-#pragma unroll
-          for (int r = 0; r < 4; ++r) x[r] = acc[i][j][4 * q + r] * RSC;
-          if constexpr (KIND == POLY) {
-            const char* am = s.a + ((long)jb * s.Mb + ib) * BLK + to;    // A is symmetric: the same four of its transpose
-            const half4 ah = *reinterpret_cast<const half4*>(am), al = *reinterpret_cast<const half4*>(am + 1024);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              x[r] = fmaf(CC, x[r], CB * ((float)ah[r] + (float)al[r]));
-              if (ib == jb && 8 * q + 4 * h + r == lr && 32 * ib + lr < s.M) x[r] += CA * SC;
-            }
-          }
-          split_quad(x, hi[q], lo[q]);
-          char* const direct = O + ((long)jb * s.Mb + ib) * BLK + to;
-          *reinterpret_cast<half4*>(direct) = hi[q];
-          *reinterpret_cast<half4*>(direct + 1024) = lo[q];
-        }
-        if (KIND <= POLY && ib == jb) continue;
-        char* const other = KIND == NEXT ? s.x + ((long)ib * s.Nb + jb) * BLK : O + ((long)ib * s.Mb + jb) * BLK;
-#pragma unroll
-        for (int plane = 0; plane < 2; ++plane) {
-          f32x16 d;
-#pragma unroll
-          for (int e = 0; e < 16; ++e) d[e] = 0.f;
-#pragma unroll
-          for (int ks = 0; ks < 2; ++ks) {
-            const half4 p0 = plane ? lo[2 * ks] : hi[2 * ks], p1 = plane ? lo[2 * ks + 1] : hi[2 * ks + 1];
-            d = __builtin_amdgcn_mfma_f32_32x32x16_f16(half8{p0[0], p0[1], p0[2], p0[3], p1[0], p1[1], p1[2], p1[3]}, one[ks], d, 0, 0, 0);
-          }
-          // d[4 q + r]: column lr is the product's row, 8 q + 4 h + r its column
+        for (int e = 0; e < 16; ++e) x[e] = acc[i][j][e] * RSC;
+        if constexpr (KIND == POLY) {
+          const char* const am = s.a + ((long)jb * s.Mb + ib) * BLK + lr * 16 + h * 8;    // A is symmetric: the same four of its transpose
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
-            half4 o;
+            const int to = (q >> 1) * 2048 + (q & 1) * 512;
+            const half4 ah = *reinterpret_cast<const half4*>(am + to), al = *reinterpret_cast<const half4*>(am + to + 1024);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) o[r] = (_Float16)d[4 * q + r];
-            *reinterpret_cast<half4*>(other + (q >> 1) * 2048 + ((q & 1) * 32 + lr) * 16 + h * 8 + plane * 1024) = o;
+            for (int r = 0; r < 4; ++r) {
+              x[4 * q + r] = fmaf(CC, x[4 * q + r], CB * ((float)ah[r] + (float)al[r]));
+              if (ib == jb && 8 * q + 4 * h + r == lr && 32 * ib + lr < s.M) x[4 * q + r] += CA * SC;
+            }
           }
         }
+        put_direct(O + ((long)jb * s.Mb + ib) * BLK, x, lr, h);
+        if (KIND == NEXT) put_turned(s.x + ((long)ib * s.Nb + jb) * BLK, x, one, lr, h);
+        else if (ib != jb) put_turned(O + ((long)ib * s.Mb + jb) * BLK, x, one, lr, h);
       }
     }
   }
+}
+
+// ---- matrices of at most 128 rows: a workgroup of eight waves holds 128 columns of X in registers, wave w the blocks (w / 2, 2 (w % 2) + 0 .. 1).
+// The operands of the three products pass through two areas of LDS of 4 x 4 blocks: X, then X^T in the first, A, then P in the second.  A matrix
+// of at most 128 columns goes through all its steps in one launch.  A longer one is cut into strips of 128 columns: a launch per step, in
+// which EVERY workgroup adds up the shares of A that the launch before left (in their order), forms P, takes its strip on and leaves its
+// share of the next A -- two products of 128^3 more per workgroup than a division of the work would need, but 2 launches a step fewer.
+constexpr int LOW_NT = 512;
+constexpr int LOW_AREA = 16 * BLK;
+
+// acc[j] += (row block u) (row block v_j)^T over nk blocks of k; u, v: this lane's 16 bytes of the first block
+__device__ __forceinline__ void low_k(f32x16 (&acc)[2], const char* u, const char* v0, const char* v1) {
+#pragma unroll
+  for (int ks = 0; ks < 2; ++ks) {
+    const half8 uh = *reinterpret_cast<const half8*>(u + ks * 2048), ul = *reinterpret_cast<const half8*>(u + ks * 2048 + 1024);
+    const half8 h0 = *reinterpret_cast<const half8*>(v0 + ks * 2048), l0 = *reinterpret_cast<const half8*>(v0 + ks * 2048 + 1024);
+    const half8 h1 = *reinterpret_cast<const half8*>(v1 + ks * 2048), l1 = *reinterpret_cast<const half8*>(v1 + ks * 2048 + 1024);
+    acc[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(uh, l0, acc[0], 0, 0, 0);   // small products first
+    acc[1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(uh, l1, acc[1], 0, 0, 0);
+    acc[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ul, h0, acc[0], 0, 0, 0);
+    acc[1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ul, h1, acc[1], 0, 0, 0);
+    acc[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(uh, h0, acc[0], 0, 0, 0);
+    acc[1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(uh, h1, acc[1], 0, 0, 0);
+  }
+}
+__device__ __forceinline__ void low_product(f32x16 (&acc)[2], const char* u, const char* v0, const char* v1, int nk) {
+  if (nk == 4) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) low_k(acc, u + k * BLK, v0 + k * BLK, v1 + k * BLK);
+  } else {
+    for (int k = 0; k < nk; ++k) low_k(acc, u + k * BLK, v0 + k * BLK, v1 + k * BLK);
+  }
+}
+__device__ __forceinline__ void clear(f32x16 (&x)[2]) {
+#pragma unroll
+  for (int j = 0; j < 2; ++j)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) x[j][e] = 0.f;
+}
+__device__ __forceinline__ void times(f32x16 (&x)[2], float f) {
+#pragma unroll
+  for (int j = 0; j < 2; ++j)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) x[j][e] *= f;
+}
+
+template <typename T, bool MUON>
+__global__ __launch_bounds__(LOW_NT) void ns_low_kernel(const Table tab, const StepArgs a, const int step /* 0: X_0 and its A (or everything) */,
+                                                        const int steps) {
+  extern __shared__ __align__(16) char lds[];
+  __shared__ double sm[LOW_NT / 64];
+  char *const area1 = lds, *const area2 = lds + LOW_AREA;
+  int wg;
+  const Mat m = tab.m[find(tab, blockIdx.x, wg)];
+  const Scratch s(m.rows, m.cols, a.ws + m.ws);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lr = lane & 31, h = lane >> 5, ib = wave >> 1, jb0 = 2 * (wave & 1);
+  const int wgs = s.low_wgs(), Mb = s.Mb;
+  const bool low_rows = ib < Mb, low_cols = low_rows && jb0 < Mb;
+  half8 one[2];
+  identity(one, lr, h);
+  f32x16 x[2], acc[2], av[2];
+
+  auto form_poly = [&]() __attribute__((always_inline)) {   // av: A, area2: A (complete).  Leaves P in area2 (complete)
+    clear(acc);
+    if (low_cols) {
+      const char* u = area2 + lane * 16;
+      low_product(acc, u + ib * 4 * BLK, u + jb0 * 4 * BLK, u + (jb0 + 1) * 4 * BLK, Mb);
+    }
+    __syncthreads();
+    if (low_cols) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int row = 32 * ib + 8 * (e >> 2) + 4 * h + (e & 3);
+          av[j][e] = fmaf(CC * RSC, acc[j][e], CB * av[j][e]) + (row == 32 * (jb0 + j) + lr && row < s.M ? CA * SC : 0.f);
+        }
+        put_direct(area2 + ((jb0 + j) * 4 + ib) * BLK, av[j], lr, h);
+      }
+    }
+    __syncthreads();
+  };
+
+  if (step == 0) {
+    const double f = scale_of<LOW_NT>(m, s, a.eps, sm);
+    f32x16 gram[2];
+    clear(gram);
+    for (int st = wg; st < s.strips(); st += wgs) {
+      clear(x);
+      if (low_rows) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const int row = 32 * ib + 8 * (e >> 2) + 4 * h + (e & 3), col = 32 * (4 * st + jb0 + j) + lr;
+            if (row < s.M && col < s.N) {
+              const long r = s.turned ? col : row, c = s.turned ? row : col;
+              const float v = MUON ? reinterpret_cast<const float*>(s.t1)[r * m.cols + c] : (float)((const T*)a.g)[m.off + r * m.ld + c];
+              x[j][e] = (float)((double)v * f);
+            }
+          }
+      }
+      if (wgs == 1) break;
+      __syncthreads();                          // (area1 may still be read for the strip before)
+      if (low_rows) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int jb = 4 * st + jb0 + j;
+          if (jb < s.Nb) put_direct(s.t0 + ((long)jb * Mb + ib) * BLK, x[j], lr, h);
+          put_turned(area1 + (ib * 4 + jb0 + j) * BLK, x[j], one, lr, h);
+        }
+      }
+      __syncthreads();
+      const char* u = area1 + lane * 16;
+      if (low_cols) low_product(gram, u + ib * 4 * BLK, u + jb0 * 4 * BLK, u + (jb0 + 1) * 4 * BLK, min(4, s.Nb - 4 * st));
+    }
+    if (wgs > 1) {
+      if (low_cols)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            *reinterpret_cast<float4*>(s.a + ((long)wg * 16 + ib * 4 + jb0 + j) * BLK + q * 1024 + lane * 16) =
+                make_float4(gram[j][4 * q], gram[j][4 * q + 1], gram[j][4 * q + 2], gram[j][4 * q + 3]);
+      return;
+    }
+    for (int k = 0; k < steps; ++k) {
+      if (low_rows)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) put_turned(area1 + (ib * 4 + jb0 + j) * BLK, x[j], one, lr, h);
+      __syncthreads();
+      clear(av);
+      const char *u1 = area1 + lane * 16, *u2 = area2 + lane * 16;
+      if (low_cols) {
+        low_product(av, u1 + ib * 4 * BLK, u1 + jb0 * 4 * BLK, u1 + (jb0 + 1) * 4 * BLK, s.Nb);
+        times(av, RSC);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) put_direct(area2 + ((jb0 + j) * 4 + ib) * BLK, av[j], lr, h);
+      }
+      __syncthreads();
+      if (low_rows)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) put_direct(area1 + ((jb0 + j) * 4 + ib) * BLK, x[j], lr, h);
+      form_poly();
+      clear(acc);
+      if (low_rows && jb0 < s.Nb) low_product(acc, u2 + ib * 4 * BLK, u1 + jb0 * 4 * BLK, u1 + (jb0 + 1) * 4 * BLK, Mb);
+      if (k + 1 < steps) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) x[j][e] = acc[j][e] * RSC;
+        __syncthreads();
+      }
+    }
+    if (low_rows)
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+        if (jb0 + j < s.Nb) write_block<T, MUON>(m, a, s, acc[j], ib, jb0 + j, lr, h);
+    return;
+  }
+
+  // a step of a longer matrix
+  const char *const shares = (step & 1) ? s.a : s.p, *const t_in = (step & 1) ? s.t0 : s.t1;
+  char *const shares_out = (step & 1) ? s.p : s.a, *const t_out = (step & 1) ? s.t1 : s.t0;
+  clear(av);
+  if (low_cols) {
+    for (int g = 0; g < wgs; ++g)
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const float4 v = *reinterpret_cast<const float4*>(shares + ((long)g * 16 + ib * 4 + jb0 + j) * BLK + q * 1024 + lane * 16);
+          av[j][4 * q] += v.x, av[j][4 * q + 1] += v.y, av[j][4 * q + 2] += v.z, av[j][4 * q + 3] += v.w;
+        }
+    times(av, RSC);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) put_direct(area2 + ((jb0 + j) * 4 + ib) * BLK, av[j], lr, h);
+  }
+  __syncthreads();
+  form_poly();
+  f32x16 gram[2];
+  clear(gram);
+  for (int st = wg; st < s.strips(); st += wgs) {
+    clear(x);
+    if (low_rows) {
+      const char* v = t_in + lane * 16;
+      low_product(x, area2 + lane * 16 + ib * 4 * BLK, v + (long)min(4 * st + jb0, s.Nb - 1) * Mb * BLK, v + (long)min(4 * st + jb0 + 1, s.Nb - 1) * Mb * BLK, Mb);
+    }
+    if (step == steps) {
+      if (low_rows)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+          if (4 * st + jb0 + j < s.Nb) write_block<T, MUON>(m, a, s, x[j], ib, 4 * st + jb0 + j, lr, h);
+      continue;
+    }
+    times(x, RSC);
+    __syncthreads();
+    if (low_rows) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int jb = 4 * st + jb0 + j;
+        if (jb < s.Nb) put_direct(t_out + ((long)jb * Mb + ib) * BLK, x[j], lr, h);
+        put_turned(area1 + (ib * 4 + jb0 + j) * BLK, x[j], one, lr, h);
+      }
+    }
+    __syncthreads();
+    const char* u = area1 + lane * 16;
+    if (low_cols) low_product(gram, u + ib * 4 * BLK, u + jb0 * 4 * BLK, u + (jb0 + 1) * 4 * BLK, min(4, s.Nb - 4 * st));
+  }
+  if (step < steps && low_cols)
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        *reinterpret_cast<float4*>(shares_out + ((long)wg * 16 + ib * 4 + jb0 + j) * BLK + q * 1024 + lane * 16) =
+            make_float4(gram[j][4 * q], gram[j][4 * q + 1], gram[j][4 * q + 2], gram[j][4 * q + 3]);
 }
 
 // ---- host side
@@ -663,18 +907,27 @@ int run(const char* who, const emx_matrix* mats, int n, const StepArgs& a, int s
     if (t.n == 0) break;
     auto half = [](int b) { return (long)(b + 1) / 2; };
     const auto parts = [](const Mat& m, const Scratch&) { return (long)parts_of((long)m.rows * m.cols); };
-    const auto full = [&](const Mat&, const Scratch& s) { return half(s.Mb) * half(s.Nb); };
-    const auto upper = [&](const Mat&, const Scratch& s) { return half(s.Mb) * (half(s.Mb) + 1) / 2; };
+    const auto full = [&](const Mat&, const Scratch& s) { return s.low() ? 0 : half(s.Mb) * half(s.Nb); };
+    const auto upper = [&](const Mat&, const Scratch& s) { return s.low() ? 0 : half(s.Mb) * (half(s.Mb) + 1) / 2; };
+    const auto low = [&](const Mat&, const Scratch& s) { return s.low() ? (long)s.low_wgs() : 0; };
+    const auto long_low = [&](const Mat&, const Scratch& s) { return s.low() && s.low_wgs() > 1 ? (long)s.low_wgs() : 0; };
     int rc;
     auto go = [&](auto kernel, long blocks, auto... more) {
+      if (blocks == 0) return (int)EMX_OK;
       EMX_REQUIRE(blocks < (1l << 31), "%s: %ld workgroups", who, blocks);
       hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(NT), 0, st, t, a, more...);
       return check_launch(who);
     };
     if ((rc = go(ns_norm_kernel<T, MUON>, number(t, parts)))) return rc;
     if ((rc = go(ns_split_kernel<T, MUON>, number(t, full)))) return rc;
-    const auto big_upper = [&](const Mat&, const Scratch& s) { return tile_count((s.Mb + BT_R - 1) / BT_R, (s.Mb + BT_C - 1) / BT_C, true); };
-    const auto big_full = [&](const Mat&, const Scratch& s) { return tile_count((s.Mb + BT_R - 1) / BT_R, (s.Nb + BT_C - 1) / BT_C, false); };
+    auto go_low = [&](long blocks, int step) {
+      if (blocks == 0) return (int)EMX_OK;
+      hipLaunchKernelGGL((ns_low_kernel<T, MUON>), dim3((unsigned)blocks), dim3(LOW_NT), 2 * LOW_AREA, st, t, a, step, steps);
+      return check_launch(who);
+    };
+    if ((rc = go_low(number(t, low), 0))) return rc;
+    const auto big_upper = [&](const Mat&, const Scratch& s) { return s.low() ? 0 : tile_count((s.Mb + BT_R - 1) / BT_R, (s.Mb + BT_C - 1) / BT_C, true); };
+    const auto big_full = [&](const Mat&, const Scratch& s) { return s.low() ? 0 : tile_count((s.Mb + BT_R - 1) / BT_R, (s.Nb + BT_C - 1) / BT_C, false); };
     const bool big = number(t, big_full) >= BIG_TILES;
     auto product = [&](auto small_kernel, auto big_kernel, bool up, int k) {
       if (big) {
@@ -688,7 +941,7 @@ int run(const char* who, const emx_matrix* mats, int n, const StepArgs& a, int s
       if ((rc = product(ns_product_kernel<POLY, T, MUON>, ns_big_kernel<POLY, T, MUON>, true, k))) return rc;
       if (k + 1 < steps) rc = product(ns_product_kernel<NEXT, T, MUON>, ns_big_kernel<NEXT, T, MUON>, false, k);
       else rc = product(ns_product_kernel<LAST, T, MUON>, ns_big_kernel<LAST, T, MUON>, false, k);
-      if (rc) return rc;
+      if (rc || (rc = go_low(number(t, long_low), k + 1))) return rc;
     }
   }
   return EMX_OK;
