@@ -38,6 +38,7 @@ constexpr int BLK = 4096;                     // bytes of an operand's 32 x 32 b
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef _Float16 half4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef unsigned uint4v __attribute__((ext_vector_type(4)));
 
 struct Mat {
   long off, ld;      // first element and row stride in the flat tensors
@@ -198,14 +199,11 @@ __device__ __forceinline__ double scale_of(const Mat& m, const Scratch& s, float
 
 // eight values of a row as the hi and lo units of an operand
 __device__ __forceinline__ void split_unit(const float (&v)[8], char* hi, char* lo) {
-  half8 h, l;
+  unsigned x[4], y[4];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    h[e] = (_Float16)v[e];
-    l[e] = (_Float16)(v[e] - (float)h[e]);
-  }
-  *reinterpret_cast<half8*>(hi) = h;
-  *reinterpret_cast<half8*>(lo) = l;
+  for (int p = 0; p < 4; ++p) split_f16_pair(v[2 * p], v[2 * p + 1], x[p], y[p]);
+  *reinterpret_cast<uint4v*>(hi) = uint4v{x[0], x[1], x[2], x[3]};
+  *reinterpret_cast<uint4v*>(lo) = uint4v{y[0], y[1], y[2], y[3]};
 }
 
 // ---- 2: X_0 and its transpose as operands: a workgroup per 64 x 64 of X
@@ -436,15 +434,15 @@ __device__ __forceinline__ void tile_of(int t, int tr, int tc, bool upper, int& 
   tj = c0 + t / h, ti = r0 + t % h;
 }
 
-// four values of a product's transpose (v: rows 8 q + 4 h .. + 3 of column lr) as they are stored
-__device__ __forceinline__ void split_quad(const float (&v)[4], half4& hi, half4& lo) {
+// The two planes of a 32 x 32 block as the registers hold it (x: element 4 q + r = row 8 q + 4 h + r of column lr): pairs of rows.
+// (x comes out of ordinary vector instructions: split_f16_pair's assembly may not read a matrix instruction's result as it is.)
+struct Planes {
+  unsigned hi[8], lo[8];
+  __device__ __forceinline__ explicit Planes(const f32x16& x) {
 #pragma unroll
-  for (int r = 0; r < 4; ++r) {
-    hi[r] = (_Float16)v[r];
-    lo[r] = (_Float16)(v[r] - (float)hi[r]);
+    for (int p = 0; p < 8; ++p) split_f16_pair(x[2 * p], x[2 * p + 1], hi[p], lo[p]);
   }
-}
-
+};
 // A permuted identity that turns a block by two matrix instructions: k-slot (h, e) of K-step ks stands for the block's row
 // 16 ks + 4 h + (e < 4 ? e : e + 4), which is where the accumulators of a product have it.
 __device__ __forceinline__ void identity(half8 (&one)[2], int lr, int h) {
@@ -453,45 +451,34 @@ __device__ __forceinline__ void identity(half8 (&one)[2], int lr, int h) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) one[ks][e] = (_Float16)(lr == 16 * ks + 4 * h + (e < 4 ? e : e + 4) ? 1.f : 0.f);
 }
-// a block of values (scaled) as operand planes: its transpose as it lies in the registers ...
-__device__ __forceinline__ void put_direct(char* block, const f32x16& x, int lr, int h) {
+// a block as an operand: its transpose as it lies in the registers ...
+__device__ __forceinline__ void put_direct(char* block, const Planes& x, int lr, int h) {
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
-    const float v[4] = {x[4 * q], x[4 * q + 1], x[4 * q + 2], x[4 * q + 3]};
-    half4 hi, lo;
-    split_quad(v, hi, lo);
     char* const to = block + (q >> 1) * 2048 + ((q & 1) * 32 + lr) * 16 + h * 8;
-    *reinterpret_cast<half4*>(to) = hi;
-    *reinterpret_cast<half4*>(to + 1024) = lo;
+    *reinterpret_cast<uint2*>(to) = make_uint2(x.hi[2 * q], x.hi[2 * q + 1]);
+    *reinterpret_cast<uint2*>(to + 1024) = make_uint2(x.lo[2 * q], x.lo[2 * q + 1]);
   }
 }
-// ... and the block itself, turned by matrix instructions
-__device__ __forceinline__ void put_turned(char* block, const f32x16& x, const half8 (&one)[2], int lr, int h) {
-  half4 hi[4], lo[4];
-#pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    const float v[4] = {x[4 * q], x[4 * q + 1], x[4 * q + 2], x[4 * q + 3]};
-    split_quad(v, hi[q], lo[q]);
-  }
+// ... and the block itself, turned by matrix instructions (their results are the planes' values: nothing is rounded)
+__device__ __forceinline__ void put_turned(char* block, const Planes& x, const half8 (&one)[2], int lr, int h) {
 #pragma unroll
   for (int plane = 0; plane < 2; ++plane) {
+    const unsigned(&v)[8] = plane ? x.lo : x.hi;
     f32x16 d;
 #pragma unroll
     for (int e = 0; e < 16; ++e) d[e] = 0.f;
 #pragma unroll
-    for (int ks = 0; ks < 2; ++ks) {
-      const half4 p0 = plane ? lo[2 * ks] : hi[2 * ks], p1 = plane ? lo[2 * ks + 1] : hi[2 * ks + 1];
-      d = __builtin_amdgcn_mfma_f32_32x32x16_f16(half8{p0[0], p0[1], p0[2], p0[3], p1[0], p1[1], p1[2], p1[3]}, one[ks], d, 0, 0, 0);
-    }
+    for (int ks = 0; ks < 2; ++ks)
+      d = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8, uint4v{v[4 * ks], v[4 * ks + 1], v[4 * ks + 2], v[4 * ks + 3]}), one[ks], d, 0, 0, 0);
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      half4 o;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) o[r] = (_Float16)d[4 * q + r];
-      *reinterpret_cast<half4*>(block + (q >> 1) * 2048 + ((q & 1) * 32 + lr) * 16 + h * 8 + plane * 1024) = o;
-    }
+    for (int q = 0; q < 4; ++q)
+      *reinterpret_cast<uint2*>(block + (q >> 1) * 2048 + ((q & 1) * 32 + lr) * 16 + h * 8 + plane * 1024) =
+          make_uint2(__builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_pkrtz(d[4 * q], d[4 * q + 1])),
+                     __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_pkrtz(d[4 * q + 2], d[4 * q + 3])));
   }
 }
+
 template <int KIND, typename T, bool MUON>
 __global__ __launch_bounds__(NT, 2) void ns_big_kernel(const Table tab, const StepArgs a, const int odd, const int total) {
   __shared__ __align__(16) char lds[2][BT_C * BLK];
@@ -622,56 +609,57 @@ __global__ __launch_bounds__(NT, 2) void ns_big_kernel(const Table tab, const St
             }
           }
         }
-        put_direct(O + ((long)jb * s.Mb + ib) * BLK, x, lr, h);
-        if (KIND == NEXT) put_turned(s.x + ((long)ib * s.Nb + jb) * BLK, x, one, lr, h);
-        else if (ib != jb) put_turned(O + ((long)ib * s.Mb + jb) * BLK, x, one, lr, h);
+        const Planes y(x);
+        put_direct(O + ((long)jb * s.Mb + ib) * BLK, y, lr, h);
+        if (KIND == NEXT) put_turned(s.x + ((long)ib * s.Nb + jb) * BLK, y, one, lr, h);
+        else if (ib != jb) put_turned(O + ((long)ib * s.Mb + jb) * BLK, y, one, lr, h);
       }
     }
   }
 }
 
-// ---- matrices of at most 128 rows: a workgroup of eight waves holds 128 columns of X in registers, wave w the blocks (w / 2, 2 (w % 2) + 0 .. 1).
-// The operands of the three products pass through two areas of LDS of 4 x 4 blocks: X, then X^T in the first, A, then P in the second.  A matrix
-// of at most 128 columns goes through all its steps in one launch.  A longer one is cut into strips of 128 columns: a launch per step, in
-// which EVERY workgroup adds up the shares of A that the launch before left (in their order), forms P, takes its strip on and leaves its
-// share of the next A -- two products of 128^3 more per workgroup than a division of the work would need, but 2 launches a step fewer.
-constexpr int LOW_NT = 512;
+// ---- matrices of at most 128 rows: a workgroup of sixteen waves holds 128 columns of X in registers, a wave one block.  The operands of the
+// three products pass through two areas of LDS of 4 x 4 blocks: X, then X^T in the first, A, then P in the second.  A matrix of at most
+// 128 columns goes through all its steps in one launch.  A longer one is cut into strips of 128 columns: a launch per step, in which EVERY
+// workgroup adds up the shares of A that the launch before left (in their order), forms P, takes its strip on and leaves its share of
+// the next A -- one product of 128^3 and the sum more per workgroup than a division of that work would need, but 2 launches a step fewer.
+// A and P are symmetric: the ten waves on and above the diagonal form them, dealt to the SIMDs by (row + column) % 4, three at most to each.
+// What bounds it is the LDS (512 KB a product at 128 bytes a clock; 72 matrix instructions a wave and step are 3.8 us) and what stands
+// between the barriers.  Two blocks a wave read a quarter less and are slower (two waves per SIMD: 59 us against 49 for five steps of
+// 128 x 128 before the symmetry was used, four blocks a wave 88).
+constexpr int LOW_NT = 1024;
 constexpr int LOW_AREA = 16 * BLK;
 
-// acc[j] += (row block u) (row block v_j)^T over nk blocks of k; u, v: this lane's 16 bytes of the first block
-__device__ __forceinline__ void low_k(f32x16 (&acc)[2], const char* u, const char* v0, const char* v1) {
+__device__ __forceinline__ void clear(f32x16& x) {
 #pragma unroll
-  for (int ks = 0; ks < 2; ++ks) {
-    const half8 uh = *reinterpret_cast<const half8*>(u + ks * 2048), ul = *reinterpret_cast<const half8*>(u + ks * 2048 + 1024);
-    const half8 h0 = *reinterpret_cast<const half8*>(v0 + ks * 2048), l0 = *reinterpret_cast<const half8*>(v0 + ks * 2048 + 1024);
-    const half8 h1 = *reinterpret_cast<const half8*>(v1 + ks * 2048), l1 = *reinterpret_cast<const half8*>(v1 + ks * 2048 + 1024);
-    acc[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(uh, l0, acc[0], 0, 0, 0);   // small products first
-    acc[1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(uh, l1, acc[1], 0, 0, 0);
-    acc[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ul, h0, acc[0], 0, 0, 0);
-    acc[1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ul, h1, acc[1], 0, 0, 0);
-    acc[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(uh, h0, acc[0], 0, 0, 0);
-    acc[1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(uh, h1, acc[1], 0, 0, 0);
+  for (int e = 0; e < 16; ++e) x[e] = 0.f;
+}
+__device__ __forceinline__ void times(f32x16& x, float f) {
+#pragma unroll
+  for (int e = 0; e < 16; ++e) x[e] *= f;
+}
+// acc += (row block u of one area) (row block v of the other)^T over nk blocks of k; u, v: this lane's 16 bytes of the first block
+__device__ __forceinline__ void low_product(f32x16& acc, const char* u, const char* v, int nk) {
+  half8 fu[2][2], fv[2][2];   // [K-step parity][plane]
+  auto read = [&](const int ks, const int k) __attribute__((always_inline)) {
+#pragma unroll
+    for (int plane = 0; plane < 2; ++plane) {
+      fu[ks][plane] = *reinterpret_cast<const half8*>(u + k * BLK + ks * 2048 + plane * 1024);
+      fv[ks][plane] = *reinterpret_cast<const half8*>(v + k * BLK + ks * 2048 + plane * 1024);
+    }
+  };
+  auto multiply = [&](const int ks) __attribute__((always_inline)) {
+#pragma unroll
+    for (int pass = 0; pass < 3; ++pass)        // small products first
+      acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(fu[ks][pass == 1], fv[ks][pass == 0], acc, 0, 0, 0);
+  };
+  read(0, 0);
+  for (int k = 0; k < nk; ++k) {
+    read(1, k);
+    multiply(0);
+    read(0, min(k + 1, nk - 1));
+    multiply(1);
   }
-}
-__device__ __forceinline__ void low_product(f32x16 (&acc)[2], const char* u, const char* v0, const char* v1, int nk) {
-  if (nk == 4) {
-#pragma unroll
-    for (int k = 0; k < 4; ++k) low_k(acc, u + k * BLK, v0 + k * BLK, v1 + k * BLK);
-  } else {
-    for (int k = 0; k < nk; ++k) low_k(acc, u + k * BLK, v0 + k * BLK, v1 + k * BLK);
-  }
-}
-__device__ __forceinline__ void clear(f32x16 (&x)[2]) {
-#pragma unroll
-  for (int j = 0; j < 2; ++j)
-#pragma unroll
-    for (int e = 0; e < 16; ++e) x[j][e] = 0.f;
-}
-__device__ __forceinline__ void times(f32x16 (&x)[2], float f) {
-#pragma unroll
-  for (int j = 0; j < 2; ++j)
-#pragma unroll
-    for (int e = 0; e < 16; ++e) x[j][e] *= f;
 }
 
 template <typename T, bool MUON>
@@ -684,167 +672,152 @@ __global__ __launch_bounds__(LOW_NT) void ns_low_kernel(const Table tab, const S
   const Mat m = tab.m[find(tab, blockIdx.x, wg)];
   const Scratch s(m.rows, m.cols, a.ws + m.ws);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int lr = lane & 31, h = lane >> 5, ib = wave >> 1, jb0 = 2 * (wave & 1);
+  const int lr = lane & 31, h = lane >> 5, ib = wave >> 2, jb = (wave - ib) & 3;
   const int wgs = s.low_wgs(), Mb = s.Mb;
-  const bool low_rows = ib < Mb, low_cols = low_rows && jb0 < Mb;
+  const bool rows = ib < Mb, square = ib <= jb && jb < Mb;   // this wave has a block of X; of the upper half of A and P
+  const char *const u1 = area1 + ib * 4 * BLK + lane * 16, *const u2 = area2 + ib * 4 * BLK + lane * 16;
+  const char *const v1 = area1 + jb * 4 * BLK + lane * 16, *const v2 = area2 + jb * 4 * BLK + lane * 16;
   half8 one[2];
   identity(one, lr, h);
-  f32x16 x[2], acc[2], av[2];
+  f32x16 x, av;
 
+  auto keep_symmetric = [&](char* area, const f32x16& z) __attribute__((always_inline)) {
+    const Planes y(z);
+    put_direct(area + (jb * 4 + ib) * BLK, y, lr, h);
+    if (ib != jb) put_turned(area + (ib * 4 + jb) * BLK, y, one, lr, h);
+  };
   auto form_poly = [&]() __attribute__((always_inline)) {   // av: A, area2: A (complete).  Leaves P in area2 (complete)
-    clear(acc);
-    if (low_cols) {
-      const char* u = area2 + lane * 16;
-      low_product(acc, u + ib * 4 * BLK, u + jb0 * 4 * BLK, u + (jb0 + 1) * 4 * BLK, Mb);
-    }
+    f32x16 sq;
+    clear(sq);
+    if (square) low_product(sq, u2, v2, Mb);
     __syncthreads();
-    if (low_cols) {
+    if (square) {
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int row = 32 * ib + 8 * (e >> 2) + 4 * h + (e & 3);
-          av[j][e] = fmaf(CC * RSC, acc[j][e], CB * av[j][e]) + (row == 32 * (jb0 + j) + lr && row < s.M ? CA * SC : 0.f);
-        }
-        put_direct(area2 + ((jb0 + j) * 4 + ib) * BLK, av[j], lr, h);
+      for (int e = 0; e < 16; ++e) {
+        const int row = 32 * ib + 8 * (e >> 2) + 4 * h + (e & 3);
+        av[e] = fmaf(CC * RSC, sq[e], CB * av[e]) + (row == 32 * jb + lr && row < s.M ? CA * SC : 0.f);
       }
+      keep_symmetric(area2, av);
     }
     __syncthreads();
+  };
+  auto share = [&](const char* shares, int g, int q) __attribute__((always_inline)) {
+    return reinterpret_cast<float4*>(const_cast<char*>(shares) + ((long)g * 16 + ib * 4 + jb) * BLK + q * 1024 + lane * 16);
+  };
+  auto leave_share = [&](char* shares, const f32x16& y) __attribute__((always_inline)) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) *share(shares, wg, q) = make_float4(y[4 * q], y[4 * q + 1], y[4 * q + 2], y[4 * q + 3]);
   };
 
   if (step == 0) {
     const double f = scale_of<LOW_NT>(m, s, a.eps, sm);
-    f32x16 gram[2];
+    f32x16 gram;
     clear(gram);
     for (int st = wg; st < s.strips(); st += wgs) {
       clear(x);
-      if (low_rows) {
+      if (rows) {
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const int row = 32 * ib + 8 * (e >> 2) + 4 * h + (e & 3), col = 32 * (4 * st + jb0 + j) + lr;
-            if (row < s.M && col < s.N) {
-              const long r = s.turned ? col : row, c = s.turned ? row : col;
-              const float v = MUON ? reinterpret_cast<const float*>(s.t1)[r * m.cols + c] : (float)((const T*)a.g)[m.off + r * m.ld + c];
-              x[j][e] = (float)((double)v * f);
-            }
+        for (int e = 0; e < 16; ++e) {
+          const int row = 32 * ib + 8 * (e >> 2) + 4 * h + (e & 3), col = 32 * (4 * st + jb) + lr;
+          if (row < s.M && col < s.N) {
+            const long r = s.turned ? col : row, c = s.turned ? row : col;
+            const float v = MUON ? reinterpret_cast<const float*>(s.t1)[r * m.cols + c] : (float)((const T*)a.g)[m.off + r * m.ld + c];
+            x[e] = (float)((double)v * f);
           }
+        }
       }
       if (wgs == 1) break;
       __syncthreads();                          // (area1 may still be read for the strip before)
-      if (low_rows) {
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const int jb = 4 * st + jb0 + j;
-          if (jb < s.Nb) put_direct(s.t0 + ((long)jb * Mb + ib) * BLK, x[j], lr, h);
-          put_turned(area1 + (ib * 4 + jb0 + j) * BLK, x[j], one, lr, h);
-        }
+      if (rows) {
+        const Planes y(x);
+        if (4 * st + jb < s.Nb) put_direct(s.t0 + ((long)(4 * st + jb) * Mb + ib) * BLK, y, lr, h);
+        put_turned(area1 + (ib * 4 + jb) * BLK, y, one, lr, h);
       }
       __syncthreads();
-      const char* u = area1 + lane * 16;
-      if (low_cols) low_product(gram, u + ib * 4 * BLK, u + jb0 * 4 * BLK, u + (jb0 + 1) * 4 * BLK, min(4, s.Nb - 4 * st));
+      if (square) low_product(gram, u1, v1, min(4, s.Nb - 4 * st));
     }
     if (wgs > 1) {
-      if (low_cols)
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-          for (int q = 0; q < 4; ++q)
-            *reinterpret_cast<float4*>(s.a + ((long)wg * 16 + ib * 4 + jb0 + j) * BLK + q * 1024 + lane * 16) =
-                make_float4(gram[j][4 * q], gram[j][4 * q + 1], gram[j][4 * q + 2], gram[j][4 * q + 3]);
+      if (square) leave_share(s.a, gram);
       return;
     }
     for (int k = 0; k < steps; ++k) {
-      if (low_rows)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) put_turned(area1 + (ib * 4 + jb0 + j) * BLK, x[j], one, lr, h);
+      const Planes y(x);
+      if (rows) put_turned(area1 + (ib * 4 + jb) * BLK, y, one, lr, h);
       __syncthreads();
       clear(av);
-      const char *u1 = area1 + lane * 16, *u2 = area2 + lane * 16;
-      if (low_cols) {
-        low_product(av, u1 + ib * 4 * BLK, u1 + jb0 * 4 * BLK, u1 + (jb0 + 1) * 4 * BLK, s.Nb);
+      if (square) {
+        low_product(av, u1, v1, s.Nb);
         times(av, RSC);
-#pragma unroll
-        for (int j = 0; j < 2; ++j) put_direct(area2 + ((jb0 + j) * 4 + ib) * BLK, av[j], lr, h);
+        keep_symmetric(area2, av);
       }
       __syncthreads();
-      if (low_rows)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) put_direct(area1 + ((jb0 + j) * 4 + ib) * BLK, x[j], lr, h);
+      if (rows) put_direct(area1 + (jb * 4 + ib) * BLK, y, lr, h);
       form_poly();
-      clear(acc);
-      if (low_rows && jb0 < s.Nb) low_product(acc, u2 + ib * 4 * BLK, u1 + jb0 * 4 * BLK, u1 + (jb0 + 1) * 4 * BLK, Mb);
+      clear(x);
+      if (rows && jb < s.Nb) low_product(x, u2, v1, Mb);
       if (k + 1 < steps) {
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) x[j][e] = acc[j][e] * RSC;
+        times(x, RSC);
         __syncthreads();
       }
     }
-    if (low_rows)
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-        if (jb0 + j < s.Nb) write_block<T, MUON>(m, a, s, acc[j], ib, jb0 + j, lr, h);
+    if (rows && jb < s.Nb) write_block<T, MUON>(m, a, s, x, ib, jb, lr, h);
     return;
   }
 
   // a step of a longer matrix
   const char *const shares = (step & 1) ? s.a : s.p, *const t_in = (step & 1) ? s.t0 : s.t1;
   char *const shares_out = (step & 1) ? s.p : s.a, *const t_out = (step & 1) ? s.t1 : s.t0;
+  half8 t[4];                                   // this wave's block of the strip's X^T on its way to area1: row block ib, k-block jb
+  auto request_t = [&](int st) __attribute__((always_inline)) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) t[q] = *reinterpret_cast<const half8*>(t_in + ((long)min(4 * st + ib, s.Nb - 1) * Mb + min(jb, Mb - 1)) * BLK + q * 1024 + lane * 16);
+  };
+  auto keep_t = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) *reinterpret_cast<half8*>(area1 + (ib * 4 + jb) * BLK + q * 1024 + lane * 16) = t[q];
+  };
+  request_t(wg);
   clear(av);
-  if (low_cols) {
+  if (square) {
+#pragma unroll 4
     for (int g = 0; g < wgs; ++g)
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const float4 v = *reinterpret_cast<const float4*>(shares + ((long)g * 16 + ib * 4 + jb0 + j) * BLK + q * 1024 + lane * 16);
-          av[j][4 * q] += v.x, av[j][4 * q + 1] += v.y, av[j][4 * q + 2] += v.z, av[j][4 * q + 3] += v.w;
-        }
+      for (int q = 0; q < 4; ++q) {
+        const float4 v = *share(shares, g, q);
+        av[4 * q] += v.x, av[4 * q + 1] += v.y, av[4 * q + 2] += v.z, av[4 * q + 3] += v.w;
+      }
     times(av, RSC);
-#pragma unroll
-    for (int j = 0; j < 2; ++j) put_direct(area2 + ((jb0 + j) * 4 + ib) * BLK, av[j], lr, h);
+    keep_symmetric(area2, av);
   }
+  keep_t();
   __syncthreads();
   form_poly();
-  f32x16 gram[2];
+  f32x16 gram;
   clear(gram);
   for (int st = wg; st < s.strips(); st += wgs) {
-    clear(x);
-    if (low_rows) {
-      const char* v = t_in + lane * 16;
-      low_product(x, area2 + lane * 16 + ib * 4 * BLK, v + (long)min(4 * st + jb0, s.Nb - 1) * Mb * BLK, v + (long)min(4 * st + jb0 + 1, s.Nb - 1) * Mb * BLK, Mb);
+    if (st != wg) {
+      __syncthreads();                          // (area1 may still be read for the strip before)
+      request_t(st);
+      keep_t();
+      __syncthreads();
     }
+    clear(x);
+    if (rows) low_product(x, u2, v1, Mb);
     if (step == steps) {
-      if (low_rows)
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-          if (4 * st + jb0 + j < s.Nb) write_block<T, MUON>(m, a, s, x[j], ib, 4 * st + jb0 + j, lr, h);
+      if (rows && 4 * st + jb < s.Nb) write_block<T, MUON>(m, a, s, x, ib, 4 * st + jb, lr, h);
       continue;
     }
     times(x, RSC);
     __syncthreads();
-    if (low_rows) {
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int jb = 4 * st + jb0 + j;
-        if (jb < s.Nb) put_direct(t_out + ((long)jb * Mb + ib) * BLK, x[j], lr, h);
-        put_turned(area1 + (ib * 4 + jb0 + j) * BLK, x[j], one, lr, h);
-      }
+    if (rows) {
+      const Planes y(x);
+      if (4 * st + jb < s.Nb) put_direct(t_out + ((long)(4 * st + jb) * Mb + ib) * BLK, y, lr, h);
+      put_turned(area1 + (ib * 4 + jb) * BLK, y, one, lr, h);
     }
     __syncthreads();
-    const char* u = area1 + lane * 16;
-    if (low_cols) low_product(gram, u + ib * 4 * BLK, u + jb0 * 4 * BLK, u + (jb0 + 1) * 4 * BLK, min(4, s.Nb - 4 * st));
+    if (square) low_product(gram, u1, v1, min(4, s.Nb - 4 * st));
   }
-  if (step < steps && low_cols)
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-      for (int q = 0; q < 4; ++q)
-        *reinterpret_cast<float4*>(shares_out + ((long)wg * 16 + ib * 4 + jb0 + j) * BLK + q * 1024 + lane * 16) =
-            make_float4(gram[j][4 * q], gram[j][4 * q + 1], gram[j][4 * q + 2], gram[j][4 * q + 3]);
+  if (step < steps && square) leave_share(shares_out, gram);
 }
 
 // ---- host side
