@@ -18,6 +18,7 @@
 // l % 32, rows 8 q + 4 (l / 32) + r -- are four consecutive k of an operand whose ROWS are the product's columns: a product writes its
 // transpose in operand layout straight from registers.  M and N are padded to 32 with zeros, which stay zero.
 #include <algorithm>
+#include <climits>
 #include <cstdint>
 #include <type_traits>
 #include <vector>
@@ -29,7 +30,7 @@ namespace {
 using namespace emx;
 
 constexpr int NT = 256;
-constexpr int MAX_TABLE = 64;                 // matrices of one launch
+constexpr int MAX_TABLE = 48;                 // matrices of one launch (the table is an argument of the first: 4 KB at most)
 constexpr int MAX_PARTS = 1024;               // shares of a matrix' sum of squares
 constexpr float CA = 3.4445f, CB = -4.7750f, CC = 2.0315f;
 constexpr float SC = 16384.f, RSC = 1.f / 16384.f;
@@ -40,17 +41,33 @@ typedef _Float16 half4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef unsigned uint4v __attribute__((ext_vector_type(4)));
 
+// the launches whose workgroups are numbered through the matrices
+enum { L_NORM = 0, L_SPLIT, L_LOW, L_LONG_LOW, L_UPPER, L_FULL, L_COUNT };
+
 struct Mat {
-  long off, ld;      // first element and row stride in the flat tensors
-  long ws;           // the matrix' scratch, from the workspace's begin
+  long off, ld;        // first element and row stride in the flat tensors
+  long ws;             // the matrix' scratch, from the workspace's begin
   int rows, cols;
-  float scale;       // of the update
-  int begin;         // the launch's first workgroup for this matrix
+  float scale;         // of the update
+  int begin[L_COUNT];  // each launch's first workgroup (or tile) for this matrix
 };
-struct Table {
+struct StepArgs {
+  const void* g;       // gradients: flat buffer, or (slices) the parts of their sum
+  void* out;           // orthogonalize: the result's flat buffer
+  float *w, *mom;      // optimizer step
+  long slice_stride;
+  int n_slices, nesterov, steps;
+  float beta, keep, lr, eps;    // keep = 1 - lr weight_decay
+};
+// Everything a call is about.  The first launch gets it as an argument and leaves a copy at the workspace's begin, from which the others read it:
+// an argument of this size comes from host memory at microseconds a dependent load, the copy out of the L2.
+struct alignas(16) Table {
+  StepArgs a;
   int n;
   Mat m[MAX_TABLE];
 };
+constexpr long TABLE_BYTES = 4096;
+static_assert(sizeof(Table) <= 4032 && sizeof(Table) % 16 == 0, "the first launch's arguments");
 
 // The scratch of one matrix: the shares of its sum of squares, X^T twice (read and written by a step; the second also holds the optimizer step's
 // direction u at the begin) and, M > 128: X, A and P; M <= 128: the shares of A twice, 16 blocks from each workgroup.
@@ -84,27 +101,17 @@ struct Scratch {
 // (1024 elements and more to a share: the optimizer step reads up to 32 gradient parts of each)
 __host__ __device__ inline int parts_of(long n) { return (int)(n <= 1024l * MAX_PARTS ? (n + 1023) / 1024 : MAX_PARTS); }
 
-// the matrix a workgroup belongs to, and its number inside it
-__device__ __forceinline__ int find(const Table& t, int block, int& inside) {
-  int lo = 0, hi = t.n - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (t.m[mid].begin <= block) lo = mid;
-    else hi = mid - 1;
+// the matrix a workgroup (or tile) belongs to, and its number inside it: all lanes look at once
+__device__ __forceinline__ int find(const Mat* m, int n, int launch, int block, int& inside) {
+  int at = 0;
+  if (n > 1) {
+    const int lane = threadIdx.x & 63;
+    const bool before = lane < n && m[lane].begin[launch] <= block;
+    at = __builtin_amdgcn_readfirstlane(__popcll(__ballot(before))) - 1;
   }
-  inside = block - t.m[lo].begin;
-  return lo;
+  inside = block - m[at].begin[launch];
+  return at;
 }
-
-struct StepArgs {
-  const void* g;       // gradients: flat buffer, or (slices) the parts of their sum
-  void* out;           // orthogonalize: the result's flat buffer
-  float *w, *mom;      // optimizer step
-  char* ws;
-  long slice_stride;
-  int n_slices, nesterov;
-  float beta, keep, lr, eps;    // keep = 1 - lr weight_decay
-};
 
 // ---- 1: the sum of squares in shares; the optimizer step also forms its update's direction u here.  Four consecutive elements per
 // thread at a time where the rows allow it (their length is a multiple of 4), the parts of a gradient eight at a time.
@@ -166,11 +173,16 @@ __device__ __forceinline__ double wave_sum64(double v) {
   return v;
 }
 template <typename T, bool MUON>
-__global__ __launch_bounds__(NT) void ns_norm_kernel(const Table tab, const StepArgs a) {
+__global__ __launch_bounds__(NT) void ns_norm_kernel(char* ws, const Table tab) {
   __shared__ double sm[NT / 64];
+  if (blockIdx.x == 0) {                        // (not read in this launch)
+    const int4* const from = reinterpret_cast<const int4*>(&tab);
+    for (int i = threadIdx.x; i < (int)(sizeof(Table) / 16); i += NT) reinterpret_cast<int4*>(ws)[i] = from[i];
+  }
   int part;
-  const Mat m = tab.m[find(tab, blockIdx.x, part)];
-  const Scratch s(m.rows, m.cols, a.ws + m.ws);
+  const StepArgs& a = tab.a;
+  const Mat m = tab.m[find(tab.m, tab.n, L_NORM, blockIdx.x, part)];
+  const Scratch s(m.rows, m.cols, ws + m.ws);
   const unsigned total = (unsigned)m.rows * m.cols;
   const int parts = parts_of(total);
   const unsigned chunk = ((total + parts - 1) / parts + 3) & ~3u;
@@ -208,12 +220,14 @@ __device__ __forceinline__ void split_unit(const float (&v)[8], char* hi, char* 
 
 // ---- 2: X_0 and its transpose as operands: a workgroup per 64 x 64 of X
 template <typename T, bool MUON>
-__global__ __launch_bounds__(NT) void ns_split_kernel(const Table tab, const StepArgs a) {
+__global__ __launch_bounds__(NT) void ns_split_kernel(char* ws, const int n) {
   __shared__ float tile[64][65];
   __shared__ double sm[NT / 64];
+  const Table& tab = *reinterpret_cast<const Table*>(ws);
+  const StepArgs& a = tab.a;
   int inside;
-  const Mat m = tab.m[find(tab, blockIdx.x, inside)];
-  const Scratch s(m.rows, m.cols, a.ws + m.ws);
+  const Mat m = tab.m[find(tab.m, n, L_SPLIT, blockIdx.x, inside)];
+  const Scratch s(m.rows, m.cols, ws + m.ws);
   const int tid = threadIdx.x;
   const int tn = (s.Nb + 1) / 2, ti = inside / tn, tj = inside - ti * tn;
   const double f = scale_of<NT>(m, s, a.eps, sm);
@@ -244,13 +258,6 @@ __global__ __launch_bounds__(NT) void ns_split_kernel(const Table tab, const Ste
 
 // ---- 3: the products.  KIND 0: A = X X^T; 1: P = a I + b A + c A A^T; 2: X <- P X; 3: the last step's X, written out
 enum { GRAM = 0, POLY = 1, NEXT = 2, LAST = 3 };
-__device__ __forceinline__ void triangle(int t, int nb, int& ti, int& tj) {   // row-major over ti <= tj
-  ti = (int)((2.f * nb + 1.f - sqrtf((2.f * nb + 1.f) * (2.f * nb + 1.f) - 8.f * t)) * 0.5f);
-  while (ti > 0 && ti * nb - ti * (ti - 1) / 2 > t) --ti;
-  while ((ti + 1) * nb - (ti + 1) * ti / 2 <= t) ++ti;
-  tj = ti + t - (ti * nb - ti * (ti - 1) / 2);
-}
-
 // A 32 x 32 block of the last X into the caller's tensors (x: row 32 ib + 8 q + 4 h + r, column 32 jb + lr, scaled by 2^28): the update of w, or
 // the result.  All of a block's reads stand in front of its writes.  A turned matrix has four consecutive elements per lane.
 template <typename T, bool MUON>
@@ -306,130 +313,45 @@ __device__ __forceinline__ void write_block(const Mat& m, const StepArgs& a, con
   }
 }
 
-template <int KIND, typename T, bool MUON>
-__global__ __launch_bounds__(NT) void ns_product_kernel(const Table tab, const StepArgs a, const int odd) {
-  int inside;
-  const Mat m = tab.m[find(tab, blockIdx.x, inside)];
-  const Scratch s(m.rows, m.cols, a.ws + m.ws);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int lr = lane & 31, h = lane >> 5;
-  char *const t_in = odd ? s.t1 : s.t0, *const t_out = odd ? s.t0 : s.t1;
-  int ti, tj;
-  if constexpr (KIND <= POLY) {
-    triangle(inside, (s.Mb + 1) / 2, ti, tj);
-  } else {
-    const int tn = (s.Nb + 1) / 2;
-    ti = inside / tn, tj = inside - ti * tn;
-  }
-  const int ib = 2 * ti + (wave >> 1), jb = 2 * tj + (wave & 1);     // this wave's 32 x 32 block of the product
-  const int Jb = KIND <= POLY ? s.Mb : s.Nb, Kb = KIND == GRAM ? s.Nb : s.Mb;
-  if (ib >= s.Mb || jb >= Jb) return;
-  const char* U = (KIND == GRAM ? s.x : KIND == POLY ? s.a : s.p) + (long)ib * Kb * BLK + lane * 16;
-  const char* V = (KIND == GRAM ? s.x : KIND == POLY ? s.a : t_in) + (long)jb * Kb * BLK + lane * 16;
-  // Long sums in two levels: an accumulator takes 256 k (48 additions), then joins the sum.  (One chain over 4096 k rounds 768 times: 8e-6 of
-  // the result where float32 in blocks is off by 1e-6.)
-  f32x16 sum, acc, zero;
-#pragma unroll
-  for (int i = 0; i < 16; ++i) sum[i] = zero[i] = 0.f;
-  for (int k0 = 0; k0 < 2 * Kb; k0 += 16) {
-    const int k1 = min(k0 + 16, 2 * Kb);
-    acc = zero;
-    for (int k = k0; k < k1; ++k) {
-      const half8 uh = *reinterpret_cast<const half8*>(U + k * 2048l), ul = *reinterpret_cast<const half8*>(U + k * 2048l + 1024);
-      const half8 vh = *reinterpret_cast<const half8*>(V + k * 2048l), vl = *reinterpret_cast<const half8*>(V + k * 2048l + 1024);
-      acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(uh, vl, acc, 0, 0, 0);   // small products first
-      acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(ul, vh, acc, 0, 0, 0);
-      acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(uh, vh, acc, 0, 0, 0);
-    }
-#pragma unroll
-    for (int i = 0; i < 16; ++i) sum[i] += acc[i];
-  }
-  acc = sum;
-  // acc[4 q + r]: row 32 ib + 8 q + 4 h + r, column 32 jb + lr
-  if constexpr (KIND == LAST) {
-    write_block<T, MUON>(m, a, s, acc, ib, jb, lr, h);
-  } else {
-    char* const O = KIND == GRAM ? s.a : KIND == POLY ? s.p : t_out;
-    const int rows_b = KIND == NEXT ? s.Mb : s.Mb;                   // blocks along k of the transposed result
-    char* const direct = O + ((long)jb * rows_b + ib) * BLK;         // rows: the product's columns; k: its rows
-    char* const other = KIND == NEXT ? s.x + ((long)ib * s.Nb + jb) * BLK : ib != jb ? O + ((long)ib * s.Mb + jb) * BLK : nullptr;
-    const bool both = KIND == NEXT || ti != tj;                      // (a diagonal tile's four blocks are all computed)
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const int at = (q >> 1) * 2048 + ((q & 1) * 32 + lr) * 16 + h * 8;
-      float v[4];
-#pragma unroll
-      for (int r = 0; r < 4; ++r) v[r] = acc[4 * q + r] * RSC;
-      if constexpr (KIND == POLY) {
-        const char* am = s.a + ((long)jb * s.Mb + ib) * BLK + at;    // A is symmetric: the same four of its transpose
-        const half4 ah = *reinterpret_cast<const half4*>(am), al = *reinterpret_cast<const half4*>(am + 1024);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          v[r] = fmaf(CC, v[r], CB * ((float)ah[r] + (float)al[r]));
-          if (ib == jb && 8 * q + 4 * h + r == lr && 32 * ib + lr < s.M) v[r] += CA * SC;
-        }
-      }
-      half4 hi, lo;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        hi[r] = (_Float16)v[r];
-        lo[r] = (_Float16)(v[r] - (float)hi[r]);
-      }
-      *reinterpret_cast<half4*>(direct + at) = hi;
-      *reinterpret_cast<half4*>(direct + at + 1024) = lo;
-      if (both) {
-        // rows: the product's rows; k: its columns
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int b = (lr >> 4) * 2048 + (((lr >> 3) & 1) * 32 + 8 * q + 4 * h + r) * 16 + (lr & 7) * 2;
-          *reinterpret_cast<_Float16*>(other + b) = hi[r];
-          *reinterpret_cast<_Float16*>(other + b + 1024) = lo[r];
-        }
-      }
-    }
-  }
-}
-
-// ---- the same products in tiles of 256 x 128 for large matrices: four waves, 64 x 128 each.  A wave's operand of 64 rows is its own and
-// goes from global memory into registers (every piece is what a matrix instruction reads); the operand of 128 columns is shared through LDS.
+// ---- 3: the products, in tiles of 256 x 128 or 128 x 128 (RB = 2, 1): four waves, RB 32 x 128 each.  A wave's operand of RB 32 rows is its own
+// and goes from global memory into registers (every piece is what a matrix instruction reads); the operand of 128 columns is shared through LDS.
 // Per 32 k a workgroup reads 48 KB for 192 matrix instructions, its LDS traffic is 80 KB: 32 and 52 bytes a clock at their full rate.
-constexpr int BT_R = 8, BT_C = 4;             // blocks of 32 a tile has: rows, columns
+constexpr int BT_C = 4;                       // blocks of 32 a tile has: columns; 4 RB rows
 // tiles of a product, in the order they are handed out: bands of 4 tile rows, column by column inside a band
 constexpr int BAND = 4;
-constexpr long BIG_TILES = 64;
-__host__ __device__ inline long band_count(int r0, int tr, int tc, bool upper) {
+__host__ __device__ inline long band_count(int r0, int tr, int tc, int rb, bool upper) {
   const int h = min(BAND, tr - r0);
   if (!upper) return (long)h * tc;
-  const int nc = tc - 2 * r0;                 // columns from the diagonal on: column 2 r0 + d has min(h, d / 2 + 1) tiles
-  if (nc >= 2 * h) return h * (h + 1) + (long)(nc - 2 * h) * h;
-  const int k = nc / 2;
-  return k * (k + 1) + (nc & 1) * (k + 1);
+  const int nc = tc - rb * r0;                // columns from the diagonal on: column rb r0 + d has min(h, d / rb + 1) tiles
+  if (nc >= rb * h) return rb * h * (h + 1) / 2 + (long)(nc - rb * h) * h;
+  const int k = nc / rb;
+  return rb * k * (k + 1) / 2 + (nc % rb) * (k + 1);
 }
-__host__ __device__ inline long tile_count(int tr, int tc, bool upper) {
+__host__ __device__ inline long tile_count(int tr, int tc, int rb, bool upper) {
   long n = 0;
-  for (int r0 = 0; r0 < tr && (!upper || 2 * r0 < tc); r0 += BAND) n += band_count(r0, tr, tc, upper);
+  for (int r0 = 0; r0 < tr && (!upper || rb * r0 < tc); r0 += BAND) n += band_count(r0, tr, tc, rb, upper);
   return n;
 }
-__device__ __forceinline__ void tile_of(int t, int tr, int tc, bool upper, int& ti, int& tj) {
+__device__ __forceinline__ void tile_of(int t, int tr, int tc, int rb, bool upper, int& ti, int& tj) {
   int r0 = 0;
   for (;;) {
-    const int n = (int)band_count(r0, tr, tc, upper);
+    const int n = (int)band_count(r0, tr, tc, rb, upper);
     if (t < n || r0 + BAND >= tr) break;
     t -= n, r0 += BAND;
   }
   const int h = min(BAND, tr - r0);
   int c0 = 0;
   if (upper) {
-    c0 = 2 * r0;
-    for (int d = 0; d < 2 * h; ++d) {
-      const int n = d / 2 + 1;
+    c0 = rb * r0;
+    for (int d = 0; d < rb * h; ++d) {
+      const int n = d / rb + 1;
       if (t < n) {
         ti = r0 + t, tj = c0 + d;
         return;
       }
       t -= n;
     }
-    c0 += 2 * h;
+    c0 += rb * h;
   }
   tj = c0 + t / h, ti = r0 + t % h;
 }
@@ -479,43 +401,77 @@ __device__ __forceinline__ void put_turned(char* block, const Planes& x, const h
   }
 }
 
+// A block of a product where it belongs (x: element 4 q + r = row 32 ib + 8 q + 4 h + r of column 32 jb + lr, scaled by 2^28)
 template <int KIND, typename T, bool MUON>
-__global__ __launch_bounds__(NT, 2) void ns_big_kernel(const Table tab, const StepArgs a, const int odd, const int total) {
+__device__ __forceinline__ void store_block(const Mat& m, const StepArgs& a, const Scratch& s, f32x16 x, int ib, int jb, char* t_out, int lr, int h) {
+  if (ib >= s.Mb || jb >= (KIND <= POLY ? s.Mb : s.Nb) || (KIND <= POLY && ib > jb)) return;   // (A and P: the upper half, stored twice)
+  if constexpr (KIND == LAST) {
+    write_block<T, MUON>(m, a, s, x, ib, jb, lr, h);
+  } else {
+    half8 one[2];
+    identity(one, lr, h);
+    char* const O = KIND == GRAM ? s.a : KIND == POLY ? s.p : t_out;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) x[e] *= RSC;
+    if constexpr (KIND == POLY) {
+      const char* const am = s.a + ((long)jb * s.Mb + ib) * BLK + lr * 16 + h * 8;    // A is symmetric: the same four of its transpose
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int to = (q >> 1) * 2048 + (q & 1) * 512;
+        const half4 ah = *reinterpret_cast<const half4*>(am + to), al = *reinterpret_cast<const half4*>(am + to + 1024);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          x[4 * q + r] = fmaf(CC, x[4 * q + r], CB * ((float)ah[r] + (float)al[r]));
+          if (ib == jb && 8 * q + 4 * h + r == lr && 32 * ib + lr < s.M) x[4 * q + r] += CA * SC;
+        }
+      }
+    }
+    const Planes y(x);
+    put_direct(O + ((long)jb * s.Mb + ib) * BLK, y, lr, h);
+    if (KIND == NEXT) put_turned(s.x + ((long)ib * s.Nb + jb) * BLK, y, one, lr, h);
+    else if (ib != jb) put_turned(O + ((long)ib * s.Mb + jb) * BLK, y, one, lr, h);
+  }
+}
+
+template <int KIND, typename T, bool MUON, int RB>
+__global__ __launch_bounds__(NT, RB == 2 ? 2 : 3) void ns_big_kernel(char* ws, const int n, const int odd, const int total, const int run) {
   __shared__ __align__(16) char lds[2][BT_C * BLK];
-  // one eighth of the tiles to each XCD, consecutive ones: they share operands in its L2
-  const int per = (total + 7) >> 3, at = (int)(blockIdx.x & 7) * per + (int)(blockIdx.x >> 3);
+  // runs of consecutive tiles to each XCD: they share operands in its L2
+  const int turn = (int)(blockIdx.x >> 3), at = ((turn / run) * 8 + (int)(blockIdx.x & 7)) * run + turn % run;
   if (at >= total) return;
   int inside;
-  const Mat m = tab.m[find(tab, at, inside)];
-  const Scratch s(m.rows, m.cols, a.ws + m.ws);
+  const Table& tab = *reinterpret_cast<const Table*>(ws);
+  const StepArgs& a = tab.a;
+  const Mat m = tab.m[find(tab.m, n, KIND <= POLY ? L_UPPER : L_FULL, at, inside)];
+  const Scratch s(m.rows, m.cols, ws + m.ws);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lr = lane & 31, h = lane >> 5;
   char *const t_in = odd ? s.t1 : s.t0, *const t_out = odd ? s.t0 : s.t1;
   const int Jb = KIND <= POLY ? s.Mb : s.Nb, Kb = KIND == GRAM ? s.Nb : s.Mb;
   int ti, tj;
-  tile_of(inside, (s.Mb + BT_R - 1) / BT_R, (Jb + BT_C - 1) / BT_C, KIND <= POLY, ti, tj);
-  const int ib0 = BT_R * ti + 2 * wave, jb0 = BT_C * tj;
+  tile_of(inside, (s.Mb + 4 * RB - 1) / (4 * RB), (Jb + BT_C - 1) / BT_C, RB, KIND <= POLY, ti, tj);
+  const int ib0 = RB * (4 * ti + wave), jb0 = BT_C * tj;   // this wave's first blocks
   const char* const Ub = KIND == GRAM ? s.x : KIND == POLY ? s.a : s.p;
   const char* const Vb = KIND == GRAM ? s.x : KIND == POLY ? s.a : t_in;
   // (blocks beyond the matrix are read from its last one and not stored)
-  const char* U[2];
+  const char* U[RB];
 #pragma unroll
-  for (int i = 0; i < 2; ++i) U[i] = Ub + (long)min(ib0 + i, s.Mb - 1) * Kb * BLK + lane * 16;
+  for (int i = 0; i < RB; ++i) U[i] = Ub + (long)min(ib0 + i, s.Mb - 1) * Kb * BLK + lane * 16;
   const char* V = Vb + (long)min(jb0 + wave, Jb - 1) * Kb * BLK + lane * 16;   // this wave's block of the shared operand
-  f32x16 acc[2][BT_C];
+  f32x16 acc[RB][BT_C];
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+  for (int i = 0; i < RB; ++i)
 #pragma unroll
     for (int j = 0; j < BT_C; ++j)
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
-  // The k loop is written in the order it is to run: a GROUP is two blocks of columns of one K-step, 12 matrix instructions on four
+  // The k loop is written in the order it is to run: a GROUP is two blocks of columns of one K-step, 6 RB matrix instructions on 2 RB
   // accumulators; the next group's reads of LDS stand in front of them (the compiler left to itself puts each read right before its use),
   // and no load is conditional (the last ones are repeated), which keeps the counts of loads in flight exact.
-  half8 u[2][2][2], v[4], w[2][2][2];           // [K-step][block][plane]; the shared operand's next block; [group parity][column block][plane]
+  half8 u[2][RB][2], v[4], w[2][2][2];           // [K-step][block][plane]; the shared operand's next block; [group parity][column block][plane]
   auto request_u = [&](const int ks, const long k) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < RB; ++i) {
       u[ks][i][0] = *reinterpret_cast<const half8*>(U[i] + k * BLK + ks * 2048);
       u[ks][i][1] = *reinterpret_cast<const half8*>(U[i] + k * BLK + ks * 2048 + 1024);
     }
@@ -542,7 +498,7 @@ __global__ __launch_bounds__(NT, 2) void ns_big_kernel(const Table tab, const St
 #pragma unroll
       for (int j = 0; j < 2; ++j)
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < RB; ++i)
           acc[i][j0 + j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(u[ks][i][pass == 1], w[g & 1][j][pass == 0], acc[i][j0 + j], 0, 0, 0);
   };
   request_v(0);
@@ -577,45 +533,108 @@ __global__ __launch_bounds__(NT, 2) void ns_big_kernel(const Table tab, const St
     __builtin_amdgcn_sched_barrier(0);
     request_u(1, min(k + 1, Kb - 1));
   }
-  // acc[i][j][4 q + r]: row 32 (ib0 + i) + 8 q + 4 h + r, column 32 (jb0 + j) + lr
-  if constexpr (KIND == LAST) {
+#pragma unroll
+  for (int i = 0; i < RB; ++i)
+#pragma unroll
+    for (int j = 0; j < BT_C; ++j) store_block<KIND, T, MUON>(m, a, s, acc[i][j], ib0 + i, jb0 + j, t_out, lr, h);
+}
+
+// ---- the products in tiles of 64 x 64, for matrices that would leave most of the machine idle in larger ones: the four waves of a
+// workgroup take a quarter of k each, straight from global memory (four K-steps of operands in registers: three travel under the products of
+// one), and add up through LDS, a block to each wave.
+template <int KIND, typename T, bool MUON>
+__global__ __launch_bounds__(NT, 2) void ns_mid_kernel(char* ws, const int n, const int odd, const int total, const int run) {
+  __shared__ __align__(16) float4 fold[4][3][4][64];   // [block][wave but its own][q][lane]
+  const int turn = (int)(blockIdx.x >> 3), at = ((turn / run) * 8 + (int)(blockIdx.x & 7)) * run + turn % run;
+  if (at >= total) return;
+  int inside;
+  const Table& tab = *reinterpret_cast<const Table*>(ws);
+  const StepArgs& a = tab.a;
+  const Mat m = tab.m[find(tab.m, n, KIND <= POLY ? L_UPPER : L_FULL, at, inside)];
+  const Scratch s(m.rows, m.cols, ws + m.ws);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lr = lane & 31, h = lane >> 5;
+  char *const t_in = odd ? s.t1 : s.t0, *const t_out = odd ? s.t0 : s.t1;
+  const int Jb = KIND <= POLY ? s.Mb : s.Nb, Kb = KIND == GRAM ? s.Nb : s.Mb;
+  int ti, tj;
+  tile_of(inside, (s.Mb + 1) / 2, (Jb + 1) / 2, 1, KIND <= POLY, ti, tj);
+  const int ib0 = 2 * ti, jb0 = 2 * tj;
+  const char* const Ub = KIND == GRAM ? s.x : KIND == POLY ? s.a : s.p;
+  const char* const Vb = KIND == GRAM ? s.x : KIND == POLY ? s.a : t_in;
+  // (blocks beyond the matrix are read from its last one and not stored)
+  const char *U[2], *V[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    U[i] = Ub + (long)min(ib0 + i, s.Mb - 1) * Kb * BLK + lane * 16;
+    V[i] = Vb + (long)min(jb0 + i, Jb - 1) * Kb * BLK + lane * 16;
+  }
+  const int k0 = 2 * (wave * Kb / 4), k1 = 2 * ((wave + 1) * Kb / 4);   // this wave's K-steps
+  f32x16 acc[2][2];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) acc[i >> 1][i & 1][e] = 0.f;
+  half8 f[4][2][2][2];                          // [K-step % 4][operand][block][plane]
+  auto request = [&](const int slot, const int k) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int j = 0; j < BT_C; ++j) write_block<T, MUON>(m, a, s, acc[i][j], ib0 + i, jb0 + j, lr, h);
-  } else {
-    char* const O = KIND == GRAM ? s.a : KIND == POLY ? s.p : t_out;
-    half8 one[2];
-    identity(one, lr, h);
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-#pragma unroll
-      for (int j = 0; j < BT_C; ++j) {
-        const int ib = ib0 + i, jb = jb0 + j;
-        if (ib >= s.Mb || jb >= Jb || (KIND <= POLY && ib > jb)) continue;
-        f32x16 x;
-#pragma unroll
-        for (int e = 0; e < 16; ++e) x[e] = acc[i][j][e] * RSC;
-        if constexpr (KIND == POLY) {
-          const char* const am = s.a + ((long)jb * s.Mb + ib) * BLK + lr * 16 + h * 8;    // A is symmetric: the same four of its transpose
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const int to = (q >> 1) * 2048 + (q & 1) * 512;
-            const half4 ah = *reinterpret_cast<const half4*>(am + to), al = *reinterpret_cast<const half4*>(am + to + 1024);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              x[4 * q + r] = fmaf(CC, x[4 * q + r], CB * ((float)ah[r] + (float)al[r]));
-              if (ib == jb && 8 * q + 4 * h + r == lr && 32 * ib + lr < s.M) x[4 * q + r] += CA * SC;
-            }
-          }
-        }
-        const Planes y(x);
-        put_direct(O + ((long)jb * s.Mb + ib) * BLK, y, lr, h);
-        if (KIND == NEXT) put_turned(s.x + ((long)ib * s.Nb + jb) * BLK, y, one, lr, h);
-        else if (ib != jb) put_turned(O + ((long)ib * s.Mb + jb) * BLK, y, one, lr, h);
+      for (int plane = 0; plane < 2; ++plane) {
+        f[slot][0][i][plane] = *reinterpret_cast<const half8*>(U[i] + k * 2048l + plane * 1024);
+        f[slot][1][i][plane] = *reinterpret_cast<const half8*>(V[i] + k * 2048l + plane * 1024);
       }
+  };
+  const int last = max(k1, 1) - 1;
+  request(0, min(k0, last));
+  asm volatile("" ::: "memory");
+  request(1, min(k0 + 1, last));
+  asm volatile("" ::: "memory");
+  request(2, min(k0 + 2, last));
+  asm volatile("" ::: "memory");
+  for (int k = k0; k < k1; k += 4) {
+#pragma unroll
+    for (int slot = 0; slot < 4; ++slot) {
+      request((slot + 3) & 3, min(k + slot + 3, last));
+      __builtin_amdgcn_sched_barrier(0);
+      if (k + slot < k1) {
+#pragma unroll
+        for (int pass = 0; pass < 3; ++pass)    // small products first
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+              acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[slot][0][i][pass == 1], f[slot][1][j][pass == 0], acc[i][j], 0, 0, 0);
+      }
+      __builtin_amdgcn_sched_barrier(0);
     }
   }
+  // block b of the tile: wave b adds up the four waves' shares, in their order
+#pragma unroll
+  for (int b = 0; b < 4; ++b)
+    if (b != wave)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const f32x16& y = acc[b >> 1][b & 1];
+        fold[b][wave - (wave > b)][q][lane] = make_float4(y[4 * q], y[4 * q + 1], y[4 * q + 2], y[4 * q + 3]);
+      }
+  __syncthreads();
+  f32x16 x;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) x[e] = wave == 0 ? acc[0][0][e] : wave == 1 ? acc[0][1][e] : wave == 2 ? acc[1][0][e] : acc[1][1][e];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    float4 p[3];
+#pragma unroll
+    for (int i = 0; i < 3; ++i) p[i] = fold[wave][i][q][lane];
+    const float4 own = make_float4(x[4 * q], x[4 * q + 1], x[4 * q + 2], x[4 * q + 3]);
+    const float4 s0 = wave == 0 ? own : p[0], s1 = wave == 1 ? own : wave == 0 ? p[0] : p[1], s2 = wave == 2 ? own : wave == 3 ? p[2] : p[1],
+                 s3 = wave == 3 ? own : p[2];
+    x[4 * q] = (s0.x + s1.x) + (s2.x + s3.x);
+    x[4 * q + 1] = (s0.y + s1.y) + (s2.y + s3.y);
+    x[4 * q + 2] = (s0.z + s1.z) + (s2.z + s3.z);
+    x[4 * q + 3] = (s0.w + s1.w) + (s2.w + s3.w);
+  }
+  store_block<KIND, T, MUON>(m, a, s, x, ib0 + (wave >> 1), jb0 + (wave & 1), t_out, lr, h);
 }
 
 // ---- matrices of at most 128 rows: a workgroup of sixteen waves holds 128 columns of X in registers, a wave one block.  The operands of the
@@ -663,14 +682,16 @@ __device__ __forceinline__ void low_product(f32x16& acc, const char* u, const ch
 }
 
 template <typename T, bool MUON>
-__global__ __launch_bounds__(LOW_NT) void ns_low_kernel(const Table tab, const StepArgs a, const int step /* 0: X_0 and its A (or everything) */,
-                                                        const int steps) {
+__global__ __launch_bounds__(LOW_NT) void ns_low_kernel(char* ws, const int n, const int step /* 0: X_0 and its A (or everything) */) {
   extern __shared__ __align__(16) char lds[];
   __shared__ double sm[LOW_NT / 64];
   char *const area1 = lds, *const area2 = lds + LOW_AREA;
   int wg;
-  const Mat m = tab.m[find(tab, blockIdx.x, wg)];
-  const Scratch s(m.rows, m.cols, a.ws + m.ws);
+  const Table& tab = *reinterpret_cast<const Table*>(ws);
+  const StepArgs& a = tab.a;
+  const int steps = a.steps;
+  const Mat m = tab.m[find(tab.m, n, step ? L_LONG_LOW : L_LOW, blockIdx.x, wg)];
+  const Scratch s(m.rows, m.cols, ws + m.ws);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lr = lane & 31, h = lane >> 5, ib = wave >> 2, jb = (wave - ib) & 3;
   const int wgs = s.low_wgs(), Mb = s.Mb;
@@ -710,7 +731,7 @@ __global__ __launch_bounds__(LOW_NT) void ns_low_kernel(const Table tab, const S
   };
 
   if (step == 0) {
-    const double f = scale_of<LOW_NT>(m, s, a.eps, sm);
+    double f = 0.0;
     f32x16 gram;
     clear(gram);
     for (int st = wg; st < s.strips(); st += wgs) {
@@ -721,11 +742,13 @@ __global__ __launch_bounds__(LOW_NT) void ns_low_kernel(const Table tab, const S
           const int row = 32 * ib + 8 * (e >> 2) + 4 * h + (e & 3), col = 32 * (4 * st + jb) + lr;
           if (row < s.M && col < s.N) {
             const long r = s.turned ? col : row, c = s.turned ? row : col;
-            const float v = MUON ? reinterpret_cast<const float*>(s.t1)[r * m.cols + c] : (float)((const T*)a.g)[m.off + r * m.ld + c];
-            x[e] = (float)((double)v * f);
+            x[e] = MUON ? reinterpret_cast<const float*>(s.t1)[r * m.cols + c] : (float)((const T*)a.g)[m.off + r * m.ld + c];
           }
         }
       }
+      if (st == wg) f = scale_of<LOW_NT>(m, s, a.eps, sm);   // (behind the first loads)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) x[e] = (float)((double)x[e] * f);
       if (wgs == 1) break;
       __syncthreads();                          // (area1 may still be read for the strip before)
       if (rows) {
@@ -851,70 +874,96 @@ bool empty(const emx_matrix& m) { return m.rows == 0 || m.cols == 0; }
 
 // the matrices of one launch group: at most MAX_TABLE of them from index i on; returns the index behind them
 int group(const emx_matrix* mats, int n, int i, Table& t, size_t& bytes) {
-  t.n = 0, bytes = 0;
+  t.n = 0, bytes = TABLE_BYTES;
   for (; i < n && t.n < MAX_TABLE; ++i) {
     const emx_matrix& m = mats[i];
     if (empty(m)) continue;
-    t.m[t.n++] = Mat{m.offset, m.rows == 1 ? m.cols : m.ld, (long)bytes, m.rows, m.cols, m.scale, 0};
+    t.m[t.n++] = Mat{m.offset, m.rows == 1 ? m.cols : m.ld, (long)bytes, m.rows, m.cols, m.scale, {}};
     bytes += Scratch::bytes(m.rows, m.cols);
   }
   return i;
 }
 
+// Which tiles a product runs in.  64 x 64 with k shared out over the waves below 128 tiles of 128 x 128: such a launch is bound by the time from
+// one load to the next, not by its products (five steps: 1000 x 1000, 64 tiles, 196 us against 370; two 1024 x 1024, 128 tiles, 356 and
+// 376; four, 256 tiles, 501 and 442).  Else 256 x 128, two workgroups to a CU, where the last round of them is at least as full as with 128 x 128,
+// three to a CU (a tile of 256 x 128 reads a quarter less per product: 4096 x 4096 in 512 tiles 334 us a product against 371 in 1024;
+// six 1000 x 1500 in 288 tiles 82 us against 72 in 576; the upper half of 4096 x 4096 in 272 tiles 283 us against 256 in 528).
 template <typename F>
-long number(Table& t, F blocks) {   // hands out the workgroups of a launch
+int tile_size(F tiles, bool up) {
+  const auto fill = [](long n, long slots) { return (double)n / (double)((n + slots - 1) / slots * slots); };
+  const long n1 = tiles(1, up);
+  if (n1 < 128) return 0;
+  return fill(tiles(2, up), 512) >= fill(n1, 768) ? 2 : 1;
+}
+
+// hands out the workgroups (or tiles) of a launch
+template <typename F>
+long number(Table& t, int launch, F blocks) {
   long at = 0;
   for (int i = 0; i < t.n; ++i) {
-    t.m[i].begin = (int)at;
+    t.m[i].begin[launch] = (int)std::min(at, (long)INT_MAX);
     at += blocks(t.m[i], Scratch(t.m[i].rows, t.m[i].cols, nullptr));
   }
   return at;
 }
 
 template <typename T, bool MUON>
-int run(const char* who, const emx_matrix* mats, int n, const StepArgs& a, int steps, hipStream_t st) {
+int run(const char* who, const emx_matrix* mats, int n, const StepArgs& a, char* ws, hipStream_t st) {
   for (int i = 0; i < n;) {
-    Table t;
+    Table t{};
+    t.a = a;
     size_t bytes;
     i = group(mats, n, i, t, bytes);
     if (t.n == 0) break;
-    auto half = [](int b) { return (long)(b + 1) / 2; };
-    const auto parts = [](const Mat& m, const Scratch&) { return (long)parts_of((long)m.rows * m.cols); };
-    const auto full = [&](const Mat&, const Scratch& s) { return s.low() ? 0 : half(s.Mb) * half(s.Nb); };
-    const auto upper = [&](const Mat&, const Scratch& s) { return s.low() ? 0 : half(s.Mb) * (half(s.Mb) + 1) / 2; };
-    const auto low = [&](const Mat&, const Scratch& s) { return s.low() ? (long)s.low_wgs() : 0; };
-    const auto long_low = [&](const Mat&, const Scratch& s) { return s.low() && s.low_wgs() > 1 ? (long)s.low_wgs() : 0; };
-    int rc;
-    auto go = [&](auto kernel, long blocks, auto... more) {
+    // the long ones first: a launch ends with short tiles
+    const auto length = [](const Mat& m) { return std::max(m.rows, m.cols); };
+    std::stable_sort(t.m, t.m + t.n, [&](const Mat& x, const Mat& y) { return length(x) > length(y); });
+    const bool uneven = length(t.m[0]) != length(t.m[t.n - 1]);
+
+    const long norms = number(t, L_NORM, [](const Mat& m, const Scratch&) { return (long)parts_of((long)m.rows * m.cols); });
+    const long splits = number(t, L_SPLIT, [](const Mat&, const Scratch& s) { return s.low() ? 0 : (long)((s.Mb + 1) / 2) * ((s.Nb + 1) / 2); });
+    const long lows = number(t, L_LOW, [](const Mat&, const Scratch& s) { return s.low() ? (long)s.low_wgs() : 0; });
+    const long long_lows = number(t, L_LONG_LOW, [](const Mat&, const Scratch& s) { return s.low() && s.low_wgs() > 1 ? (long)s.low_wgs() : 0; });
+    // the tiles of the products, in blocks of 32: 2 x 2 (size 0), 4 x 4 (1), 8 x 4 (2)
+    const auto tiles = [&](int size, bool up) {
+      return number(t, up ? L_UPPER : L_FULL, [&](const Mat&, const Scratch& s) {
+        const int r = size == 0 ? 2 : 4 * size, c = size == 0 ? 2 : BT_C;
+        return s.low() ? 0 : tile_count((s.Mb + r - 1) / r, ((up ? s.Mb : s.Nb) + c - 1) / c, size == 2 ? 2 : 1, up);
+      });
+    };
+    const int size_up = tile_size(tiles, true), size_full = tile_size(tiles, false);
+    const long uppers = tiles(size_up, true), fulls = tiles(size_full, false);
+    for (const long blocks : {norms, splits, lows, uppers, fulls}) EMX_REQUIRE(blocks < (1l << 30), "%s: %ld workgroups", who, blocks);
+
+    hipLaunchKernelGGL((ns_norm_kernel<T, MUON>), dim3((unsigned)norms), dim3(NT), 0, st, ws, t);
+    int rc = check_launch(who);
+    if (rc) return rc;
+    if (splits) {
+      hipLaunchKernelGGL((ns_split_kernel<T, MUON>), dim3((unsigned)splits), dim3(NT), 0, st, ws, t.n);
+      if ((rc = check_launch(who))) return rc;
+    }
+    const auto low = [&](long blocks, int step) {
       if (blocks == 0) return (int)EMX_OK;
-      EMX_REQUIRE(blocks < (1l << 31), "%s: %ld workgroups", who, blocks);
-      hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(NT), 0, st, t, a, more...);
+      hipLaunchKernelGGL((ns_low_kernel<T, MUON>), dim3((unsigned)blocks), dim3(LOW_NT), 2 * LOW_AREA, st, ws, t.n, step);
       return check_launch(who);
     };
-    if ((rc = go(ns_norm_kernel<T, MUON>, number(t, parts)))) return rc;
-    if ((rc = go(ns_split_kernel<T, MUON>, number(t, full)))) return rc;
-    auto go_low = [&](long blocks, int step) {
-      if (blocks == 0) return (int)EMX_OK;
-      hipLaunchKernelGGL((ns_low_kernel<T, MUON>), dim3((unsigned)blocks), dim3(LOW_NT), 2 * LOW_AREA, st, t, a, step, steps);
+    const auto product = [&](auto mid, auto big1, auto big2, bool up, int k) {
+      const int size = up ? size_up : size_full;
+      const long count = up ? uppers : fulls;
+      if (count == 0) return (int)EMX_OK;
+      // consecutive tiles to an XCD: an eighth of them all, or -- where their lengths differ -- a few in turn, so that each gets long ones
+      const long r = uneven ? 8 : (count + 7) / 8, blocks = (count + 8 * r - 1) / (8 * r) * 8 * r;
+      hipLaunchKernelGGL((size == 0 ? mid : size == 1 ? big1 : big2), dim3((unsigned)blocks), dim3(NT), 0, st, ws, t.n, k & 1, (int)count, (int)r);
       return check_launch(who);
     };
-    if ((rc = go_low(number(t, low), 0))) return rc;
-    const auto big_upper = [&](const Mat&, const Scratch& s) { return s.low() ? 0 : tile_count((s.Mb + BT_R - 1) / BT_R, (s.Mb + BT_C - 1) / BT_C, true); };
-    const auto big_full = [&](const Mat&, const Scratch& s) { return s.low() ? 0 : tile_count((s.Mb + BT_R - 1) / BT_R, (s.Nb + BT_C - 1) / BT_C, false); };
-    const bool big = number(t, big_full) >= BIG_TILES;
-    auto product = [&](auto small_kernel, auto big_kernel, bool up, int k) {
-      if (big) {
-        const long tiles = up ? number(t, big_upper) : number(t, big_full);
-        return go(big_kernel, 8 * ((tiles + 7) / 8), k & 1, (int)tiles);
-      }
-      return go(small_kernel, up ? number(t, upper) : number(t, full), k & 1);
-    };
-    for (int k = 0; k < steps; ++k) {
-      if ((rc = product(ns_product_kernel<GRAM, T, MUON>, ns_big_kernel<GRAM, T, MUON>, true, k))) return rc;
-      if ((rc = product(ns_product_kernel<POLY, T, MUON>, ns_big_kernel<POLY, T, MUON>, true, k))) return rc;
-      if (k + 1 < steps) rc = product(ns_product_kernel<NEXT, T, MUON>, ns_big_kernel<NEXT, T, MUON>, false, k);
-      else rc = product(ns_product_kernel<LAST, T, MUON>, ns_big_kernel<LAST, T, MUON>, false, k);
-      if (rc || (rc = go_low(number(t, long_low), k + 1))) return rc;
+    if ((rc = low(lows, 0))) return rc;
+    for (int k = 0; k < a.steps; ++k) {
+      if ((rc = product(ns_mid_kernel<GRAM, T, MUON>, ns_big_kernel<GRAM, T, MUON, 1>, ns_big_kernel<GRAM, T, MUON, 2>, true, k))) return rc;
+      if ((rc = product(ns_mid_kernel<POLY, T, MUON>, ns_big_kernel<POLY, T, MUON, 1>, ns_big_kernel<POLY, T, MUON, 2>, true, k))) return rc;
+      if (k + 1 < a.steps) rc = product(ns_mid_kernel<NEXT, T, MUON>, ns_big_kernel<NEXT, T, MUON, 1>, ns_big_kernel<NEXT, T, MUON, 2>, false, k);
+      else rc = product(ns_mid_kernel<LAST, T, MUON>, ns_big_kernel<LAST, T, MUON, 1>, ns_big_kernel<LAST, T, MUON, 2>, false, k);
+      if (rc || (rc = low(long_lows, k + 1))) return rc;
     }
   }
   return EMX_OK;
@@ -950,11 +999,11 @@ int emx_orthogonalize(const emx_matrix* mats, int n_mats, const void* g, void* o
     return fail(EMX_EWORKSPACE, "%s: workspace of %zu bytes at %p, %zu needed on a 16-byte boundary", who, ws_bytes, ws,
                 emx_orthogonalize_ws_bytes(mats, n_mats));
   StepArgs a{};
-  a.g = g, a.out = out, a.ws = (char*)ws, a.n_slices = 1, a.eps = eps;
+  a.g = g, a.out = out, a.n_slices = 1, a.steps = steps, a.eps = eps;
   hipStream_t st = (hipStream_t)stream;
-  if (dtype == EMX_F16) return run<_Float16, false>(who, mats, n_mats, a, steps, st);
-  if (dtype == EMX_BF16) return run<__bf16, false>(who, mats, n_mats, a, steps, st);
-  return run<float, false>(who, mats, n_mats, a, steps, st);
+  if (dtype == EMX_F16) return run<_Float16, false>(who, mats, n_mats, a, (char*)ws, st);
+  if (dtype == EMX_BF16) return run<__bf16, false>(who, mats, n_mats, a, (char*)ws, st);
+  return run<float, false>(who, mats, n_mats, a, (char*)ws, st);
 }
 
 int emx_muon_step(const emx_matrix* mats, int n_mats, float* w, const float* g, int n_slices, int64_t slice_stride, float* momentum, float lr,
@@ -975,9 +1024,9 @@ int emx_muon_step(const emx_matrix* mats, int n_mats, float* w, const float* g, 
     return fail(EMX_EWORKSPACE, "%s: workspace of %zu bytes at %p, %zu needed on a 16-byte boundary", who, ws_bytes, ws,
                 emx_orthogonalize_ws_bytes(mats, n_mats));
   StepArgs a{};
-  a.g = g, a.w = w, a.mom = momentum, a.ws = (char*)ws, a.slice_stride = slice_stride, a.n_slices = n_slices, a.nesterov = nesterov != 0;
+  a.g = g, a.w = w, a.mom = momentum, a.slice_stride = slice_stride, a.n_slices = n_slices, a.nesterov = nesterov != 0, a.steps = steps;
   a.beta = beta, a.keep = (float)(1.0 - (double)lr * weight_decay), a.lr = lr, a.eps = eps;
-  return run<float, true>(who, mats, n_mats, a, steps, (hipStream_t)stream);
+  return run<float, true>(who, mats, n_mats, a, (char*)ws, (hipStream_t)stream);
 }
 
 }  // extern "C"
