@@ -2,16 +2,17 @@
 // polynomial iteration -- matrix products only -- and the optimizer step that uses them.
 //
 //   X_0 = G / (|G|_F + eps)    (G transposed where it has more rows than columns, so that X is M x N with M <= N)
-//   A = X X^T,  P = a I + b A + c A^2,  X <- P X       `steps` times; (a, b, c) = (3.4445, -4.7750, 2.0315)
+//   A = X X^T,  P = b A + c A^2,  X <- a X + P X       `steps` times; (a, b, c) = (3.4445, -4.7750, 2.0315)
 //
 // A singular value s of X goes to s (a + b s^2 + c s^4): that polynomial maps [0, 1] into [0, 1.2024] and [0, 1.2024] into itself, and
 // multiplies the small ones by up to 3.4, so after five steps those above ~1e-2 lie around one.  Hence the bounds every stored value
-// obeys, whatever G is: |X| <= 1.21, |A| <= 1.45, |P| <= 3.45.
+// obeys, whatever G is: |X| <= 1.21, |A| <= 1.45, |P| <= 2.81.
 //
 // Arithmetic: as the dense layers', every float32 product is THREE f16 matrix instructions on operands split into two f16 planes (hi = f16(v),
-// lo = f16(v - hi): 22 bits), accumulated in float32.  The bounds above make ONE fixed scale of 2^14 enough for X, A and P (|P| 2^14 <= 56.5e3
+// lo = f16(v - hi): 22 bits), accumulated in float32.  The bounds above make ONE fixed scale of 2^14 enough for X, A and P (|P| 2^14 <= 46.1e3
 // < 65504; what is lost below is 2^-24 2^-14 of the matrix' norm).  The norm is summed in 64 bits: an error of its scale is the one that
-// the iteration turns into an error of every singular value.
+// the iteration turns into an error of every singular value.  a X joins P X behind its sum, not as a diagonal of P: the sum then rounds at the
+// size of P X alone (4096 x 4096: 4.4e-6 off with it inside).
 //
 // Layout of an operand (X, X^T, A, P): blocks of 32 rows x 32 k; a block is two K-steps of 16, each a hi and a lo PIECE of 1 KB -- what one
 // v_mfma_f32_32x32x16_f16 reads: lane l holds row l % 32, k = 8 (l / 32) .. + 7.  The accumulators of such an instruction -- lane l: column
@@ -42,7 +43,7 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef unsigned uint4v __attribute__((ext_vector_type(4)));
 
 // the launches whose workgroups are numbered through the matrices
-enum { L_NORM = 0, L_SPLIT, L_LOW, L_LONG_LOW, L_UPPER, L_FULL, L_COUNT };
+enum { L_NORM = 0, L_SPLIT, L_LOW, L_UPPER, L_FULL, L_COUNT };
 
 struct Mat {
   long off, ld;        // first element and row stride in the flat tensors
@@ -57,6 +58,7 @@ struct StepArgs {
   float *w, *mom;      // optimizer step
   long slice_stride;
   int n_slices, nesterov, steps;
+  int low_steps;       // matrices of at most 128 rows: a launch per step, for all of them as one of them is longer than 128 columns
   float beta, keep, lr, eps;    // keep = 1 - lr weight_decay
 };
 // Everything a call is about.  The first launch gets it as an argument and leaves a copy at the workspace's begin, from which the others read it:
@@ -401,10 +403,23 @@ __device__ __forceinline__ void put_turned(char* block, const Planes& x, const h
   }
 }
 
+// x += f (hi + lo) for the transpose of an operand's block: where put_direct puts it
+__device__ __forceinline__ void add_planes(f32x16& x, const char* block, float f, int lr, int h) {
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const char* const at = block + (q >> 1) * 2048 + ((q & 1) * 32 + lr) * 16 + h * 8;
+    const half4 hi = *reinterpret_cast<const half4*>(at), lo = *reinterpret_cast<const half4*>(at + 1024);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) x[4 * q + r] = fmaf(f, (float)hi[r] + (float)lo[r], x[4 * q + r]);
+  }
+}
+
 // A block of a product where it belongs (x: element 4 q + r = row 32 ib + 8 q + 4 h + r of column 32 jb + lr, scaled by 2^28)
 template <int KIND, typename T, bool MUON>
-__device__ __forceinline__ void store_block(const Mat& m, const StepArgs& a, const Scratch& s, f32x16 x, int ib, int jb, char* t_out, int lr, int h) {
+__device__ __forceinline__ void store_block(const Mat& m, const StepArgs& a, const Scratch& s, f32x16 x, int ib, int jb, const char* t_in, char* t_out, int lr,
+                                            int h) {
   if (ib >= s.Mb || jb >= (KIND <= POLY ? s.Mb : s.Nb) || (KIND <= POLY && ib > jb)) return;   // (A and P: the upper half, stored twice)
+  if constexpr (KIND >= NEXT) add_planes(x, t_in + ((long)jb * s.Mb + ib) * BLK, CA * SC, lr, h);
   if constexpr (KIND == LAST) {
     write_block<T, MUON>(m, a, s, x, ib, jb, lr, h);
   } else {
@@ -414,17 +429,9 @@ __device__ __forceinline__ void store_block(const Mat& m, const StepArgs& a, con
 #pragma unroll
     for (int e = 0; e < 16; ++e) x[e] *= RSC;
     if constexpr (KIND == POLY) {
-      const char* const am = s.a + ((long)jb * s.Mb + ib) * BLK + lr * 16 + h * 8;    // A is symmetric: the same four of its transpose
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int to = (q >> 1) * 2048 + (q & 1) * 512;
-        const half4 ah = *reinterpret_cast<const half4*>(am + to), al = *reinterpret_cast<const half4*>(am + to + 1024);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          x[4 * q + r] = fmaf(CC, x[4 * q + r], CB * ((float)ah[r] + (float)al[r]));
-          if (ib == jb && 8 * q + 4 * h + r == lr && 32 * ib + lr < s.M) x[4 * q + r] += CA * SC;
-        }
-      }
+      for (int e = 0; e < 16; ++e) x[e] *= CC;
+      add_planes(x, s.a + ((long)jb * s.Mb + ib) * BLK, CB, lr, h);    // A is symmetric: its transpose
     }
     const Planes y(x);
     put_direct(O + ((long)jb * s.Mb + ib) * BLK, y, lr, h);
@@ -434,7 +441,7 @@ __device__ __forceinline__ void store_block(const Mat& m, const StepArgs& a, con
 }
 
 template <int KIND, typename T, bool MUON, int RB>
-__global__ __launch_bounds__(NT, RB == 2 ? 2 : 3) void ns_big_kernel(char* ws, const int n, const int odd, const int total, const int run) {
+__global__ __launch_bounds__(NT, 2) void ns_big_kernel(char* ws, const int n, const int odd, const int total, const int run) {
   __shared__ __align__(16) char lds[2][BT_C * BLK];
   // runs of consecutive tiles to each XCD: they share operands in its L2
   const int turn = (int)(blockIdx.x >> 3), at = ((turn / run) * 8 + (int)(blockIdx.x & 7)) * run + turn % run;
@@ -509,6 +516,12 @@ __global__ __launch_bounds__(NT, RB == 2 ? 2 : 3) void ns_big_kernel(char* ws, c
   asm volatile("" ::: "memory");
   request_u(1, 0);
   asm volatile("" ::: "memory");
+  f32x16 sum[BT_C];
+  if constexpr (RB == 1)
+#pragma unroll
+    for (int j = 0; j < BT_C; ++j)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) sum[j][e] = 0.f;
   for (int k = 0; k < Kb; ++k) {
     const int buf = k & 1;
     __syncthreads();                            // the buffer is written, and the other one read to its end
@@ -532,11 +545,28 @@ __global__ __launch_bounds__(NT, RB == 2 ? 2 : 3) void ns_big_kernel(char* ws, c
     multiply(3);
     __builtin_amdgcn_sched_barrier(0);
     request_u(1, min(k + 1, Kb - 1));
+    if constexpr (RB == 1) {                    // sums in two levels, 256 k to the first (with RB = 2 there are no registers for it)
+      if ((k & 7) == 7) {
+#pragma unroll
+        for (int j = 0; j < BT_C; ++j)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            sum[j][e] += acc[0][j][e];
+            acc[0][j][e] = 0.f;
+          }
+      }
+    }
+  }
+  if constexpr (RB == 1) {
+#pragma unroll
+    for (int j = 0; j < BT_C; ++j)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[0][j][e] += sum[j][e];
   }
 #pragma unroll
   for (int i = 0; i < RB; ++i)
 #pragma unroll
-    for (int j = 0; j < BT_C; ++j) store_block<KIND, T, MUON>(m, a, s, acc[i][j], ib0 + i, jb0 + j, t_out, lr, h);
+    for (int j = 0; j < BT_C; ++j) store_block<KIND, T, MUON>(m, a, s, acc[i][j], ib0 + i, jb0 + j, t_in, t_out, lr, h);
 }
 
 // ---- the products in tiles of 64 x 64, for matrices that would leave most of the machine idle in larger ones: the four waves of a
@@ -634,13 +664,13 @@ __global__ __launch_bounds__(NT, 2) void ns_mid_kernel(char* ws, const int n, co
     x[4 * q + 2] = (s0.z + s1.z) + (s2.z + s3.z);
     x[4 * q + 3] = (s0.w + s1.w) + (s2.w + s3.w);
   }
-  store_block<KIND, T, MUON>(m, a, s, x, ib0 + (wave >> 1), jb0 + (wave & 1), t_out, lr, h);
+  store_block<KIND, T, MUON>(m, a, s, x, ib0 + (wave >> 1), jb0 + (wave & 1), t_in, t_out, lr, h);
 }
 
 // ---- matrices of at most 128 rows: a workgroup of sixteen waves holds 128 columns of X in registers, a wave one block.  The operands of the
-// three products pass through two areas of LDS of 4 x 4 blocks: X, then X^T in the first, A, then P in the second.  A matrix of at most
-// 128 columns goes through all its steps in one launch.  A longer one is cut into strips of 128 columns: a launch per step, in which EVERY
-// workgroup adds up the shares of A that the launch before left (in their order), forms P, takes its strip on and leaves its share of
+// three products pass through two areas of LDS of 4 x 4 blocks: X, then X^T in the first, A, then P in the second.  Matrices of at
+// most 128 columns go through all their steps in one launch.  Longer ones are cut into strips of 128 columns: a launch per step (then for the
+// short ones too: their 40 us would stand in front of the others' steps), in which EVERY workgroup adds up the shares of A that the launch before left (in their order), forms P, takes its strip on and leaves its share of
 // the next A -- one product of 128^3 and the sum more per workgroup than a division of that work would need, but 2 launches a step fewer.
 // A and P are symmetric: the ten waves on and above the diagonal form them, dealt to the SIMDs by (row + column) % 4, three at most to each.
 // What bounds it is the LDS (512 KB a product at 128 bytes a clock; 72 matrix instructions a wave and step are 3.8 us) and what stands
@@ -690,7 +720,7 @@ __global__ __launch_bounds__(LOW_NT) void ns_low_kernel(char* ws, const int n, c
   const Table& tab = *reinterpret_cast<const Table*>(ws);
   const StepArgs& a = tab.a;
   const int steps = a.steps;
-  const Mat m = tab.m[find(tab.m, n, step ? L_LONG_LOW : L_LOW, blockIdx.x, wg)];
+  const Mat m = tab.m[find(tab.m, n, L_LOW, blockIdx.x, wg)];
   const Scratch s(m.rows, m.cols, ws + m.ws);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lr = lane & 31, h = lane >> 5, ib = wave >> 2, jb = (wave - ib) & 3;
@@ -715,8 +745,7 @@ __global__ __launch_bounds__(LOW_NT) void ns_low_kernel(char* ws, const int n, c
     if (square) {
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
-        const int row = 32 * ib + 8 * (e >> 2) + 4 * h + (e & 3);
-        av[e] = fmaf(CC * RSC, sq[e], CB * av[e]) + (row == 32 * jb + lr && row < s.M ? CA * SC : 0.f);
+        av[e] = fmaf(CC * RSC, sq[e], CB * av[e]);
       }
       keep_symmetric(area2, av);
     }
@@ -749,7 +778,7 @@ __global__ __launch_bounds__(LOW_NT) void ns_low_kernel(char* ws, const int n, c
       if (st == wg) f = scale_of<LOW_NT>(m, s, a.eps, sm);   // (behind the first loads)
 #pragma unroll
       for (int e = 0; e < 16; ++e) x[e] = (float)((double)x[e] * f);
-      if (wgs == 1) break;
+      if (!a.low_steps) break;                  // (one strip)
       __syncthreads();                          // (area1 may still be read for the strip before)
       if (rows) {
         const Planes y(x);
@@ -759,7 +788,7 @@ __global__ __launch_bounds__(LOW_NT) void ns_low_kernel(char* ws, const int n, c
       __syncthreads();
       if (square) low_product(gram, u1, v1, min(4, s.Nb - 4 * st));
     }
-    if (wgs > 1) {
+    if (a.low_steps) {
       if (square) leave_share(s.a, gram);
       return;
     }
@@ -777,7 +806,10 @@ __global__ __launch_bounds__(LOW_NT) void ns_low_kernel(char* ws, const int n, c
       if (rows) put_direct(area1 + (jb * 4 + ib) * BLK, y, lr, h);
       form_poly();
       clear(x);
-      if (rows && jb < s.Nb) low_product(x, u2, v1, Mb);
+      if (rows && jb < s.Nb) {
+        low_product(x, u2, v1, Mb);
+        add_planes(x, area1 + (jb * 4 + ib) * BLK, CA * SC, lr, h);
+      }
       if (k + 1 < steps) {
         times(x, RSC);
         __syncthreads();
@@ -825,7 +857,10 @@ __global__ __launch_bounds__(LOW_NT) void ns_low_kernel(char* ws, const int n, c
       __syncthreads();
     }
     clear(x);
-    if (rows) low_product(x, u2, v1, Mb);
+    if (rows) {
+      low_product(x, u2, v1, Mb);
+      add_planes(x, area1 + (jb * 4 + ib) * BLK, CA * SC, lr, h);
+    }
     if (step == steps) {
       if (rows && 4 * st + jb < s.Nb) write_block<T, MUON>(m, a, s, x, ib, 4 * st + jb, lr, h);
       continue;
@@ -886,15 +921,14 @@ int group(const emx_matrix* mats, int n, int i, Table& t, size_t& bytes) {
 
 // Which tiles a product runs in.  64 x 64 with k shared out over the waves below 128 tiles of 128 x 128: such a launch is bound by the time from
 // one load to the next, not by its products (five steps: 1000 x 1000, 64 tiles, 196 us against 370; two 1024 x 1024, 128 tiles, 356 and
-// 376; four, 256 tiles, 501 and 442).  Else 256 x 128, two workgroups to a CU, where the last round of them is at least as full as with 128 x 128,
-// three to a CU (a tile of 256 x 128 reads a quarter less per product: 4096 x 4096 in 512 tiles 334 us a product against 371 in 1024;
-// six 1000 x 1500 in 288 tiles 82 us against 72 in 576; the upper half of 4096 x 4096 in 272 tiles 283 us against 256 in 528).
+// 376; four, 256 tiles, 501 and 442).  Else 128 x 128, and 256 x 128 -- which reads a quarter less per product -- where these leave at most a
+// fifth of the places of their last round empty (two to a CU; 4096 x 4096 in 512 tiles 334 us a product against 371 in 1024; six
+// 1000 x 1500 in 288 tiles 82 us against 72 in 576; the upper half of 4096 x 4096 in 272 tiles 283 us against 256 in 528).
 template <typename F>
 int tile_size(F tiles, bool up) {
-  const auto fill = [](long n, long slots) { return (double)n / (double)((n + slots - 1) / slots * slots); };
-  const long n1 = tiles(1, up);
-  if (n1 < 128) return 0;
-  return fill(tiles(2, up), 512) >= fill(n1, 768) ? 2 : 1;
+  if (tiles(1, up) < 128) return 0;
+  const long n = tiles(2, up), rounds = (n + 511) / 512;
+  return 5 * n >= 4 * 512 * rounds ? 2 : 1;
 }
 
 // hands out the workgroups (or tiles) of a launch
@@ -924,7 +958,7 @@ int run(const char* who, const emx_matrix* mats, int n, const StepArgs& a, char*
     const long norms = number(t, L_NORM, [](const Mat& m, const Scratch&) { return (long)parts_of((long)m.rows * m.cols); });
     const long splits = number(t, L_SPLIT, [](const Mat&, const Scratch& s) { return s.low() ? 0 : (long)((s.Mb + 1) / 2) * ((s.Nb + 1) / 2); });
     const long lows = number(t, L_LOW, [](const Mat&, const Scratch& s) { return s.low() ? (long)s.low_wgs() : 0; });
-    const long long_lows = number(t, L_LONG_LOW, [](const Mat&, const Scratch& s) { return s.low() && s.low_wgs() > 1 ? (long)s.low_wgs() : 0; });
+    t.a.low_steps = std::any_of(t.m, t.m + t.n, [](const Mat& m) { const Scratch s(m.rows, m.cols, nullptr); return s.low() && s.strips() > 1; });
     // the tiles of the products, in blocks of 32: 2 x 2 (size 0), 4 x 4 (1), 8 x 4 (2)
     const auto tiles = [&](int size, bool up) {
       return number(t, up ? L_UPPER : L_FULL, [&](const Mat&, const Scratch& s) {
@@ -963,7 +997,7 @@ int run(const char* who, const emx_matrix* mats, int n, const StepArgs& a, char*
       if ((rc = product(ns_mid_kernel<POLY, T, MUON>, ns_big_kernel<POLY, T, MUON, 1>, ns_big_kernel<POLY, T, MUON, 2>, true, k))) return rc;
       if (k + 1 < a.steps) rc = product(ns_mid_kernel<NEXT, T, MUON>, ns_big_kernel<NEXT, T, MUON, 1>, ns_big_kernel<NEXT, T, MUON, 2>, false, k);
       else rc = product(ns_mid_kernel<LAST, T, MUON>, ns_big_kernel<LAST, T, MUON, 1>, ns_big_kernel<LAST, T, MUON, 2>, false, k);
-      if (rc || (rc = low(long_lows, k + 1))) return rc;
+      if (rc || (t.a.low_steps && (rc = low(lows, k + 1)))) return rc;
     }
   }
   return EMX_OK;
