@@ -830,14 +830,15 @@ def _element_type(t, what) -> int:
 
 def _like(t, ref, what) -> None:
     """``t`` on the device of ``ref``, and a device of the GPU's"""
-    if not t.is_cuda or t.device != ref.device:
+    dev = t.get_device()
+    if dev < 0 or dev != ref.get_device():
         raise EmxError(f"{what}: a tensor on {ref.device} expected (a GPU), got {t.device}")
 
 
 def _rows(t, ref, what) -> int:
     """the row stride of a [rows, D] tensor like ``ref`` (its device, type and shape) whose columns lie side by side"""
     _like(t, ref, what)
-    if t.dtype != ref.dtype or t.shape != ref.shape or t.dim() != 2:
+    if t.dtype is not ref.dtype or t.shape != ref.shape or t.dim() != 2:
         raise EmxError(f"{what}: {ref.dtype} [rows, D] like the input's {tuple(ref.shape)} expected, got {t.dtype} {tuple(t.shape)}")
     stride, col = t.stride()
     if col != 1 and t.shape[1] > 1:
@@ -850,17 +851,23 @@ def _vector(t, n, ref, what):
     if t is None:
         return None
     _like(t, ref, what)
-    if t.dtype != torch.float32 or t.numel() != n or not t.is_contiguous():
+    if t.dtype is not torch.float32 or t.numel() != n or not t.is_contiguous():
         raise EmxError(f"{what}: {n} contiguous float32 values expected, got {t.dtype} {tuple(t.shape)}, strides {t.stride()}")
     return t.data_ptr()
 
 
-def _on_device(device, fn, what, *args) -> None:
-    """``fn(*args, stream)`` on torch's current stream of ``device``, whichever device is current"""
-    if device.index != torch.cuda.current_device():
-        with torch.cuda.device(device):
-            return _check(fn(*args, _stream()), what)
-    _check(fn(*args, _stream()), what)
+# torch's current stream as a handle without a Stream object around it: 0.1 us of a call that takes five
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def _on_device(index, fn, what, *args) -> None:
+    """``fn(*args, stream)`` on torch's current stream of device ``index``, whichever device is current"""
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
+            return _check(fn(*args, _raw_stream(index)), what)
+    rc = fn(*args, _raw_stream(index))
+    if rc:
+        _check(rc, what)
 
 
 def layernorm_fwd(x, gamma, beta, eps, y, mean=None, rstd=None):
@@ -869,8 +876,8 @@ def layernorm_fwd(x, gamma, beta, eps, y, mean=None, rstd=None):
     code = _element_type(x, "x")
     ldx, ldy = _rows(x, x, "x"), _rows(y, x, "y")
     n, D = x.shape
-    _on_device(x.device, load().emx_layernorm_fwd, "emx_layernorm_fwd", x.data_ptr(), code, n, D, ldx, _vector(gamma, D, x, "gamma"),
-               _vector(beta, D, x, "beta"), float(eps), y.data_ptr(), ldy, _vector(mean, n, x, "mean"), _vector(rstd, n, x, "rstd"))
+    _on_device(x.get_device(), load().emx_layernorm_fwd, "emx_layernorm_fwd", x.data_ptr(), code, n, D, ldx, _vector(gamma, D, x, "gamma"),
+               _vector(beta, D, x, "beta"), eps, y.data_ptr(), ldy, _vector(mean, n, x, "mean"), _vector(rstd, n, x, "rstd"))
 
 
 def layernorm_ws_floats(n_rows, D) -> int:
@@ -886,7 +893,7 @@ def layernorm_bwd(dy, x, gamma, mean, rstd, dx, dgamma, dbeta, ws=None):
     n, D = x.shape
     if ws is not None:
         _vector(ws, ws.numel(), x, "ws")
-    _on_device(x.device, load().emx_layernorm_bwd, "emx_layernorm_bwd", dy.data_ptr(), ld_dy, x.data_ptr(), ldx, code, n, D,
+    _on_device(x.get_device(), load().emx_layernorm_bwd, "emx_layernorm_bwd", dy.data_ptr(), ld_dy, x.data_ptr(), ldx, code, n, D,
                _vector(gamma, D, x, "gamma"), _vector(mean, n, x, "mean"), _vector(rstd, n, x, "rstd"),
                None if dx is None else dx.data_ptr(), ld_dx, _vector(dgamma, D, x, "dgamma"), _vector(dbeta, D, x, "dbeta"),
                None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel())
@@ -941,7 +948,7 @@ def orthogonalize(plan: MatrixPlan, g, out, steps: int = 5, eps: float = 1e-7):
     code = _element_type(g, "g")
     if out.dtype != g.dtype:
         raise EmxError(f"out: {g.dtype} like g expected, got {out.dtype}")
-    _on_device(plan.ws.device, load().emx_orthogonalize, "emx_orthogonalize", *plan._args, plan._flat(g, "g"), plan._flat(out, "out"), code, int(steps),
+    _on_device(plan.ws.get_device(), load().emx_orthogonalize, "emx_orthogonalize", *plan._args, plan._flat(g, "g"), plan._flat(out, "out"), code, int(steps),
                float(eps), *plan._ws_args)
 
 
@@ -955,7 +962,7 @@ def muon_step(plan: MatrixPlan, w, g, momentum_buffer, lr, momentum: float = 0.9
     slices, stride = g.shape if g.dim() == 2 else (1, 0)
     if slices > 1 and stride < plan.end:
         raise EmxError(f"g: slices of {stride} elements, the matrices reach to {plan.end}")
-    _on_device(plan.ws.device, load().emx_muon_step, "emx_muon_step", *plan._args, plan._flat(w, "w"), plan._flat(g, "g", slices, stride), slices, stride,
+    _on_device(plan.ws.get_device(), load().emx_muon_step, "emx_muon_step", *plan._args, plan._flat(w, "w"), plan._flat(g, "g", slices, stride), slices, stride,
                plan._flat(momentum_buffer, "momentum_buffer"), float(lr), float(momentum), int(bool(nesterov)), float(weight_decay), int(steps), float(eps),
                *plan._ws_args)
 
