@@ -1279,7 +1279,11 @@ __global__ __launch_bounds__(NTC) __attribute__((amdgpu_waves_per_eu(4, 4))) voi
                                                                                                            p_with_cost, a);
 }
 
-// The operand store from the flat parameter buffer (the optimizer keeps it current afterwards).  Two launches: the layers'
+__global__ __launch_bounds__(256) void mlp_clear_kernel(float* __restrict__ p, long n) {
+  for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long)gridDim.x * 256) p[i] = 0.f;
+}
+
+// The operand store from the flat parameter buffer (the optimizer keeps it current afterwards).  Cleared, then two launches: the layers'
 // exact maxima -> headers (scale, both slots seeded, wop.h), then one wave per 32 x 32 block writes the pieces.
 __global__ __launch_bounds__(256) void mlp_mirror_max_kernel(const WopArgs wa, const float* __restrict__ params, char* __restrict__ store) {
   __shared__ unsigned red[4];
@@ -2151,7 +2155,12 @@ int emx_mlp_mirror(const emx_mlp_desc* desc, const float* params, float* mirror,
   WopArgs wa;
   fill_wop_args(desc, wa);
   // the zero padding of the layers (to whole 128 x 128 units) is written here, once; the optimizer rewrites real blocks only
-  if (hipMemsetAsync(mirror, 0, (size_t)wop_total_bytes(wa), (hipStream_t)stream) != hipSuccess) return emx::check_launch("emx_mlp_mirror (memset)");
+  // (by a kernel: a step that is captured after the weights were written by anything but emx_adam_step* has this call in its graph, and a
+  //  memset node there has given wrong results on replays after the first)
+  const long words = (long)wop_total_bytes(wa) / 4;
+  hipLaunchKernelGGL(mlp_clear_kernel, dim3((unsigned)std::min((words + 4 * 256 - 1) / (4 * 256), 2048l)), dim3(256), 0, (hipStream_t)stream, mirror, words);
+  rc = emx::check_launch("mlp_clear_kernel");
+  if (rc) return rc;
   hipLaunchKernelGGL(mlp_mirror_max_kernel, dim3((unsigned)desc->n_layers), dim3(256), 0, (hipStream_t)stream, wa, params,
                      reinterpret_cast<char*>(mirror));
   rc = emx::check_launch("mlp_mirror_max_kernel");
