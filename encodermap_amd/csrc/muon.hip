@@ -43,7 +43,7 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef unsigned uint4v __attribute__((ext_vector_type(4)));
 
 // the launches whose workgroups are numbered through the matrices
-enum { L_NORM = 0, L_SPLIT, L_LOW, L_UPPER, L_FULL, L_COUNT };
+enum { L_NORM = 0, L_SPLIT, L_LOW, L_GRAM, L_JOIN, L_POLY, L_FULL, L_COUNT };
 
 struct Mat {
   long off, ld;        // first element and row stride in the flat tensors
@@ -78,7 +78,7 @@ constexpr int LOW_WGS = 32;                   // ... 128 columns each, or more w
 struct Scratch {
   int M, N, Mb, Nb;
   bool turned;
-  char *t0, *t1, *x, *a, *p;
+  char *t0, *t1, *x, *a, *p, *parts;
   double* part;
   __host__ __device__ Scratch(int rows, int cols, char* base) {
     turned = rows > cols;
@@ -90,14 +90,22 @@ struct Scratch {
     x = t1 + xn;
     a = low() ? x : x + xn;
     p = a + an;
+    parts = p + an;
   }
   __host__ __device__ bool low() const { return Mb <= LOW; }
   __host__ __device__ int strips() const { return (Nb + 3) / 4; }     // of 128 columns
   __host__ __device__ int low_wgs() const { return strips() < LOW_WGS ? strips() : LOW_WGS; }
+  // A of a matrix four times as long as high and more (and 4096 at least): its sums are cut into four to eight parts, of about the length of the
+  // other products.  (Two parts cost more in ns_join_kernel, 9 us, than they save: four 2048 x 512 308 us against 271.)
+  __host__ __device__ int gram_parts() const {
+    const int n = Nb / (Mb > 32 ? Mb : 32);
+    return n < 4 ? 1 : n < 8 ? n : 8;
+  }
   __host__ static size_t bytes(int rows, int cols) {
     const Scratch s(rows, cols, nullptr);
     const size_t xn = (size_t)s.Mb * s.Nb;
-    return MAX_PARTS * 8 + (s.low() ? 2 * xn + 2 * (size_t)s.low_wgs() * 16 : 3 * xn + 2 * (size_t)s.Mb * s.Mb) * BLK;
+    const size_t an = (size_t)s.Mb * s.Mb;
+    return MAX_PARTS * 8 + (s.low() ? 2 * xn + 2 * (size_t)s.low_wgs() * 16 : 3 * xn + (2 + (s.gram_parts() > 1 ? s.gram_parts() : 0)) * an) * BLK;
   }
 };
 // (1024 elements and more to a share: the optimizer step reads up to 32 gradient parts of each)
@@ -414,11 +422,22 @@ __device__ __forceinline__ void add_planes(f32x16& x, const char* block, float f
   }
 }
 
+__device__ __forceinline__ float4* part_of(const Scratch& s, int part, int ib, int jb, int q, int lane) {
+  return reinterpret_cast<float4*>(s.parts + (((long)part * s.Mb + ib) * s.Mb + jb) * BLK + q * 1024 + lane * 16);
+}
+
 // A block of a product where it belongs (x: element 4 q + r = row 32 ib + 8 q + 4 h + r of column 32 jb + lr, scaled by 2^28)
 template <int KIND, typename T, bool MUON>
-__device__ __forceinline__ void store_block(const Mat& m, const StepArgs& a, const Scratch& s, f32x16 x, int ib, int jb, const char* t_in, char* t_out, int lr,
-                                            int h) {
+__device__ __forceinline__ void store_block(const Mat& m, const StepArgs& a, const Scratch& s, f32x16 x, int ib, int jb, int part /* of the sum; -1: all of it */,
+                                            const char* t_in, char* t_out, int lr, int h) {
   if (ib >= s.Mb || jb >= (KIND <= POLY ? s.Mb : s.Nb) || (KIND <= POLY && ib > jb)) return;   // (A and P: the upper half, stored twice)
+  if constexpr (KIND == GRAM) {
+    if (part >= 0) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) *part_of(s, part, ib, jb, q, 32 * h + lr) = make_float4(x[4 * q], x[4 * q + 1], x[4 * q + 2], x[4 * q + 3]);
+      return;
+    }
+  }
   if constexpr (KIND >= NEXT) add_planes(x, t_in + ((long)jb * s.Mb + ib) * BLK, CA * SC, lr, h);
   if constexpr (KIND == LAST) {
     write_block<T, MUON>(m, a, s, x, ib, jb, lr, h);
@@ -449,12 +468,15 @@ __global__ __launch_bounds__(NT, 2) void ns_big_kernel(char* ws, const int n, co
   int inside;
   const Table& tab = *reinterpret_cast<const Table*>(ws);
   const StepArgs& a = tab.a;
-  const Mat m = tab.m[find(tab.m, n, KIND <= POLY ? L_UPPER : L_FULL, at, inside)];
+  const Mat m = tab.m[find(tab.m, n, KIND == GRAM ? L_GRAM : KIND == POLY ? L_POLY : L_FULL, at, inside)];
   const Scratch s(m.rows, m.cols, ws + m.ws);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lr = lane & 31, h = lane >> 5;
   char *const t_in = odd ? s.t1 : s.t0, *const t_out = odd ? s.t0 : s.t1;
-  const int Jb = KIND <= POLY ? s.Mb : s.Nb, Kb = KIND == GRAM ? s.Nb : s.Mb;
+  const int Jb = KIND <= POLY ? s.Mb : s.Nb, Ks = KIND == GRAM ? s.Nb : s.Mb;   // (Ks: blocks of k in a row of the operands)
+  const int parts = KIND == GRAM ? s.gram_parts() : 1, part = inside % parts;
+  const int K0 = part * Ks / parts, Kb = (part + 1) * Ks / parts - K0;        // this workgroup's
+  inside /= parts;
   int ti, tj;
   tile_of(inside, (s.Mb + 4 * RB - 1) / (4 * RB), (Jb + BT_C - 1) / BT_C, RB, KIND <= POLY, ti, tj);
   const int ib0 = RB * (4 * ti + wave), jb0 = BT_C * tj;   // this wave's first blocks
@@ -463,8 +485,8 @@ __global__ __launch_bounds__(NT, 2) void ns_big_kernel(char* ws, const int n, co
   // (blocks beyond the matrix are read from its last one and not stored)
   const char* U[RB];
 #pragma unroll
-  for (int i = 0; i < RB; ++i) U[i] = Ub + (long)min(ib0 + i, s.Mb - 1) * Kb * BLK + lane * 16;
-  const char* V = Vb + (long)min(jb0 + wave, Jb - 1) * Kb * BLK + lane * 16;   // this wave's block of the shared operand
+  for (int i = 0; i < RB; ++i) U[i] = Ub + ((long)min(ib0 + i, s.Mb - 1) * Ks + K0) * BLK + lane * 16;
+  const char* V = Vb + ((long)min(jb0 + wave, Jb - 1) * Ks + K0) * BLK + lane * 16;   // this wave's block of the shared operand
   f32x16 acc[RB][BT_C];
 #pragma unroll
   for (int i = 0; i < RB; ++i)
@@ -566,7 +588,31 @@ __global__ __launch_bounds__(NT, 2) void ns_big_kernel(char* ws, const int n, co
 #pragma unroll
   for (int i = 0; i < RB; ++i)
 #pragma unroll
-    for (int j = 0; j < BT_C; ++j) store_block<KIND, T, MUON>(m, a, s, acc[i][j], ib0 + i, jb0 + j, t_in, t_out, lr, h);
+    for (int j = 0; j < BT_C; ++j) store_block<KIND, T, MUON>(m, a, s, acc[i][j], ib0 + i, jb0 + j, parts > 1 ? part : -1, t_in, t_out, lr, h);
+}
+
+// A of a long matrix from its parts, in their order: a wave per block
+__global__ __launch_bounds__(NT) void ns_join_kernel(char* ws, const int n) {
+  const Table& tab = *reinterpret_cast<const Table*>(ws);
+  int inside;
+  const Mat m = tab.m[find(tab.m, n, L_JOIN, blockIdx.x, inside)];
+  const Scratch s(m.rows, m.cols, ws + m.ws);
+  const int lane = threadIdx.x & 63, block = 4 * inside + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (block >= s.Mb * s.Mb) return;
+  const int ib = block / s.Mb, jb = block - ib * s.Mb;
+  if (ib > jb) return;
+  f32x16 x;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) x[e] = 0.f;
+  const int parts = s.gram_parts();
+#pragma unroll 4
+  for (int p = 0; p < parts; ++p)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const float4 v = *part_of(s, p, ib, jb, q, lane);
+      x[4 * q] += v.x, x[4 * q + 1] += v.y, x[4 * q + 2] += v.z, x[4 * q + 3] += v.w;
+    }
+  store_block<GRAM, float, false>(m, tab.a, s, x, ib, jb, -1, nullptr, nullptr, lane & 31, lane >> 5);
 }
 
 // ---- the products in tiles of 64 x 64, for matrices that would leave most of the machine idle in larger ones: the four waves of a
@@ -580,12 +626,15 @@ __global__ __launch_bounds__(NT, 2) void ns_mid_kernel(char* ws, const int n, co
   int inside;
   const Table& tab = *reinterpret_cast<const Table*>(ws);
   const StepArgs& a = tab.a;
-  const Mat m = tab.m[find(tab.m, n, KIND <= POLY ? L_UPPER : L_FULL, at, inside)];
+  const Mat m = tab.m[find(tab.m, n, KIND == GRAM ? L_GRAM : KIND == POLY ? L_POLY : L_FULL, at, inside)];
   const Scratch s(m.rows, m.cols, ws + m.ws);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lr = lane & 31, h = lane >> 5;
   char *const t_in = odd ? s.t1 : s.t0, *const t_out = odd ? s.t0 : s.t1;
-  const int Jb = KIND <= POLY ? s.Mb : s.Nb, Kb = KIND == GRAM ? s.Nb : s.Mb;
+  const int Jb = KIND <= POLY ? s.Mb : s.Nb, Ks = KIND == GRAM ? s.Nb : s.Mb;
+  const int parts = KIND == GRAM ? s.gram_parts() : 1, part = inside % parts;
+  const int K0 = part * Ks / parts, Kb = (part + 1) * Ks / parts - K0;
+  inside /= parts;
   int ti, tj;
   tile_of(inside, (s.Mb + 1) / 2, (Jb + 1) / 2, 1, KIND <= POLY, ti, tj);
   const int ib0 = 2 * ti, jb0 = 2 * tj;
@@ -595,8 +644,8 @@ __global__ __launch_bounds__(NT, 2) void ns_mid_kernel(char* ws, const int n, co
   const char *U[2], *V[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    U[i] = Ub + (long)min(ib0 + i, s.Mb - 1) * Kb * BLK + lane * 16;
-    V[i] = Vb + (long)min(jb0 + i, Jb - 1) * Kb * BLK + lane * 16;
+    U[i] = Ub + ((long)min(ib0 + i, s.Mb - 1) * Ks + K0) * BLK + lane * 16;
+    V[i] = Vb + ((long)min(jb0 + i, Jb - 1) * Ks + K0) * BLK + lane * 16;
   }
   const int k0 = 2 * (wave * Kb / 4), k1 = 2 * ((wave + 1) * Kb / 4);   // this wave's K-steps
   f32x16 acc[2][2];
@@ -664,7 +713,7 @@ __global__ __launch_bounds__(NT, 2) void ns_mid_kernel(char* ws, const int n, co
     x[4 * q + 2] = (s0.z + s1.z) + (s2.z + s3.z);
     x[4 * q + 3] = (s0.w + s1.w) + (s2.w + s3.w);
   }
-  store_block<KIND, T, MUON>(m, a, s, x, ib0 + (wave >> 1), jb0 + (wave & 1), t_in, t_out, lr, h);
+  store_block<KIND, T, MUON>(m, a, s, x, ib0 + (wave >> 1), jb0 + (wave & 1), parts > 1 ? part : -1, t_in, t_out, lr, h);
 }
 
 // ---- matrices of at most 128 rows: a workgroup of sixteen waves holds 128 columns of X in registers, a wave one block.  The operands of the
@@ -925,9 +974,9 @@ int group(const emx_matrix* mats, int n, int i, Table& t, size_t& bytes) {
 // fifth of the places of their last round empty (two to a CU; 4096 x 4096 in 512 tiles 334 us a product against 371 in 1024; six
 // 1000 x 1500 in 288 tiles 82 us against 72 in 576; the upper half of 4096 x 4096 in 272 tiles 283 us against 256 in 528).
 template <typename F>
-int tile_size(F tiles, bool up) {
-  if (tiles(1, up) < 128) return 0;
-  const long n = tiles(2, up), rounds = (n + 511) / 512;
+int tile_size(F tiles, int launch) {
+  if (tiles(launch, 1) < 128) return 0;
+  const long n = tiles(launch, 2), rounds = (n + 511) / 512;
   return 5 * n >= 4 * 512 * rounds ? 2 : 1;
 }
 
@@ -960,15 +1009,18 @@ int run(const char* who, const emx_matrix* mats, int n, const StepArgs& a, char*
     const long lows = number(t, L_LOW, [](const Mat&, const Scratch& s) { return s.low() ? (long)s.low_wgs() : 0; });
     t.a.low_steps = std::any_of(t.m, t.m + t.n, [](const Mat& m) { const Scratch s(m.rows, m.cols, nullptr); return s.low() && s.strips() > 1; });
     // the tiles of the products, in blocks of 32: 2 x 2 (size 0), 4 x 4 (1), 8 x 4 (2)
-    const auto tiles = [&](int size, bool up) {
-      return number(t, up ? L_UPPER : L_FULL, [&](const Mat&, const Scratch& s) {
+    const auto tiles = [&](int launch, int size) {
+      return number(t, launch, [&](const Mat&, const Scratch& s) {
         const int r = size == 0 ? 2 : 4 * size, c = size == 0 ? 2 : BT_C;
-        return s.low() ? 0 : tile_count((s.Mb + r - 1) / r, ((up ? s.Mb : s.Nb) + c - 1) / c, size == 2 ? 2 : 1, up);
+        const long n = s.low() ? 0 : tile_count((s.Mb + r - 1) / r, ((launch == L_FULL ? s.Nb : s.Mb) + c - 1) / c, size == 2 ? 2 : 1, launch != L_FULL);
+        return launch == L_GRAM ? n * s.gram_parts() : n;
       });
     };
-    const int size_up = tile_size(tiles, true), size_full = tile_size(tiles, false);
-    const long uppers = tiles(size_up, true), fulls = tiles(size_full, false);
-    for (const long blocks : {norms, splits, lows, uppers, fulls}) EMX_REQUIRE(blocks < (1l << 30), "%s: %ld workgroups", who, blocks);
+    int size[L_COUNT];
+    long count[L_COUNT];
+    for (const int launch : {L_GRAM, L_POLY, L_FULL}) size[launch] = tile_size(tiles, launch), count[launch] = tiles(launch, size[launch]);
+    const long joins = number(t, L_JOIN, [](const Mat&, const Scratch& s) { return s.low() || s.gram_parts() == 1 ? 0 : ((long)s.Mb * s.Mb + 3) / 4; });
+    for (const long blocks : {norms, splits, lows, joins, count[L_GRAM], count[L_POLY], count[L_FULL]}) EMX_REQUIRE(blocks < (1l << 30), "%s: %ld workgroups", who, blocks);
 
     hipLaunchKernelGGL((ns_norm_kernel<T, MUON>), dim3((unsigned)norms), dim3(NT), 0, st, ws, t);
     int rc = check_launch(who);
@@ -982,21 +1034,24 @@ int run(const char* who, const emx_matrix* mats, int n, const StepArgs& a, char*
       hipLaunchKernelGGL((ns_low_kernel<T, MUON>), dim3((unsigned)blocks), dim3(LOW_NT), 2 * LOW_AREA, st, ws, t.n, step);
       return check_launch(who);
     };
-    const auto product = [&](auto mid, auto big1, auto big2, bool up, int k) {
-      const int size = up ? size_up : size_full;
-      const long count = up ? uppers : fulls;
-      if (count == 0) return (int)EMX_OK;
+    const auto product = [&](auto mid, auto big1, auto big2, int launch, int k) {
+      const long c = count[launch];
+      if (c == 0) return (int)EMX_OK;
       // consecutive tiles to an XCD: an eighth of them all, or -- where their lengths differ -- a few in turn, so that each gets long ones
-      const long r = uneven ? 8 : (count + 7) / 8, blocks = (count + 8 * r - 1) / (8 * r) * 8 * r;
-      hipLaunchKernelGGL((size == 0 ? mid : size == 1 ? big1 : big2), dim3((unsigned)blocks), dim3(NT), 0, st, ws, t.n, k & 1, (int)count, (int)r);
+      const long r = uneven ? 8 : (c + 7) / 8, blocks = (c + 8 * r - 1) / (8 * r) * 8 * r;
+      hipLaunchKernelGGL((size[launch] == 0 ? mid : size[launch] == 1 ? big1 : big2), dim3((unsigned)blocks), dim3(NT), 0, st, ws, t.n, k & 1, (int)c, (int)r);
       return check_launch(who);
     };
     if ((rc = low(lows, 0))) return rc;
     for (int k = 0; k < a.steps; ++k) {
-      if ((rc = product(ns_mid_kernel<GRAM, T, MUON>, ns_big_kernel<GRAM, T, MUON, 1>, ns_big_kernel<GRAM, T, MUON, 2>, true, k))) return rc;
-      if ((rc = product(ns_mid_kernel<POLY, T, MUON>, ns_big_kernel<POLY, T, MUON, 1>, ns_big_kernel<POLY, T, MUON, 2>, true, k))) return rc;
-      if (k + 1 < a.steps) rc = product(ns_mid_kernel<NEXT, T, MUON>, ns_big_kernel<NEXT, T, MUON, 1>, ns_big_kernel<NEXT, T, MUON, 2>, false, k);
-      else rc = product(ns_mid_kernel<LAST, T, MUON>, ns_big_kernel<LAST, T, MUON, 1>, ns_big_kernel<LAST, T, MUON, 2>, false, k);
+      if ((rc = product(ns_mid_kernel<GRAM, T, MUON>, ns_big_kernel<GRAM, T, MUON, 1>, ns_big_kernel<GRAM, T, MUON, 2>, L_GRAM, k))) return rc;
+      if (joins) {
+        hipLaunchKernelGGL(ns_join_kernel, dim3((unsigned)joins), dim3(NT), 0, st, ws, t.n);
+        if ((rc = check_launch(who))) return rc;
+      }
+      if ((rc = product(ns_mid_kernel<POLY, T, MUON>, ns_big_kernel<POLY, T, MUON, 1>, ns_big_kernel<POLY, T, MUON, 2>, L_POLY, k))) return rc;
+      if (k + 1 < a.steps) rc = product(ns_mid_kernel<NEXT, T, MUON>, ns_big_kernel<NEXT, T, MUON, 1>, ns_big_kernel<NEXT, T, MUON, 2>, L_FULL, k);
+      else rc = product(ns_mid_kernel<LAST, T, MUON>, ns_big_kernel<LAST, T, MUON, 1>, ns_big_kernel<LAST, T, MUON, 2>, L_FULL, k);
       if (rc || (t.a.low_steps && (rc = low(lows, k + 1)))) return rc;
     }
   }
