@@ -877,7 +877,7 @@ def layernorm_fwd(x, gamma, beta, eps, y, mean=None, rstd=None):
     ldx, ldy = _rows(x, x, "x"), _rows(y, x, "y")
     n, D = x.shape
     _on_device(x.get_device(), load().emx_layernorm_fwd, "emx_layernorm_fwd", x.data_ptr(), code, n, D, ldx, _vector(gamma, D, x, "gamma"),
-               _vector(beta, D, x, "beta"), eps, y.data_ptr(), ldy, _vector(mean, n, x, "mean"), _vector(rstd, n, x, "rstd"))
+               _vector(beta, D, x, "beta"), float(eps), y.data_ptr(), ldy, _vector(mean, n, x, "mean"), _vector(rstd, n, x, "rstd"))
 
 
 def layernorm_ws_floats(n_rows, D) -> int:
@@ -916,6 +916,8 @@ class MatrixPlan:
         self.mats = (Matrix * max(self.n, 1))()
         self.end = 0            # elements a buffer needs to hold
         for entry, (offset, rows, cols, ld, scale) in zip(self.mats, mats):
+            if not (0 <= offset < 2 ** 62 and 0 <= rows < 2 ** 31 and 0 <= cols < 2 ** 31 and 0 <= ld < 2 ** 62):    # (ctypes cuts larger ones off)
+                raise EmxError(f"MatrixPlan: a matrix of {rows} x {cols} at {offset}, row stride {ld}")
             entry.offset, entry.ld, entry.rows, entry.cols, entry.scale = int(offset), int(ld), int(rows), int(cols), float(scale)
             if rows > 0 and cols > 0:
                 self.end = max(self.end, offset + (rows - 1) * (ld if rows > 1 else 0) + cols)

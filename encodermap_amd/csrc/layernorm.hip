@@ -8,6 +8,7 @@
 // squares is taken after the mean, not as a difference of two large sums.  Sums over rows are two-pass in a fixed order: n_parts
 // partial sums of consecutive rows in the caller's workspace, then one sum over the parts.
 #include <algorithm>
+#include <cstdint>
 
 #include "emx_common.h"
 
@@ -389,6 +390,10 @@ int parts_of(long n_rows, int D) {
 bool known_type(int dtype) { return dtype == EMX_F32 || dtype == EMX_F16 || dtype == EMX_BF16; }
 size_t size_of(int dtype) { return dtype == EMX_F32 ? 4 : 2; }
 
+// row offsets stay far inside 64 bits
+bool fits(int64_t n, int64_t ld) { return ld >= 0 && n <= ((int64_t)1 << 58) / std::max<int64_t>(ld, 1); }
+bool aligned(const void* p, size_t es) { return (uintptr_t)p % es == 0; }
+
 // Is [a, a + n rows) clear of [b, ...), or the very same rows (the in-place form)?
 bool disjoint_or_same(const void* a, long lda, const void* b, long ldb, long n, int D, size_t es) {
   if (a == b && lda == ldb) return true;
@@ -458,8 +463,8 @@ int emx_layernorm_fwd(const void* x, int dtype, int64_t n_rows, int D, int64_t l
   EMX_REQUIRE(n_rows >= 0 && D >= 1 && D <= EMX_LAYERNORM_MAX_D, "%s: n_rows %lld, D %d", who, (long long)n_rows, D);
   EMX_REQUIRE(eps >= 0.f, "%s: eps %g", who, (double)eps);   // (refuses NaN)
   if (n_rows == 0) return EMX_OK;
-  EMX_REQUIRE(x && y, "%s: x and y are needed", who);
-  EMX_REQUIRE(n_rows == 1 || (ldx >= 0 && ldy >= D), "%s: row strides %lld, %lld of %d columns", who, (long long)ldx, (long long)ldy, D);
+  EMX_REQUIRE(x && y && aligned(x, size_of(dtype)) && aligned(y, size_of(dtype)), "%s: x and y are needed, on element boundaries", who);
+  EMX_REQUIRE(n_rows == 1 || (fits(n_rows, ldx) && fits(n_rows, ldy) && ldy >= D), "%s: row strides %lld, %lld of %d columns", who, (long long)ldx, (long long)ldy, D);
   if (n_rows == 1) ldx = ldy = D;
   EMX_REQUIRE(disjoint_or_same(x, ldx, y, ldy, n_rows, D, size_of(dtype)), "%s: x and y overlap without being the same rows", who);
   const FwdArgs a{x, y, gamma, beta, mean, rstd, n_rows, ldx, ldy, D, eps};
@@ -480,8 +485,8 @@ int emx_layernorm_bwd(const void* dy, int64_t ld_dy, const void* x, int64_t ldx,
   const bool sums = dgamma || dbeta;
   const size_t es = size_of(dtype);
   if (n_rows > 0) {
-    EMX_REQUIRE(dy && x && mean && rstd, "%s: dy, x, mean and rstd are needed", who);
-    EMX_REQUIRE(n_rows == 1 || (ld_dy >= 0 && ldx >= 0 && (!dx || ld_dx >= D)), "%s: row strides %lld, %lld, %lld of %d columns", who,
+    EMX_REQUIRE(dy && x && mean && rstd && aligned(dy, es) && aligned(x, es) && aligned(dx, es), "%s: dy, x, mean and rstd are needed, on element boundaries", who);
+    EMX_REQUIRE(n_rows == 1 || (fits(n_rows, ld_dy) && fits(n_rows, ldx) && (!dx || (fits(n_rows, ld_dx) && ld_dx >= D))), "%s: row strides %lld, %lld, %lld of %d columns", who,
                 (long long)ld_dy, (long long)ldx, (long long)ld_dx, D);
     if (n_rows == 1) ld_dy = ldx = ld_dx = D;
     EMX_REQUIRE(!dx || (disjoint_or_same(dx, ld_dx, dy, ld_dy, n_rows, D, es) && disjoint_or_same(dx, ld_dx, x, ldx, n_rows, D, es)),

@@ -21,6 +21,7 @@
 #include <algorithm>
 #include <climits>
 #include <cstdint>
+#include <new>
 #include <type_traits>
 #include <vector>
 
@@ -928,18 +929,21 @@ __global__ __launch_bounds__(LOW_NT) void ns_low_kernel(char* ws, const int n, c
 }
 
 // ---- host side
-int check_matrices(const char* who, const emx_matrix* mats, int n) {
+struct Span {
+  int64_t a, b, ld;    // first element, behind the last one, row stride (0: one row)
+  int cols;
+};
+int check_matrices(const char* who, const emx_matrix* mats, int n) try {
   EMX_REQUIRE(n >= 0 && (n == 0 || mats), "%s: %d matrices", who, n);
-  struct Span { int64_t a, b, ld; int cols; };
   std::vector<Span> spans;
   for (int i = 0; i < n; ++i) {
     const emx_matrix& m = mats[i];
-    EMX_REQUIRE(m.rows >= 0 && m.cols >= 0 && m.offset >= 0, "%s: matrix %d: %d x %d at %lld", who, i, m.rows, m.cols, (long long)m.offset);
+    EMX_REQUIRE(m.rows >= 0 && m.cols >= 0 && m.offset >= 0 && m.offset <= (int64_t)1 << 50, "%s: matrix %d: %d x %d at %lld", who, i, m.rows, m.cols,
+                (long long)m.offset);
     if (m.rows == 0 || m.cols == 0) continue;
     if (m.rows > EMX_MATRIX_MAX_SIDE || m.cols > EMX_MATRIX_MAX_SIDE)
       return fail(EMX_EUNSUPPORTED, "%s: matrix %d: %d x %d (at most %d a side)", who, i, m.rows, m.cols, EMX_MATRIX_MAX_SIDE);
-    EMX_REQUIRE(m.rows == 1 || m.ld >= m.cols, "%s: matrix %d: row stride %lld of %d columns", who, i, (long long)m.ld, m.cols);
-    EMX_REQUIRE(m.rows == 1 || m.ld <= (int64_t)1 << 40, "%s: matrix %d: row stride %lld", who, i, (long long)m.ld);
+    EMX_REQUIRE(m.rows == 1 || (m.ld >= m.cols && m.ld <= (int64_t)1 << 40), "%s: matrix %d: row stride %lld of %d columns", who, i, (long long)m.ld, m.cols);
     spans.push_back({m.offset, m.offset + (m.rows == 1 ? 0 : (m.rows - 1) * m.ld) + m.cols, m.rows == 1 ? 0 : m.ld, m.cols});
   }
   // every element is updated by ONE matrix: spans apart, or columns side by side in rows of the same length
@@ -952,9 +956,26 @@ int check_matrices(const char* who, const emx_matrix* mats, int n) {
       EMX_REQUIRE(beside, "%s: matrices at %lld and %lld overlap", who, (long long)x.a, (long long)y.a);
     }
   return EMX_OK;
+} catch (const std::bad_alloc&) {
+  return fail(EMX_EINVAL, "%s: no host memory for %d matrices", who, n);
 }
 
 bool empty(const emx_matrix& m) { return m.rows == 0 || m.cols == 0; }
+
+// the elements from the first matrix' first to the last one's last
+void extent(const emx_matrix* mats, int n, int64_t& lo, int64_t& hi) {
+  lo = INT64_MAX, hi = 0;
+  for (int i = 0; i < n; ++i)
+    if (!empty(mats[i])) {
+      lo = std::min(lo, mats[i].offset);
+      hi = std::max(hi, mats[i].offset + (mats[i].rows == 1 ? 0 : (mats[i].rows - 1) * mats[i].ld) + mats[i].cols);
+    }
+}
+// do elements [lo, hi) of one buffer and [lo, hi + more) of another share memory?
+bool share(const void* a, const void* b, int64_t lo, int64_t hi, int64_t more, size_t es) {
+  const uintptr_t a0 = (uintptr_t)a + lo * es, a1 = (uintptr_t)a + hi * es, b0 = (uintptr_t)b + lo * es, b1 = (uintptr_t)b + (hi + more) * es;
+  return a0 < b1 && b0 < a1;
+}
 
 // the matrices of one launch group: at most MAX_TABLE of them from index i on; returns the index behind them
 int group(const emx_matrix* mats, int n, int i, Table& t, size_t& bytes) {
@@ -1058,20 +1079,30 @@ int run(const char* who, const emx_matrix* mats, int n, const StepArgs& a, char*
   return EMX_OK;
 }
 
+size_t ws_bytes_of(const emx_matrix* mats, int n) {   // (groups run one after the other, in the same scratch)
+  size_t most = 16;
+  for (int i = 0; i < n;) {
+    Table t;
+    size_t bytes;
+    i = group(mats, n, i, t, bytes);
+    most = std::max(most, bytes);
+  }
+  return most;
+}
+
+int check_workspace(const char* who, const emx_matrix* mats, int n, const void* ws, size_t ws_bytes) {
+  const size_t need = ws_bytes_of(mats, n);
+  if (!ws || ws_bytes < need || ((uintptr_t)ws & 15))
+    return fail(EMX_EWORKSPACE, "%s: workspace of %zu bytes at %p, %zu needed on a 16-byte boundary", who, ws_bytes, ws, need);
+  return EMX_OK;
+}
+
 }  // namespace
 
 extern "C" {
 
 size_t emx_orthogonalize_ws_bytes(const emx_matrix* mats, int n_mats) {
-  if (check_matrices("emx_orthogonalize_ws_bytes", mats, n_mats)) return 0;
-  size_t most = 16;
-  for (int i = 0; i < n_mats;) {
-    Table t;
-    size_t bytes;
-    i = group(mats, n_mats, i, t, bytes);
-    most = std::max(most, bytes);
-  }
-  return most;
+  return check_matrices("emx_orthogonalize_ws_bytes", mats, n_mats) ? 0 : ws_bytes_of(mats, n_mats);
 }
 
 int emx_orthogonalize(const emx_matrix* mats, int n_mats, const void* g, void* out, int dtype, int steps, float eps, void* ws, size_t ws_bytes,
@@ -1083,10 +1114,12 @@ int emx_orthogonalize(const emx_matrix* mats, int n_mats, const void* g, void* o
   EMX_REQUIRE(steps >= 1 && steps <= EMX_ORTHOGONALIZE_MAX_STEPS, "%s: %d steps", who, steps);
   EMX_REQUIRE(eps > 0.f && std::isfinite(eps), "%s: eps %g", who, (double)eps);
   if (std::all_of(mats, mats + n_mats, empty)) return EMX_OK;
-  EMX_REQUIRE(g && out, "%s: g and out are needed", who);
-  if (!ws || ws_bytes < emx_orthogonalize_ws_bytes(mats, n_mats) || ((uintptr_t)ws & 15))
-    return fail(EMX_EWORKSPACE, "%s: workspace of %zu bytes at %p, %zu needed on a 16-byte boundary", who, ws_bytes, ws,
-                emx_orthogonalize_ws_bytes(mats, n_mats));
+  const size_t es = dtype == EMX_F32 ? 4 : 2;
+  EMX_REQUIRE(g && out && (uintptr_t)g % es == 0 && (uintptr_t)out % es == 0, "%s: g and out are needed, on element boundaries", who);
+  int64_t lo, hi;
+  extent(mats, n_mats, lo, hi);
+  EMX_REQUIRE(g == out || !share(g, out, lo, hi, 0, es), "%s: g and out overlap without being the same buffer", who);
+  if ((rc = check_workspace(who, mats, n_mats, ws, ws_bytes))) return rc;
   StepArgs a{};
   a.g = g, a.out = out, a.n_slices = 1, a.steps = steps, a.eps = eps;
   hipStream_t st = (hipStream_t)stream;
@@ -1100,18 +1133,20 @@ int emx_muon_step(const emx_matrix* mats, int n_mats, float* w, const float* g, 
   const char* who = "emx_muon_step";
   int rc = check_matrices(who, mats, n_mats);
   if (rc) return rc;
-  EMX_REQUIRE(n_slices >= 1 && (n_slices == 1 || slice_stride >= 0), "%s: %d slices, stride %lld", who, n_slices, (long long)slice_stride);
+  EMX_REQUIRE(n_slices >= 1 && (n_slices == 1 || (slice_stride >= 0 && slice_stride <= ((int64_t)1 << 50) / n_slices)), "%s: %d slices, stride %lld", who, n_slices, (long long)slice_stride);
   EMX_REQUIRE(std::isfinite(lr) && beta >= 0.f && beta < 1.f && std::isfinite(weight_decay), "%s: lr %g, momentum %g, weight decay %g", who,
               (double)lr, (double)beta, (double)weight_decay);
   EMX_REQUIRE(steps >= 1 && steps <= EMX_ORTHOGONALIZE_MAX_STEPS, "%s: %d steps", who, steps);
   EMX_REQUIRE(eps > 0.f && std::isfinite(eps), "%s: eps %g", who, (double)eps);
   for (int i = 0; i < n_mats; ++i) EMX_REQUIRE(std::isfinite(mats[i].scale), "%s: matrix %d: scale %g", who, i, (double)mats[i].scale);
   if (std::all_of(mats, mats + n_mats, empty)) return EMX_OK;
-  EMX_REQUIRE(w && g && momentum, "%s: w, g and momentum are needed", who);
-  EMX_REQUIRE(w != g && w != momentum && momentum != g, "%s: w, g and momentum have to be three buffers", who);
-  if (!ws || ws_bytes < emx_orthogonalize_ws_bytes(mats, n_mats) || ((uintptr_t)ws & 15))
-    return fail(EMX_EWORKSPACE, "%s: workspace of %zu bytes at %p, %zu needed on a 16-byte boundary", who, ws_bytes, ws,
-                emx_orthogonalize_ws_bytes(mats, n_mats));
+  EMX_REQUIRE(w && g && momentum && ((uintptr_t)w | (uintptr_t)g | (uintptr_t)momentum) % 4 == 0, "%s: w, g and momentum are needed, on element boundaries", who);
+  int64_t lo, hi;
+  extent(mats, n_mats, lo, hi);
+  const int64_t more = n_slices > 1 ? (n_slices - 1) * slice_stride : 0;
+  EMX_REQUIRE(!share(w, momentum, lo, hi, 0, 4) && !share(w, g, lo, hi, more, 4) && !share(momentum, g, lo, hi, more, 4),
+              "%s: w, g and momentum have to be three buffers", who);
+  if ((rc = check_workspace(who, mats, n_mats, ws, ws_bytes))) return rc;
   StepArgs a{};
   a.g = g, a.w = w, a.mom = momentum, a.slice_stride = slice_stride, a.n_slices = n_slices, a.nesterov = nesterov != 0, a.steps = steps;
   a.beta = beta, a.keep = (float)(1.0 - (double)lr * weight_decay), a.lr = lr, a.eps = eps;

@@ -579,7 +579,8 @@ int emx_mlp_wgrad_adam_local(const emx_mlp_desc* desc, float* params, int64_t n_
  *   gamma, beta, mean, rstd, dgamma, dbeta: float32.  gamma / beta NULL: ones / zeros.  mean / rstd NULL (forward): not kept.
  *   dx, dgamma, dbeta NULL: not wanted.  dgamma and dbeta are overwritten, not added to; without rows they are zero.
  *   y may be x, dx may be dy or x (same pointer, same stride); any other overlap of their address ranges is refused.
- *   A row with an infinity or a NaN gives NaN in its own results (and in dgamma / dbeta); eps = 0 gives NaN for a constant row.
+ *   A row with an infinity or a NaN gives NaN in its own results (and in dgamma / dbeta); eps = 0 gives NaN for a constant row.  Sums are
+ *   float32: a row that leaves its mean by more than 1e19 overflows its sum of squares (rstd = 0).
  *   ws: emx_layernorm_ws_floats(n_rows, D) floats of scratch (may be NULL where dgamma and dbeta are); its contents mean nothing
  *   between calls, calls that may run at the same time need one each.
  * ------------------------------------------------------------------------------------------------ */
@@ -600,7 +601,7 @@ int emx_layernorm_bwd(const void* dy, int64_t ld_dy, const void* x, int64_t ldx,
  *   emx_matrix: a matrix of the flat buffers the call is given: rows x cols elements from `offset` on, row stride `ld` >= cols; `scale` is
  *     the factor of its update in emx_muon_step.  Matrices of a call may not share elements; rows or cols may be 0 (nothing is done).
  *   emx_orthogonalize: out <- orth(g) for every matrix; g and out (EMX_F32 / EMX_F16 / EMX_BF16, the same offsets in both) may be the same
- *     buffer.  What lies between the matrices is neither read nor written.
+ *     buffer (any other overlap is refused, as is any between w, g and momentum below).  What lies between the matrices is neither read nor written.
  *   emx_muon_step, float32:  G = sum over n_slices of g[s * slice_stride + .] in order (the weight-gradient partials of emx_mlp_wgrad, or one
  *     gradient);  momentum <- beta momentum + G;  U = nesterov ? G + beta momentum : momentum;  w <- w (1 - lr weight_decay) - lr scale orth(U).
  *     0 <= beta < 1.  The operand store of the dense-layer launches is NOT rewritten: emx_mlp_mirror afterwards.

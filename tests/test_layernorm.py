@@ -24,6 +24,8 @@ def bwd(dy=P, ld_dy=8, x=2 * P, ldx=8, dtype=0, n=4, D=8, mean=3 * P, rstd=3 * P
     dict(y=P + 4),               # shifted rows of the same memory
     dict(y=P, ldx=8, ldy=16),    # the same start with another stride
     dict(y=P + 4 * 31),          # the first row of one is the end of the other
+    dict(x=P + 2), dict(y=2 * P + 1),                     # not on an element boundary
+    dict(n=1 << 40, ldx=1 << 30), dict(n=1 << 40, ldy=1 << 30),
 ])
 def test_forward_refuses(bad):
     assert fwd(**bad) == -1
@@ -32,7 +34,7 @@ def test_forward_refuses(bad):
 
 @pytest.mark.parametrize("bad", [
     dict(dtype=9), dict(n=-1), dict(D=0), dict(dy=None), dict(x=None), dict(mean=None), dict(rstd=None), dict(ldx=-1), dict(ld_dy=-1), dict(ld_dx=7),
-    dict(dx=P + 4), dict(dx=2 * P - 4), dict(dx=P, ld_dx=16),
+    dict(dx=P + 4), dict(dx=2 * P - 4), dict(dx=P, ld_dx=16), dict(dy=P + 1), dict(x=2 * P + 2), dict(dx=4 * P + 3), dict(n=1 << 40, ldx=1 << 30, ws_floats=1 << 40),
 ])
 def test_backward_refuses(bad):
     assert bwd(**bad) == -1

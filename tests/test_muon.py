@@ -42,7 +42,7 @@ ONE = [(0, 8, 4)]
     ([(0, 8, 4, 10), (3, 8, 4, 10)], -1),            # column blocks that share a column
     ([(0, 8, 4, 10), (8, 8, 4, 10)], -1),            # ... that run over the row's end into the next row's first columns
     ([(0, 8, 4, 10), (5, 8, 4, 11)], -1),            # rows of two lengths between one another
-    ([(100, 2, 2), (0, 60, 4, 4), (96, 1, 8)], -1),
+    ([(100, 2, 2), (0, 60, 4, 4), (96, 1, 8)], -1), ([((1 << 50) + 1, 2, 2)], -1),
 ])
 def test_matrices_that_are_refused(mats, code):
     assert need(*mats) == 0
@@ -59,7 +59,7 @@ def test_matrices_that_are_taken(mats):
 
 
 @pytest.mark.parametrize("bad", [dict(dtype=3), dict(steps=0), dict(steps=65), dict(eps=0.0), dict(eps=-1.0), dict(eps=float("nan")), dict(eps=float("inf")),
-                                 dict(g=None), dict(out=None)])
+                                 dict(g=None), dict(out=None), dict(g=P + 2), dict(out=2 * P + 1), dict(out=P + 4), dict(out=P - 4 * 31)])
 def test_orthogonalize_refuses(bad):
     assert ortho(ONE, **bad) == -1
     assert b"emx_orthogonalize" in _lib.load().emx_last_error()
@@ -67,7 +67,8 @@ def test_orthogonalize_refuses(bad):
 
 @pytest.mark.parametrize("bad", [dict(slices=0), dict(slices=2, stride=-1), dict(lr=float("nan")), dict(lr=float("inf")), dict(beta=1.0), dict(beta=-0.1),
                                  dict(beta=float("nan")), dict(decay=float("nan")), dict(steps=0), dict(steps=65), dict(eps=0.0), dict(w=None), dict(g=None),
-                                 dict(m=None), dict(w=2 * P), dict(m=P), dict(m=2 * P)])
+                                 dict(m=None), dict(w=2 * P), dict(m=P), dict(m=2 * P), dict(w=P + 2), dict(m=P + 4), dict(w=2 * P + 4 * 31),
+                                 dict(g=P - 4 * 99, slices=2, stride=100), dict(slices=3, stride=1 << 60)])
 def test_muon_refuses(bad):
     assert muon(ONE, **bad) == -1
     assert b"emx_muon_step" in _lib.load().emx_last_error()
@@ -104,4 +105,7 @@ def test_plan_of_a_layout():
         _lib.orthogonalize(plan, torch.zeros(lay.n_params), torch.zeros(lay.n_params))
     with pytest.raises(_lib.EmxError, match="overlap"):
         _lib.MatrixPlan([(0, 4, 4, 4, 1.0), (15, 4, 4, 4, 1.0)], device="cpu")
+    for bad in ((0, 2 ** 32 + 4, 4, 4, 1.0), (0, 4, 2 ** 32 + 4, 4, 1.0), (-1, 4, 4, 4, 1.0), (0, 4, 4, 2 ** 64 + 4, 1.0)):
+        with pytest.raises(_lib.EmxError):
+            _lib.MatrixPlan([bad], device="cpu")
     assert C.sizeof(_lib.Matrix) == 32
