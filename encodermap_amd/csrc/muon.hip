@@ -460,27 +460,55 @@ __device__ __forceinline__ void store_block(const Mat& m, const StepArgs& a, con
   }
 }
 
+// What tile `at` of a product is: its matrix, its place, and its blocks of k
+template <int KIND, int RB>
+struct Unit {
+  Mat m;
+  Scratch s;
+  int parts, part, Ks, K0, Kb, ti, tj;   // (Ks: blocks of k in a row of the operands)
+  __device__ __forceinline__ Unit(char* ws, int n, int at) : s(1, 1, nullptr) {
+    const Table& tab = *reinterpret_cast<const Table*>(ws);
+    int inside;
+    m = tab.m[find(tab.m, n, KIND == GRAM ? L_GRAM : KIND == POLY ? L_POLY : L_FULL, at, inside)];
+    s = Scratch(m.rows, m.cols, ws + m.ws);
+    Ks = KIND == GRAM ? s.Nb : s.Mb;
+    parts = KIND == GRAM ? s.gram_parts() : 1, part = inside % parts;
+    K0 = part * Ks / parts, Kb = (part + 1) * Ks / parts - K0;
+    tile_of(inside / parts, (s.Mb + 4 * RB - 1) / (4 * RB), ((KIND <= POLY ? s.Mb : s.Nb) + BT_C - 1) / BT_C, RB, KIND <= POLY, ti, tj);
+  }
+};
+// The last tiles of a launch, too few to go round the CUs: each cut into `cuts` along k.  Their shares, behind the table in the workspace.
+__device__ __forceinline__ float4* cut_of(char* ws, int rb, int unit, int cuts, int cut, int wave, int i, int j, int q, int lane) {
+  return reinterpret_cast<float4*>(ws + TABLE_BYTES + ((((long)unit * cuts + cut) * 4 + wave) * rb * BT_C + i * BT_C + j) * BLK + q * 1024 + lane * 16);
+}
+
 template <int KIND, typename T, bool MUON, int RB>
-__global__ __launch_bounds__(NT, 2) void ns_big_kernel(char* ws, const int n, const int odd, const int total, const int run) {
+__global__ __launch_bounds__(NT, 2) void ns_big_kernel(char* ws, const int n, const int odd, const int whole, const int run, const int first_cut,
+                                                       const int cuts) {
   __shared__ __align__(16) char lds[2][BT_C * BLK];
   // runs of consecutive tiles to each XCD: they share operands in its L2
-  const int turn = (int)(blockIdx.x >> 3), at = ((turn / run) * 8 + (int)(blockIdx.x & 7)) * run + turn % run;
-  if (at >= total) return;
-  int inside;
-  const Table& tab = *reinterpret_cast<const Table*>(ws);
-  const StepArgs& a = tab.a;
-  const Mat m = tab.m[find(tab.m, n, KIND == GRAM ? L_GRAM : KIND == POLY ? L_POLY : L_FULL, at, inside)];
-  const Scratch s(m.rows, m.cols, ws + m.ws);
+  const int turn = (int)(blockIdx.x >> 3);
+  int at = ((turn / run) * 8 + (int)(blockIdx.x & 7)) * run + turn % run, cut = -1;
+  if ((int)blockIdx.x >= first_cut) {
+    const int c = (int)blockIdx.x - first_cut;
+    at = whole + c / cuts, cut = c % cuts;
+  } else if (at >= whole) {
+    return;
+  }
+  const Unit<KIND, RB> unit(ws, n, at);
+  const StepArgs& a = reinterpret_cast<const Table*>(ws)->a;
+  const Mat& m = unit.m;
+  const Scratch& s = unit.s;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lr = lane & 31, h = lane >> 5;
   char *const t_in = odd ? s.t1 : s.t0, *const t_out = odd ? s.t0 : s.t1;
-  const int Jb = KIND <= POLY ? s.Mb : s.Nb, Ks = KIND == GRAM ? s.Nb : s.Mb;   // (Ks: blocks of k in a row of the operands)
-  const int parts = KIND == GRAM ? s.gram_parts() : 1, part = inside % parts;
-  const int K0 = part * Ks / parts, Kb = (part + 1) * Ks / parts - K0;        // this workgroup's
-  inside /= parts;
-  int ti, tj;
-  tile_of(inside, (s.Mb + 4 * RB - 1) / (4 * RB), (Jb + BT_C - 1) / BT_C, RB, KIND <= POLY, ti, tj);
-  const int ib0 = RB * (4 * ti + wave), jb0 = BT_C * tj;   // this wave's first blocks
+  const int Jb = KIND <= POLY ? s.Mb : s.Nb, Ks = unit.Ks, parts = unit.parts, part = unit.part;
+  int K0 = unit.K0, Kb = unit.Kb;                          // this workgroup's blocks of k
+  if (cut >= 0) {
+    K0 += cut * unit.Kb / cuts;
+    Kb = (cut + 1) * unit.Kb / cuts - cut * unit.Kb / cuts;
+  }
+  const int ib0 = RB * (4 * unit.ti + wave), jb0 = BT_C * unit.tj;   // this wave's first blocks
   const char* const Ub = KIND == GRAM ? s.x : KIND == POLY ? s.a : s.p;
   const char* const Vb = KIND == GRAM ? s.x : KIND == POLY ? s.a : t_in;
   // (blocks beyond the matrix are read from its last one and not stored)
@@ -586,10 +614,45 @@ __global__ __launch_bounds__(NT, 2) void ns_big_kernel(char* ws, const int n, co
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[0][j][e] += sum[j][e];
   }
+  if (cut >= 0) {
+#pragma unroll
+    for (int i = 0; i < RB; ++i)
+#pragma unroll
+      for (int j = 0; j < BT_C; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          *cut_of(ws, RB, at - whole, cuts, cut, wave, i, j, q, lane) =
+              make_float4(acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]);
+    return;
+  }
 #pragma unroll
   for (int i = 0; i < RB; ++i)
 #pragma unroll
     for (int j = 0; j < BT_C; ++j) store_block<KIND, T, MUON>(m, a, s, acc[i][j], ib0 + i, jb0 + j, parts > 1 ? part : -1, t_in, t_out, lr, h);
+}
+
+// The tiles that were cut, from their shares in the shares' order: a workgroup per column of blocks
+template <int KIND, typename T, bool MUON, int RB>
+__global__ __launch_bounds__(NT) void ns_whole_kernel(char* ws, const int n, const int odd, const int whole, const int cuts) {
+  const int u = (int)blockIdx.x / BT_C, j = (int)blockIdx.x % BT_C;
+  const Unit<KIND, RB> unit(ws, n, whole + u);
+  const Scratch& s = unit.s;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+#pragma unroll
+  for (int i = 0; i < RB; ++i) {
+    f32x16 x;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) x[e] = 0.f;
+#pragma unroll 4
+    for (int c = 0; c < cuts; ++c)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const float4 v = *cut_of(ws, RB, u, cuts, c, wave, i, j, q, lane);
+        x[4 * q] += v.x, x[4 * q + 1] += v.y, x[4 * q + 2] += v.z, x[4 * q + 3] += v.w;
+      }
+    store_block<KIND, T, MUON>(unit.m, reinterpret_cast<const Table*>(ws)->a, s, x, RB * (4 * unit.ti + wave) + i, BT_C * unit.tj + j,
+                               unit.parts > 1 ? unit.part : -1, odd ? s.t1 : s.t0, odd ? s.t0 : s.t1, lane & 31, lane >> 5);
+  }
 }
 
 // A of a long matrix from its parts, in their order: a wave per block
@@ -620,7 +683,7 @@ __global__ __launch_bounds__(NT) void ns_join_kernel(char* ws, const int n) {
 // workgroup take a quarter of k each, straight from global memory (four K-steps of operands in registers: three travel under the products of
 // one), and add up through LDS, a block to each wave.
 template <int KIND, typename T, bool MUON>
-__global__ __launch_bounds__(NT, 2) void ns_mid_kernel(char* ws, const int n, const int odd, const int total, const int run) {
+__global__ __launch_bounds__(NT, 2) void ns_mid_kernel(char* ws, const int n, const int odd, const int total, const int run, int, int) {
   __shared__ __align__(16) float4 fold[4][3][4][64];   // [block][wave but its own][q][lane]
   const int turn = (int)(blockIdx.x >> 3), at = ((turn / run) * 8 + (int)(blockIdx.x & 7)) * run + turn % run;
   if (at >= total) return;
@@ -977,16 +1040,15 @@ bool share(const void* a, const void* b, int64_t lo, int64_t hi, int64_t more, s
   return a0 < b1 && b0 < a1;
 }
 
-// the matrices of one launch group: at most MAX_TABLE of them from index i on; returns the index behind them
-int group(const emx_matrix* mats, int n, int i, Table& t, size_t& bytes) {
-  t.n = 0, bytes = TABLE_BYTES;
-  for (; i < n && t.n < MAX_TABLE; ++i) {
-    const emx_matrix& m = mats[i];
-    if (empty(m)) continue;
-    t.m[t.n++] = Mat{m.offset, m.rows == 1 ? m.cols : m.ld, (long)bytes, m.rows, m.cols, m.scale, {}};
-    bytes += Scratch::bytes(m.rows, m.cols);
+// hands out the workgroups (or tiles) of a launch
+template <typename F>
+long number(Table& t, int launch, F blocks) {
+  long at = 0;
+  for (int i = 0; i < t.n; ++i) {
+    t.m[i].begin[launch] = (int)std::min(at, (long)INT_MAX);
+    at += blocks(t.m[i], Scratch(t.m[i].rows, t.m[i].cols, nullptr));
   }
-  return i;
+  return at;
 }
 
 // Which tiles a product runs in.  64 x 64 with k shared out over the waves below 128 tiles of 128 x 128: such a launch is bound by the time from
@@ -1001,79 +1063,118 @@ int tile_size(F tiles, int launch) {
   return 5 * n >= 4 * 512 * rounds ? 2 : 1;
 }
 
-// hands out the workgroups (or tiles) of a launch
-template <typename F>
-long number(Table& t, int launch, F blocks) {
-  long at = 0;
-  for (int i = 0; i < t.n; ++i) {
-    t.m[i].begin[launch] = (int)std::min(at, (long)INT_MAX);
-    at += blocks(t.m[i], Scratch(t.m[i].rows, t.m[i].cols, nullptr));
+// The last tiles of a launch that has a whole round of them for the 256 CUs and at most half a round more: cut along k into as many parts as fill
+// the round (16 at most, four blocks of k to each): the upper half of 4096 x 4096, 528 tiles, 255 us -> 193 + 8 in ns_whole_kernel; six 1000 x 1500, 576
+// tiles, 72 -> 61 + 6.  Below 1024 k a tile is done in the time that ns_whole_kernel takes.
+constexpr long CUS = 256;
+int cuts_of(int size, long count, int blocks_of_k) {
+  const long rest = count % CUS;
+  if (size == 0 || count < CUS || rest == 0 || blocks_of_k < 32) return 1;
+  return (int)std::min({CUS / rest, (long)blocks_of_k / 4, 16l});
+}
+
+// The launches of one group of matrices: at most MAX_TABLE of them from index i on.  Returns the index behind them.
+struct Plan {
+  long norms, splits, lows, joins;                     // workgroups
+  int size[L_COUNT], cuts[L_COUNT];                    // of the products: tiles, and what the last of them are cut into
+  long count[L_COUNT], whole[L_COUNT];
+  bool uneven;
+  size_t bytes;                                        // of the workspace
+};
+int plan_group(const emx_matrix* mats, int n, int i, Table& t, Plan& p) {
+  t.n = 0;
+  for (; i < n && t.n < MAX_TABLE; ++i)
+    if (!empty(mats[i])) t.m[t.n++] = Mat{mats[i].offset, mats[i].rows == 1 ? mats[i].cols : mats[i].ld, 0, mats[i].rows, mats[i].cols, mats[i].scale, {}};
+  // the long ones first: a launch ends with short tiles
+  const auto length = [](const Mat& m) { return std::max(m.rows, m.cols); };
+  std::stable_sort(t.m, t.m + t.n, [&](const Mat& x, const Mat& y) { return length(x) > length(y); });
+  p.uneven = t.n > 0 && length(t.m[0]) != length(t.m[t.n - 1]);
+  p.norms = number(t, L_NORM, [](const Mat& m, const Scratch&) { return (long)parts_of((long)m.rows * m.cols); });
+  p.splits = number(t, L_SPLIT, [](const Mat&, const Scratch& s) { return s.low() ? 0 : (long)((s.Mb + 1) / 2) * ((s.Nb + 1) / 2); });
+  p.lows = number(t, L_LOW, [](const Mat&, const Scratch& s) { return s.low() ? (long)s.low_wgs() : 0; });
+  p.joins = number(t, L_JOIN, [](const Mat&, const Scratch& s) { return s.low() || s.gram_parts() == 1 ? 0 : ((long)s.Mb * s.Mb + 3) / 4; });
+  t.a.low_steps = 0;
+  // the tiles of the products, in blocks of 32: 2 x 2 (size 0), 4 x 4 (1), 8 x 4 (2)
+  const auto tiles = [&](int launch, int size) {
+    return number(t, launch, [&](const Mat&, const Scratch& s) {
+      const int r = size == 0 ? 2 : 4 * size, c = size == 0 ? 2 : BT_C;
+      const long n = s.low() ? 0 : tile_count((s.Mb + r - 1) / r, ((launch == L_FULL ? s.Nb : s.Mb) + c - 1) / c, size == 2 ? 2 : 1, launch != L_FULL);
+      return launch == L_GRAM ? n * s.gram_parts() : n;
+    });
+  };
+  size_t shares = 0;
+  for (const int launch : {L_GRAM, L_POLY, L_FULL}) {
+    p.size[launch] = tile_size(tiles, launch);
+    p.count[launch] = p.whole[launch] = tiles(launch, p.size[launch]);
+    int shortest = INT_MAX;
+    for (int j = 0; j < t.n; ++j) {
+      const Scratch s(t.m[j].rows, t.m[j].cols, nullptr);
+      if (!s.low()) shortest = std::min(shortest, launch == L_GRAM ? s.Nb / s.gram_parts() : s.Mb);
+    }
+    p.cuts[launch] = cuts_of(p.size[launch], p.count[launch], shortest);
+    if (p.cuts[launch] > 1) {
+      p.whole[launch] = p.count[launch] / CUS * CUS;
+      shares = std::max(shares, (size_t)(p.count[launch] % CUS) * p.cuts[launch] * p.size[launch] * 16 * BLK);
+    }
   }
-  return at;
+  p.bytes = TABLE_BYTES + shares;
+  for (int j = 0; j < t.n; ++j) {
+    const Scratch s(t.m[j].rows, t.m[j].cols, nullptr);
+    if (s.low() && s.strips() > 1) t.a.low_steps = 1;
+    t.m[j].ws = (long)p.bytes;
+    p.bytes += Scratch::bytes(t.m[j].rows, t.m[j].cols);
+  }
+  return i;
 }
 
 template <typename T, bool MUON>
 int run(const char* who, const emx_matrix* mats, int n, const StepArgs& a, char* ws, hipStream_t st) {
   for (int i = 0; i < n;) {
     Table t{};
+    Plan p;
     t.a = a;
-    size_t bytes;
-    i = group(mats, n, i, t, bytes);
+    i = plan_group(mats, n, i, t, p);
     if (t.n == 0) break;
-    // the long ones first: a launch ends with short tiles
-    const auto length = [](const Mat& m) { return std::max(m.rows, m.cols); };
-    std::stable_sort(t.m, t.m + t.n, [&](const Mat& x, const Mat& y) { return length(x) > length(y); });
-    const bool uneven = length(t.m[0]) != length(t.m[t.n - 1]);
-
-    const long norms = number(t, L_NORM, [](const Mat& m, const Scratch&) { return (long)parts_of((long)m.rows * m.cols); });
-    const long splits = number(t, L_SPLIT, [](const Mat&, const Scratch& s) { return s.low() ? 0 : (long)((s.Mb + 1) / 2) * ((s.Nb + 1) / 2); });
-    const long lows = number(t, L_LOW, [](const Mat&, const Scratch& s) { return s.low() ? (long)s.low_wgs() : 0; });
-    t.a.low_steps = std::any_of(t.m, t.m + t.n, [](const Mat& m) { const Scratch s(m.rows, m.cols, nullptr); return s.low() && s.strips() > 1; });
-    // the tiles of the products, in blocks of 32: 2 x 2 (size 0), 4 x 4 (1), 8 x 4 (2)
-    const auto tiles = [&](int launch, int size) {
-      return number(t, launch, [&](const Mat&, const Scratch& s) {
-        const int r = size == 0 ? 2 : 4 * size, c = size == 0 ? 2 : BT_C;
-        const long n = s.low() ? 0 : tile_count((s.Mb + r - 1) / r, ((launch == L_FULL ? s.Nb : s.Mb) + c - 1) / c, size == 2 ? 2 : 1, launch != L_FULL);
-        return launch == L_GRAM ? n * s.gram_parts() : n;
-      });
-    };
-    int size[L_COUNT];
-    long count[L_COUNT];
-    for (const int launch : {L_GRAM, L_POLY, L_FULL}) size[launch] = tile_size(tiles, launch), count[launch] = tiles(launch, size[launch]);
-    const long joins = number(t, L_JOIN, [](const Mat&, const Scratch& s) { return s.low() || s.gram_parts() == 1 ? 0 : ((long)s.Mb * s.Mb + 3) / 4; });
-    for (const long blocks : {norms, splits, lows, joins, count[L_GRAM], count[L_POLY], count[L_FULL]}) EMX_REQUIRE(blocks < (1l << 30), "%s: %ld workgroups", who, blocks);
-
-    hipLaunchKernelGGL((ns_norm_kernel<T, MUON>), dim3((unsigned)norms), dim3(NT), 0, st, ws, t);
+    for (const long blocks : {p.norms, p.splits, p.lows, p.joins, p.count[L_GRAM], p.count[L_POLY], p.count[L_FULL]})
+      EMX_REQUIRE(blocks < (1l << 30), "%s: %ld workgroups", who, blocks);
+    hipLaunchKernelGGL((ns_norm_kernel<T, MUON>), dim3((unsigned)p.norms), dim3(NT), 0, st, ws, t);
     int rc = check_launch(who);
     if (rc) return rc;
-    if (splits) {
-      hipLaunchKernelGGL((ns_split_kernel<T, MUON>), dim3((unsigned)splits), dim3(NT), 0, st, ws, t.n);
+    if (p.splits) {
+      hipLaunchKernelGGL((ns_split_kernel<T, MUON>), dim3((unsigned)p.splits), dim3(NT), 0, st, ws, t.n);
       if ((rc = check_launch(who))) return rc;
     }
-    const auto low = [&](long blocks, int step) {
-      if (blocks == 0) return (int)EMX_OK;
-      hipLaunchKernelGGL((ns_low_kernel<T, MUON>), dim3((unsigned)blocks), dim3(LOW_NT), 2 * LOW_AREA, st, ws, t.n, step);
+    const auto low = [&](int step) {
+      if (p.lows == 0) return (int)EMX_OK;
+      hipLaunchKernelGGL((ns_low_kernel<T, MUON>), dim3((unsigned)p.lows), dim3(LOW_NT), 2 * LOW_AREA, st, ws, t.n, step);
       return check_launch(who);
     };
-    const auto product = [&](auto mid, auto big1, auto big2, int launch, int k) {
-      const long c = count[launch];
-      if (c == 0) return (int)EMX_OK;
+    const auto product = [&](auto kind, int launch, int k) {
+      constexpr int KIND = decltype(kind)::value;
+      const long whole = p.whole[launch], rest = p.count[launch] - whole;
+      const int size = p.size[launch], cuts = p.cuts[launch];
+      if (whole == 0) return (int)EMX_OK;
       // consecutive tiles to an XCD: an eighth of them all, or -- where their lengths differ -- a few in turn, so that each gets long ones
-      const long r = uneven ? 8 : (c + 7) / 8, blocks = (c + 8 * r - 1) / (8 * r) * 8 * r;
-      hipLaunchKernelGGL((size[launch] == 0 ? mid : size[launch] == 1 ? big1 : big2), dim3((unsigned)blocks), dim3(NT), 0, st, ws, t.n, k & 1, (int)c, (int)r);
+      const long run = p.uneven ? 8 : (whole + 7) / 8, blocks = (whole + 8 * run - 1) / (8 * run) * 8 * run;
+      const auto kernel = size == 0 ? ns_mid_kernel<KIND, T, MUON> : size == 1 ? ns_big_kernel<KIND, T, MUON, 1> : ns_big_kernel<KIND, T, MUON, 2>;
+      hipLaunchKernelGGL(kernel, dim3((unsigned)(blocks + rest * cuts)), dim3(NT), 0, st, ws, t.n, k & 1, (int)whole, (int)run, (int)blocks, cuts);
+      const int rc = check_launch(who);
+      if (rc || rest == 0) return rc;
+      hipLaunchKernelGGL((size == 1 ? ns_whole_kernel<KIND, T, MUON, 1> : ns_whole_kernel<KIND, T, MUON, 2>), dim3((unsigned)(rest * BT_C)), dim3(NT), 0, st, ws,
+                         t.n, k & 1, (int)whole, cuts);
       return check_launch(who);
     };
-    if ((rc = low(lows, 0))) return rc;
+    if ((rc = low(0))) return rc;
     for (int k = 0; k < a.steps; ++k) {
-      if ((rc = product(ns_mid_kernel<GRAM, T, MUON>, ns_big_kernel<GRAM, T, MUON, 1>, ns_big_kernel<GRAM, T, MUON, 2>, L_GRAM, k))) return rc;
-      if (joins) {
-        hipLaunchKernelGGL(ns_join_kernel, dim3((unsigned)joins), dim3(NT), 0, st, ws, t.n);
+      if ((rc = product(std::integral_constant<int, GRAM>{}, L_GRAM, k))) return rc;
+      if (p.joins) {
+        hipLaunchKernelGGL(ns_join_kernel, dim3((unsigned)p.joins), dim3(NT), 0, st, ws, t.n);
         if ((rc = check_launch(who))) return rc;
       }
-      if ((rc = product(ns_mid_kernel<POLY, T, MUON>, ns_big_kernel<POLY, T, MUON, 1>, ns_big_kernel<POLY, T, MUON, 2>, L_POLY, k))) return rc;
-      if (k + 1 < a.steps) rc = product(ns_mid_kernel<NEXT, T, MUON>, ns_big_kernel<NEXT, T, MUON, 1>, ns_big_kernel<NEXT, T, MUON, 2>, L_FULL, k);
-      else rc = product(ns_mid_kernel<LAST, T, MUON>, ns_big_kernel<LAST, T, MUON, 1>, ns_big_kernel<LAST, T, MUON, 2>, L_FULL, k);
-      if (rc || (t.a.low_steps && (rc = low(lows, k + 1)))) return rc;
+      if ((rc = product(std::integral_constant<int, POLY>{}, L_POLY, k))) return rc;
+      if (k + 1 < a.steps) rc = product(std::integral_constant<int, NEXT>{}, L_FULL, k);
+      else rc = product(std::integral_constant<int, LAST>{}, L_FULL, k);
+      if (rc || (t.a.low_steps && (rc = low(k + 1)))) return rc;
     }
   }
   return EMX_OK;
@@ -1083,9 +1184,9 @@ size_t ws_bytes_of(const emx_matrix* mats, int n) {   // (groups run one after t
   size_t most = 16;
   for (int i = 0; i < n;) {
     Table t;
-    size_t bytes;
-    i = group(mats, n, i, t, bytes);
-    most = std::max(most, bytes);
+    Plan p;
+    i = plan_group(mats, n, i, t, p);
+    if (t.n) most = std::max(most, p.bytes);
   }
   return most;
 }
