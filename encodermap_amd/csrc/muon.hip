@@ -824,6 +824,140 @@ __device__ __forceinline__ void low_product(f32x16& acc, const char* u, const ch
   }
 }
 
+// ---- ... and of at most 16 rows, in 64 bits: A and P have so few entries that the roundings of split operands do not average out (2 x 128: 2e-6 off
+// where float32 is off by 8e-7), and so few that plain arithmetic costs less than the launch.  The same strips, steps and shares as above; X travels
+// from step to step as float32 rows.
+constexpr int THIN = 16;
+struct Thin {
+  double x[THIN][129];       // (odd pitch: the 16 rows of a column of k lie in different banks)
+  double a[THIN][THIN + 1], p[THIN][THIN + 1];
+  double shares[LOW_NT];
+};
+static_assert(sizeof(Thin) <= 2 * LOW_AREA, "the low kernel's LDS");
+
+template <typename T, bool MUON>
+__device__ void thin_matrix(Thin& l, double* sm, const Mat& m, const Scratch& s, const StepArgs& a, const int wg, const int step) {
+  const int tid = threadIdx.x, M = s.M, wgs = s.low_wgs(), steps = a.steps;
+  const int col = tid & 127, row0 = 2 * (tid >> 7);                    // of X: two rows of a column
+  const long pitch = 32l * s.Nb;
+  int lg = 0;
+  while ((1 << lg) < M) ++lg;
+  const int entries = 1 << (2 * lg), groups = min(LOW_NT / entries, 16);   // of A; of k
+  const int entry = tid & (entries - 1), group = tid >> (2 * lg), ei = entry >> lg, ej = entry & ((1 << lg) - 1);
+  const bool mine = tid < entries && ei < M && ej < M;                 // this thread has an entry of A
+  auto gram = [&]() {                                                  // of the strip in l.x: the entry's sum, in its thread
+    double v = 0.0;
+    if (group < groups && ei < M && ej < M)
+      for (int k = group; k < 128; k += groups) v = fma(l.x[ei][k], l.x[ej][k], v);
+    l.shares[tid] = v;
+    __syncthreads();
+    v = 0.0;
+    if (mine)
+      for (int g = 0; g < groups; ++g) v += l.shares[g * entries + entry];
+    __syncthreads();
+    return v;
+  };
+  auto poly = [&](double entry_of_a) {                                 // leaves P in l.p
+    if (mine) l.a[ei][ej] = entry_of_a;
+    __syncthreads();
+    if (mine) {
+      double v = 0.0;
+      for (int k = 0; k < M; ++k) v = fma(l.a[ei][k], l.a[k][ej], v);
+      l.p[ei][ej] = fma((double)CC, v, (double)CB * entry_of_a);
+    }
+    __syncthreads();
+  };
+  auto next = [&](double (&y)[2]) {                                    // a X + P X, this thread's two
+#pragma unroll
+    for (int r = 0; r < 2; ++r) y[r] = 0.0;
+    if (row0 < M) {
+      for (int k = 0; k < M; ++k) {
+        const double v = l.x[k][col];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) y[r] = fma(row0 + r < M ? l.p[row0 + r][k] : 0.0, v, y[r]);
+      }
+#pragma unroll
+      for (int r = 0; r < 2; ++r)
+        if (row0 + r < M) y[r] = fma((double)CA, l.x[row0 + r][col], y[r]);
+    }
+    __syncthreads();
+  };
+  auto put = [&](const double (&y)[2]) {
+#pragma unroll
+    for (int r = 0; r < 2; ++r) l.x[row0 + r][col] = y[r];
+    __syncthreads();
+  };
+  auto row_of = [&](char* t, int r, int st) { return reinterpret_cast<float*>(t) + (row0 + r) * pitch + 128 * st + col; };
+  auto inside = [&](int r, int st) { return row0 + r < M && 128 * st + col < pitch; };
+  auto write = [&](const double (&y)[2], int st) {
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const int i = row0 + r, j = 128 * st + col;
+      if (i < M && j < s.N) {
+        const long at = m.off + (s.turned ? j * m.ld + i : i * m.ld + j);
+        if constexpr (MUON) a.w[at] = fmaf(a.w[at], a.keep, -(a.lr * m.scale) * (float)y[r]);
+        else ((T*)a.out)[at] = (T)(float)y[r];
+      }
+    }
+  };
+  double y[2], sum = 0.0;
+  if (step == 0) {
+    const double f = scale_of<LOW_NT>(m, s, a.eps, sm) * (double)RSC;
+    for (int st = wg; st < s.strips(); st += wgs) {
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const int i = row0 + r, j = 128 * st + col;
+        y[r] = 0.0;
+        if (i < M && j < s.N) {
+          const long gr = s.turned ? j : i, gc = s.turned ? i : j;
+          y[r] = f * (double)(MUON ? reinterpret_cast<const float*>(s.t1)[gr * m.cols + gc] : (float)((const T*)a.g)[m.off + gr * m.ld + gc]);
+        }
+        if (a.low_steps) {
+          y[r] = (double)(float)y[r];
+          if (inside(r, st)) *row_of(s.t0, r, st) = (float)y[r];
+        }
+      }
+      put(y);
+      sum += gram();
+    }
+    if (a.low_steps) {
+      if (mine) reinterpret_cast<double*>(s.a + (long)wg * 16 * BLK)[entry] = sum;
+      return;
+    }
+    for (int k = 0; k < steps; ++k) {
+      poly(k == 0 ? sum : gram());
+      next(y);
+      put(y);
+    }
+    write(y, 0);
+    return;
+  }
+  char *const shares_in = (step & 1) ? s.a : s.p, *const shares_out = (step & 1) ? s.p : s.a;
+  char *const t_in = (step & 1) ? s.t0 : s.t1, *const t_out = (step & 1) ? s.t1 : s.t0;
+  if (mine)
+    for (int g = 0; g < wgs; ++g) sum += reinterpret_cast<const double*>(shares_in + (long)g * 16 * BLK)[entry];
+  poly(sum);
+  sum = 0.0;
+  for (int st = wg; st < s.strips(); st += wgs) {
+#pragma unroll
+    for (int r = 0; r < 2; ++r) y[r] = inside(r, st) ? (double)*row_of(t_in, r, st) : 0.0;
+    put(y);
+    next(y);
+    if (step == steps) {
+      write(y, st);
+      continue;
+    }
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      y[r] = (double)(float)y[r];
+      if (inside(r, st)) *row_of(t_out, r, st) = (float)y[r];
+    }
+    put(y);
+    sum += gram();
+  }
+  if (step < steps && mine) reinterpret_cast<double*>(shares_out + (long)wg * 16 * BLK)[entry] = sum;
+}
+
 template <typename T, bool MUON>
 __global__ __launch_bounds__(LOW_NT) void ns_low_kernel(char* ws, const int n, const int step /* 0: X_0 and its A (or everything) */) {
   extern __shared__ __align__(16) char lds[];
@@ -838,6 +972,10 @@ __global__ __launch_bounds__(LOW_NT) void ns_low_kernel(char* ws, const int n, c
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lr = lane & 31, h = lane >> 5, ib = wave >> 2, jb = (wave - ib) & 3;
   const int wgs = s.low_wgs(), Mb = s.Mb;
+  if (s.M <= THIN) {
+    thin_matrix<T, MUON>(*reinterpret_cast<Thin*>(lds), sm, m, s, a, wg, step);
+    return;
+  }
   const bool rows = ib < Mb, square = ib <= jb && jb < Mb;   // this wave has a block of X; of the upper half of A and P
   const char *const u1 = area1 + ib * 4 * BLK + lane * 16, *const u2 = area2 + ib * 4 * BLK + lane * 16;
   const char *const v1 = area1 + jb * 4 * BLK + lane * 16, *const v2 = area2 + jb * 4 * BLK + lane * 16;
