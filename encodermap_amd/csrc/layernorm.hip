@@ -363,20 +363,24 @@ __global__ __launch_bounds__(SUM_NT) void ln_sum_kernel(const float* __restrict_
                                                         float* __restrict__ dbeta) {
   __shared__ float sm[32][33];
   const int c = threadIdx.x & 31, w = threadIdx.x >> 5;
-  const long e = (long)blockIdx.x * 32 + c, E = 2l * D;
-  float s = 0.f;
-  if (e < E) {
+  const long E = 2l * D;
+  for (long e0 = (long)blockIdx.x * 32; e0 < E; e0 += (long)gridDim.x * 32) {   // (once, but for rows of more than 2^24 values)
+    const long e = e0 + c;
+    float s = 0.f;
+    if (e < E) {
 #pragma unroll 8
-    for (int p = w; p < n_parts; p += 32) s += part[(long)p * E + e];
-  }
-  sm[w][c] = s;
-  __syncthreads();
-  if (w == 0 && e < E) {
-    float v = 0.f;
+      for (int p = w; p < n_parts; p += 32) s += part[(long)p * E + e];
+    }
+    sm[w][c] = s;
+    __syncthreads();
+    if (w == 0 && e < E) {
+      float v = 0.f;
 #pragma unroll
-    for (int k = 0; k < 32; ++k) v += sm[k][c];
-    float* out = e < D ? dgamma : dbeta;
-    if (out) out[e < D ? e : e - D] = v;
+      for (int k = 0; k < 32; ++k) v += sm[k][c];
+      float* out = e < D ? dgamma : dbeta;
+      if (out) out[e < D ? e : e - D] = v;
+    }
+    if (e0 + (long)gridDim.x * 32 < E) __syncthreads();
   }
 }
 
@@ -409,27 +413,38 @@ int by_type(int dtype, F f) {
   return f(0.f);
 }
 
+// (a launch has fewer than 2^32 threads: 2^31 at most here, the rows behind them in the next one)
 template <typename T, int TPR, int NV, int U>
-void start_fwd(const FwdArgs& a, hipStream_t st) {
+int start_fwd(const char* who, const FwdArgs& all, hipStream_t st) {
   constexpr int NB = TPR > NT ? TPR : NT;
-  const long rows = (long)(NB / TPR) * U;
-  hipLaunchKernelGGL((ln_fwd_kernel<T, TPR, NV, U>), dim3((unsigned)((a.n_rows + rows - 1) / rows)), dim3(NB), 0, st, a);
+  constexpr long rows = (long)(NB / TPR) * U, most = rows * ((1l << 31) / NB);
+  for (long r0 = 0; r0 < all.n_rows; r0 += most) {
+    FwdArgs a = all;
+    a.x = (const T*)all.x + r0 * all.ldx;
+    a.y = (T*)all.y + r0 * all.ldy;
+    a.mean = all.mean ? all.mean + r0 : nullptr;
+    a.rstd = all.rstd ? all.rstd + r0 : nullptr;
+    a.n_rows = std::min(all.n_rows - r0, most);
+    hipLaunchKernelGGL((ln_fwd_kernel<T, TPR, NV, U>), dim3((unsigned)((a.n_rows + rows - 1) / rows)), dim3(NB), 0, st, a);
+    if (const int rc = check_launch(who)) return rc;
+  }
+  return EMX_OK;
 }
 template <typename T>
-void launch_fwd(const FwdArgs& a, hipStream_t st) {
-  int nv = (a.D + Lane<T>::V - 1) / Lane<T>::V;   // 16-byte vectors of a row
-  if (a.n_rows >= (1l << 31)) nv = 1 << 30;   // (more workgroups than a launch has: the form whose workgroups walk)
-  if (nv <= 8) return start_fwd<T, 8, 1, 4>(a, st);
-  if (nv <= 16) return start_fwd<T, 16, 1, 4>(a, st);
-  if (nv <= 32) return start_fwd<T, 32, 1, 4>(a, st);
-  if (nv <= 64) return start_fwd<T, 64, 1, 4>(a, st);
-  if (nv <= 128) return start_fwd<T, 64, 2, 2>(a, st);
-  if (nv <= 256) return start_fwd<T, 64, 4, 1>(a, st);
-  if (nv <= 512) return start_fwd<T, 256, 2, 1>(a, st);
-  if (nv <= 1024) return start_fwd<T, 256, 4, 1>(a, st);
-  if (nv <= 2048) return start_fwd<T, 1024, 2, 1>(a, st);
-  if (nv <= 4096) return start_fwd<T, 1024, 4, 1>(a, st);
+int launch_fwd(const char* who, const FwdArgs& a, hipStream_t st) {
+  const int nv = (a.D + Lane<T>::V - 1) / Lane<T>::V;   // 16-byte vectors of a row
+  if (nv <= 8) return start_fwd<T, 8, 1, 4>(who, a, st);
+  if (nv <= 16) return start_fwd<T, 16, 1, 4>(who, a, st);
+  if (nv <= 32) return start_fwd<T, 32, 1, 4>(who, a, st);
+  if (nv <= 64) return start_fwd<T, 64, 1, 4>(who, a, st);
+  if (nv <= 128) return start_fwd<T, 64, 2, 2>(who, a, st);
+  if (nv <= 256) return start_fwd<T, 64, 4, 1>(who, a, st);
+  if (nv <= 512) return start_fwd<T, 256, 2, 1>(who, a, st);
+  if (nv <= 1024) return start_fwd<T, 256, 4, 1>(who, a, st);
+  if (nv <= 2048) return start_fwd<T, 1024, 2, 1>(who, a, st);
+  if (nv <= 4096) return start_fwd<T, 1024, 4, 1>(who, a, st);
   hipLaunchKernelGGL(ln_fwd_long_kernel<T>, dim3((unsigned)std::min<long>(a.n_rows, 1 << 20)), dim3(NT), 0, st, a);
+  return check_launch(who);
 }
 template <typename T, int TPR, int NV>
 bool start_bwd(const BwdArgs& a, hipStream_t st) {
@@ -469,8 +484,7 @@ int emx_layernorm_fwd(const void* x, int dtype, int64_t n_rows, int D, int64_t l
   EMX_REQUIRE(disjoint_or_same(x, ldx, y, ldy, n_rows, D, size_of(dtype)), "%s: x and y overlap without being the same rows", who);
   const FwdArgs a{x, y, gamma, beta, mean, rstd, n_rows, ldx, ldy, D, eps};
   return by_type(dtype, [&](auto t) {
-    launch_fwd<decltype(t)>(a, (hipStream_t)stream);
-    return check_launch(who);
+    return launch_fwd<decltype(t)>(who, a, (hipStream_t)stream);
   });
 }
 
@@ -515,7 +529,7 @@ int emx_layernorm_bwd(const void* dy, int64_t ld_dy, const void* x, int64_t ldx,
     if (rc) return rc;
   }
   if (!sums) return EMX_OK;
-  hipLaunchKernelGGL(ln_sum_kernel, dim3((unsigned)((2l * D + 31) / 32)), dim3(SUM_NT), 0, st, ws, parts, D, dgamma, dbeta);
+  hipLaunchKernelGGL(ln_sum_kernel, dim3((unsigned)std::min((2l * D + 31) / 32, 1l << 20)), dim3(SUM_NT), 0, st, ws, parts, D, dgamma, dbeta);
   return check_launch(who);
 }
 

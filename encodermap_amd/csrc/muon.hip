@@ -1274,7 +1274,7 @@ int run(const char* who, const emx_matrix* mats, int n, const StepArgs& a, char*
     i = plan_group(mats, n, i, t, p);
     if (t.n == 0) break;
     for (const long blocks : {p.norms, p.splits, p.lows, p.joins, p.count[L_GRAM], p.count[L_POLY], p.count[L_FULL]})
-      EMX_REQUIRE(blocks < (1l << 30), "%s: %ld workgroups", who, blocks);
+      EMX_REQUIRE(blocks < (1l << 24), "%s: %ld workgroups", who, blocks);
     hipLaunchKernelGGL((ns_norm_kernel<T, MUON>), dim3((unsigned)p.norms), dim3(NT), 0, st, ws, t);
     int rc = check_launch(who);
     if (rc) return rc;
