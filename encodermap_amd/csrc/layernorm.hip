@@ -4,9 +4,10 @@
 //   backward   h_j = (x_j - mu) r,  t_j = dy_j gamma_j,  dx_j = r (t_j - 1/D sum_k t_k - h_j 1/D sum_k t_k h_k)
 //              dgamma_j = sum_rows dy_j h_j,  dbeta_j = sum_rows dy_j
 //
-// All arithmetic is float32 whatever the rows' type (f16 / bf16 rows are rounded once, when they are stored); the centred sum of
-// squares is taken after the mean, not as a difference of two large sums.  Sums over rows are two-pass in a fixed order: n_parts
-// partial sums of consecutive rows in the caller's workspace, then one sum over the parts.
+// All arithmetic is float32 whatever the rows' type (f16 / bf16 rows are rounded once, when they are stored), but for the sums of rows too long
+// for the registers, which are taken in 64 bits; the centred sum of squares is taken after the mean, not as a difference of two large
+// sums.  Sums over rows are two-pass in a fixed order: n_parts partial sums of consecutive rows in the caller's workspace, then one sum
+// over the parts.
 #include <algorithm>
 #include <cstdint>
 
@@ -62,10 +63,18 @@ __device__ __forceinline__ float row_sum(float v, float* area) {
   for (int i = 0; i < TPR / 64; ++i) s += area[i];
   return s;
 }
+// the sum over a workgroup, in each of its threads, in 64 bits
 template <int N>
-__device__ __forceinline__ float block_all_sum(float v, float* smem /* N / 64 floats */) {
+__device__ __forceinline__ double block_sum64(double v, double* area /* N / 64 */) {
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) v += __shfl_xor(v, d);
   __syncthreads();   // (the area may still be read from the sum before)
-  return row_sum<N>(v, smem);
+  if ((threadIdx.x & 63) == 0) area[threadIdx.x >> 6] = v;
+  __syncthreads();
+  double s = 0.0;
+#pragma unroll
+  for (int i = 0; i < N / 64; ++i) s += area[i];
+  return s;
 }
 
 // 16 bytes of a row; the address is a multiple of the element's size only
@@ -290,23 +299,24 @@ __global__ __launch_bounds__(TPR > NT ? TPR : NT) void ln_bwd_kernel(const BwdAr
   }
 }
 
-// ---- rows of any length: one workgroup per row, the row is walked once per sum
+// ---- rows of any length: one workgroup per row, the row is walked once per sum.  A thread adds up to 2^20 values of its own: in 64 bits (in 32
+// the roundings of equal terms all go one way: 2^20 times 1.1 comes out 1 % off)
 template <typename T>
 __global__ __launch_bounds__(NT) void ln_fwd_long_kernel(const FwdArgs a) {
-  __shared__ float sm[NT / 64];
-  const float inv = 1.f / (float)a.D;
+  __shared__ double sm[NT / 64];
+  const double inv = 1.0 / (double)a.D;
   for (long r = blockIdx.x; r < a.n_rows; r += gridDim.x) {
     const T* x = (const T*)a.x + r * a.ldx;
     T* y = (T*)a.y + r * a.ldy;
-    float s = 0.f;
-    for (int j = threadIdx.x; j < a.D; j += NT) s += (float)x[j];
-    const float mu = block_all_sum<NT>(s, sm) * inv;
-    s = 0.f;
+    double s = 0.0;
+    for (int j = threadIdx.x; j < a.D; j += NT) s += (double)(float)x[j];
+    const float mu = (float)(block_sum64<NT>(s, sm) * inv);
+    s = 0.0;
     for (int j = threadIdx.x; j < a.D; j += NT) {
       const float c = (float)x[j] - mu;
-      s = fmaf(c, c, s);
+      s = fma((double)c, (double)c, s);
     }
-    const float rs = 1.f / sqrtf(fmaf(block_all_sum<NT>(s, sm), inv, a.eps));
+    const float rs = (float)(1.0 / sqrt(fma(block_sum64<NT>(s, sm), inv, (double)a.eps)));
     for (int j = threadIdx.x; j < a.D; j += NT)
       y[j] = (T)fmaf(((float)x[j] - mu) * rs, a.gamma ? a.gamma[j] : 1.f, a.beta ? a.beta[j] : 0.f);
     if (threadIdx.x == 0) {
@@ -318,21 +328,20 @@ __global__ __launch_bounds__(NT) void ln_fwd_long_kernel(const FwdArgs a) {
 
 template <typename T>
 __global__ __launch_bounds__(NT) void ln_bwd_long_kernel(const BwdArgs a) {
-  __shared__ float sm[NT / 64];
-  const float inv = 1.f / (float)a.D;
+  __shared__ double sm[NT / 64];
+  const double inv = 1.0 / (double)a.D;
   for (long r = blockIdx.x; r < a.n_rows; r += gridDim.x) {
     const T* x = (const T*)a.x + r * a.ldx;
     const T* dy = (const T*)a.dy + r * a.ld_dy;
     T* dx = (T*)a.dx + r * a.ld_dx;
     const float mu = a.mean[r], rs = a.rstd[r];
-    float s = 0.f, q = 0.f;
+    double s64 = 0.0, q64 = 0.0;
     for (int j = threadIdx.x; j < a.D; j += NT) {
       const float t = (float)dy[j] * (a.gamma ? a.gamma[j] : 1.f);
-      s += t;
-      q = fmaf(t, ((float)x[j] - mu) * rs, q);
+      s64 += (double)t;
+      q64 = fma((double)t, (double)(((float)x[j] - mu) * rs), q64);
     }
-    s = block_all_sum<NT>(s, sm) * inv;
-    q = block_all_sum<NT>(q, sm) * inv;
+    const float s = (float)(block_sum64<NT>(s64, sm) * inv), q = (float)(block_sum64<NT>(q64, sm) * inv);
     for (int j = threadIdx.x; j < a.D; j += NT) {
       const float t = (float)dy[j] * (a.gamma ? a.gamma[j] : 1.f), h = ((float)x[j] - mu) * rs;
       dx[j] = (T)(rs * (t - fmaf(h, q, s)));

@@ -29,6 +29,10 @@ def room(request):
     torch.cuda.empty_cache()
 
 
+def test_rows_of_2_27_values(lib):
+    ln.run_backward(lib, 2, 2 ** 27 + 5, "f16", pad=0, offset=3.0)
+
+
 def test_more_rows_than_a_launch_has_threads_for(lib):
     """1024 threads to a row: 2^22 rows are 2^32 threads"""
     n, D, eps = 2 ** 22 + 3, 8200, 1e-3
