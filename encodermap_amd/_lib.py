@@ -817,7 +817,8 @@ def mlp_wgrad_adam_local(plan: MlpPlan, row_begin, row_end, ws, finish: "FinishD
                                            _stream()), "emx_mlp_wgrad_adam_local")
 
 
-# ---- ADC path ---------------------------------------------------------------------------------------------------
+# ---- layer norm, orthogonalised updates ---------------------------------------------------------------------------
+_LAYERNORM_MAX_D = 1 << 28     # EMX_LAYERNORM_MAX_D
 _ELEMENT_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}   # EMX_F32, EMX_F16, EMX_BF16
 
 
@@ -843,6 +844,8 @@ def _rows(t, ref, what) -> int:
     stride, col = t.stride()
     if col != 1 and t.shape[1] > 1:
         raise EmxError(f"{what}: the columns of a row have to lie side by side, got strides {t.stride()}")
+    if t.shape[1] > _LAYERNORM_MAX_D:    # (ctypes cuts an int to 32 bits)
+        raise EmxError(f"{what}: rows of {t.shape[1]} values, {_LAYERNORM_MAX_D} at most")
     return stride
 
 
@@ -881,6 +884,8 @@ def layernorm_fwd(x, gamma, beta, eps, y, mean=None, rstd=None):
 
 
 def layernorm_ws_floats(n_rows, D) -> int:
+    if not (0 <= n_rows < 2 ** 63 and 1 <= D <= _LAYERNORM_MAX_D):
+        raise EmxError(f"layernorm_ws_floats: {n_rows} rows of {D} values (at most {_LAYERNORM_MAX_D})")
     return int(load().emx_layernorm_ws_floats(int(n_rows), int(D)))
 
 
@@ -944,13 +949,20 @@ class MatrixPlan:
         return t.data_ptr()
 
 
+def _int32(value, what) -> int:
+    value = int(value)
+    if not -2 ** 31 <= value < 2 ** 31:    # (ctypes cuts it)
+        raise EmxError(f"{what} {value}")
+    return value
+
+
 def orthogonalize(plan: MatrixPlan, g, out, steps: int = 5, eps: float = 1e-7):
     """The matrices of ``out`` <- those of ``g`` orthogonalised (include/emx.h: emx_orthogonalize); flat buffers of one type (float32 / float16 /
     bfloat16) and any shape; ``out`` may be ``g``."""
     code = _element_type(g, "g")
     if out.dtype != g.dtype:
         raise EmxError(f"out: {g.dtype} like g expected, got {out.dtype}")
-    _on_device(plan.ws.get_device(), load().emx_orthogonalize, "emx_orthogonalize", *plan._args, plan._flat(g, "g"), plan._flat(out, "out"), code, int(steps),
+    _on_device(plan.ws.get_device(), load().emx_orthogonalize, "emx_orthogonalize", *plan._args, plan._flat(g, "g"), plan._flat(out, "out"), code, _int32(steps, "steps"),
                float(eps), *plan._ws_args)
 
 
@@ -964,11 +976,12 @@ def muon_step(plan: MatrixPlan, w, g, momentum_buffer, lr, momentum: float = 0.9
     slices, stride = g.shape if g.dim() == 2 else (1, 0)
     if slices > 1 and stride < plan.end:
         raise EmxError(f"g: slices of {stride} elements, the matrices reach to {plan.end}")
-    _on_device(plan.ws.get_device(), load().emx_muon_step, "emx_muon_step", *plan._args, plan._flat(w, "w"), plan._flat(g, "g", slices, stride), slices, stride,
-               plan._flat(momentum_buffer, "momentum_buffer"), float(lr), float(momentum), int(bool(nesterov)), float(weight_decay), int(steps), float(eps),
+    _on_device(plan.ws.get_device(), load().emx_muon_step, "emx_muon_step", *plan._args, plan._flat(w, "w"), plan._flat(g, "g", slices, stride), _int32(slices, "slices"), stride,
+               plan._flat(momentum_buffer, "momentum_buffer"), float(lr), float(momentum), int(bool(nesterov)), float(weight_decay), _int32(steps, "steps"), float(eps),
                *plan._ws_args)
 
 
+# ---- ADC path ---------------------------------------------------------------------------------------------------
 def colmean(x, out):
     B, n = x.shape
     _check(load().emx_colmean(_ptr(x), B, n, x.stride(0), _ptr(out), _stream()), "emx_colmean")

@@ -375,12 +375,12 @@ __global__ __launch_bounds__(SUM_NT) void ln_sum_kernel(const float* __restrict_
   const long E = 2l * D;
   for (long e0 = (long)blockIdx.x * 32; e0 < E; e0 += (long)gridDim.x * 32) {   // (once, but for rows of more than 2^24 values)
     const long e = e0 + c;
-    float s = 0.f;
+    double s = 0.0;   // (up to 2048 parts)
     if (e < E) {
 #pragma unroll 8
-      for (int p = w; p < n_parts; p += 32) s += part[(long)p * E + e];
+      for (int p = w; p < n_parts; p += 32) s += (double)part[(long)p * E + e];
     }
-    sm[w][c] = s;
+    sm[w][c] = (float)s;
     __syncthreads();
     if (w == 0 && e < E) {
       float v = 0.f;
@@ -393,11 +393,12 @@ __global__ __launch_bounds__(SUM_NT) void ln_sum_kernel(const float* __restrict_
   }
 }
 
-// The parts of a backward pass: consecutive rows each.
+// The parts of a backward pass: consecutive rows each, at most 512 of them while a launch's second dimension (65535) allows it -- a thread adds
+// a part's rows one after the other in 32 bits.
 int parts_of(long n_rows, int D) {
   if (n_rows <= 0) return 0;
   const long cap = std::min(1024l, std::max(32l, (4l << 20) / D));
-  return (int)std::min((n_rows + 7) / 8, cap);
+  return (int)std::min((n_rows + 7) / 8, std::max(cap, std::min((n_rows + 511) / 512, 65535l)));
 }
 
 bool known_type(int dtype) { return dtype == EMX_F32 || dtype == EMX_F16 || dtype == EMX_BF16; }
@@ -487,6 +488,7 @@ int emx_layernorm_fwd(const void* x, int dtype, int64_t n_rows, int D, int64_t l
   EMX_REQUIRE(n_rows >= 0 && D >= 1 && D <= EMX_LAYERNORM_MAX_D, "%s: n_rows %lld, D %d", who, (long long)n_rows, D);
   EMX_REQUIRE(eps >= 0.f, "%s: eps %g", who, (double)eps);   // (refuses NaN)
   if (n_rows == 0) return EMX_OK;
+  EMX_REQUIRE(!mean || mean != rstd, "%s: mean and rstd are the same vector", who);
   EMX_REQUIRE(x && y && aligned(x, size_of(dtype)) && aligned(y, size_of(dtype)), "%s: x and y are needed, on element boundaries", who);
   EMX_REQUIRE(n_rows == 1 || (fits(n_rows, ldx) && fits(n_rows, ldy) && ldy >= D), "%s: row strides %lld, %lld of %d columns", who, (long long)ldx, (long long)ldy, D);
   if (n_rows == 1) ldx = ldy = D;
@@ -518,6 +520,7 @@ int emx_layernorm_bwd(const void* dy, int64_t ld_dy, const void* x, int64_t ldx,
   const int parts = parts_of(n_rows, D);
   if (sums && parts > 0 && (!ws || ws_floats < emx_layernorm_ws_floats(n_rows, D)))
     return fail(EMX_EWORKSPACE, "%s: workspace of %zu floats, %zu needed", who, ws ? ws_floats : (size_t)0, emx_layernorm_ws_floats(n_rows, D));
+  EMX_REQUIRE(!dgamma || dgamma != dbeta, "%s: dgamma and dbeta are the same vector", who);
   hipStream_t st = (hipStream_t)stream;
   if (n_rows > 0) {
     const BwdArgs a{dy, x, dx, gamma, mean, rstd, sums ? ws : nullptr, n_rows, ld_dy, ldx, ld_dx, (n_rows + parts - 1) / parts, D, parts};

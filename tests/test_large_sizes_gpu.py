@@ -56,6 +56,22 @@ def test_more_rows_than_a_launch_has_threads_for(lib):
         assert (x[r:r + 2 ** 17].float().square().mean(1) - 1).abs().max().item() < 0.02     # (eps and the rounding to 8 bits: 0.001 + 2 x 2^-9)
 
 
+def test_columns_of_2_27_rows(lib):
+    """equal terms are the worst that a long sum can be given: their roundings all go one way"""
+    n, D = 2 ** 27, 2
+    gen = torch.Generator("cuda").manual_seed(1)
+    x = torch.randn(n, D, generator=gen, device="cuda")
+    mean, rstd = torch.zeros(n, device="cuda"), torch.ones(n, device="cuda")
+    dy = torch.full((1, D), 1.1, device="cuda")
+    dg, db = torch.empty(D, device="cuda"), torch.empty(D, device="cuda")
+    ws = torch.empty(lib.layernorm_ws_floats(n, D), device="cuda")
+    lib.layernorm_bwd(dy.expand(n, D), x, None, mean, rstd, None, dg, db, ws)
+    one = dy[0].double()
+    ln.check(db, n * one, 500 * ln.U * n * one, "dbeta")
+    k = 6.0     # (the largest |x| of 2^28 normal ones)
+    ln.check(dg, one * x.sum(0, dtype=torch.float64), 500 * ln.U * one * x.abs().sum(0, dtype=torch.float64) + (200 + 100 * k) * ln.U * (1 + k) * n * one, "dgamma")
+
+
 def test_the_largest_matrix(lib):
     """G = (H x 1) diag(B_0 .. B_127): H the 128 x 128 matrix of signs whose rows are orthogonal, so that G has no zeros, orth(G) is
     (H / sqrt(128) x 1) diag(f(B_j)), and the formula is one of 256 x 256 matrices"""
@@ -90,3 +106,18 @@ def test_the_largest_matrix(lib):
     assert torch.isfinite(off) and (out[side * side:] == 7.0).all()
     limit = om.bound(side, side, steps)
     assert off.sqrt().item() <= limit, f"{off.sqrt().item():.3g} off, {limit:.3g} allowed of {f.norm().item():.3g}"
+
+
+def test_what_an_int_does_not_hold_is_refused(lib):
+    x = torch.empty(1, 2 ** 32 + 8, dtype=torch.float16, device="cuda")
+    with pytest.raises(lib.EmxError, match="values"):
+        lib.layernorm_fwd(x, None, None, 1e-3, x)
+    g = torch.zeros(64, device="cuda")
+    plan = lib.MatrixPlan([(0, 8, 8, 8, 1.0)])
+    with pytest.raises(lib.EmxError, match="steps"):
+        lib.orthogonalize(plan, g, g, steps=2 ** 32 + 5)
+    with pytest.raises(lib.EmxError, match="steps"):
+        lib.muon_step(plan, g.clone(), g, g.clone(), lr=0.1, steps=2 ** 32 + 5)
+    parts = torch.zeros(2 ** 31, 1, device="cuda")
+    with pytest.raises(lib.EmxError, match="slices"):
+        lib.muon_step(lib.MatrixPlan([(0, 1, 1, 1, 1.0)]), g.clone(), parts, g.clone(), lr=0.1)
