@@ -844,8 +844,6 @@ def _rows(t, ref, what) -> int:
     stride, col = t.stride()
     if col != 1 and t.shape[1] > 1:
         raise EmxError(f"{what}: the columns of a row have to lie side by side, got strides {t.stride()}")
-    if t.shape[1] > _LAYERNORM_MAX_D:    # (ctypes cuts an int to 32 bits)
-        raise EmxError(f"{what}: rows of {t.shape[1]} values, {_LAYERNORM_MAX_D} at most")
     return stride
 
 
@@ -879,6 +877,8 @@ def layernorm_fwd(x, gamma, beta, eps, y, mean=None, rstd=None):
     code = _element_type(x, "x")
     ldx, ldy = _rows(x, x, "x"), _rows(y, x, "y")
     n, D = x.shape
+    if D > _LAYERNORM_MAX_D:    # (ctypes cuts an int to 32 bits)
+        raise EmxError(f"x: rows of {D} values, {_LAYERNORM_MAX_D} at most")
     _on_device(x.get_device(), load().emx_layernorm_fwd, "emx_layernorm_fwd", x.data_ptr(), code, n, D, ldx, _vector(gamma, D, x, "gamma"),
                _vector(beta, D, x, "beta"), float(eps), y.data_ptr(), ldy, _vector(mean, n, x, "mean"), _vector(rstd, n, x, "rstd"))
 
@@ -896,6 +896,8 @@ def layernorm_bwd(dy, x, gamma, mean, rstd, dx, dgamma, dbeta, ws=None):
     ldx, ld_dy = _rows(x, x, "x"), _rows(dy, x, "dy")
     ld_dx = _rows(dx, x, "dx") if dx is not None else 0
     n, D = x.shape
+    if D > _LAYERNORM_MAX_D:
+        raise EmxError(f"x: rows of {D} values, {_LAYERNORM_MAX_D} at most")
     if ws is not None:
         _vector(ws, ws.numel(), x, "ws")
     _on_device(x.get_device(), load().emx_layernorm_bwd, "emx_layernorm_bwd", dy.data_ptr(), ld_dy, x.data_ptr(), ldx, code, n, D,

@@ -299,26 +299,77 @@ __global__ __launch_bounds__(TPR > NT ? TPR : NT) void ln_bwd_kernel(const BwdAr
   }
 }
 
-// ---- rows of any length: one workgroup per row, the row is walked once per sum.  A thread adds up to 2^20 values of its own: in 64 bits (in 32
-// the roundings of equal terms all go one way: 2^20 times 1.1 comes out 1 % off)
+// ---- rows of any length: one workgroup per row walks it once per sum, four vectors of each thread on their way at a time.  A vector's values are
+// added in 32 bits, the vectors of a thread -- up to 2^16 of them -- in 64 (in 32 the roundings of equal terms all go one way: 2^20 times
+// 1.1 comes out 1 % off).
+constexpr int LONG_NT = 1024, LONG_U = 4;
+template <typename T, typename F>
+__device__ __forceinline__ void walk(const T* x, int D, F take /* (vector, its first column, elements of the row from there on) */) {
+  constexpr int V = Lane<T>::V, step = LONG_NT * V;
+  for (int c0 = threadIdx.x * V; c0 < D; c0 += LONG_U * step) {
+    typename Lane<T>::vec raw[LONG_U];
+#pragma unroll
+    for (int u = 0; u < LONG_U; ++u)
+      if (c0 + u * step < D) raw[u] = Lane<T>::load(x + c0 + u * step, D - (c0 + u * step));
+#pragma unroll
+    for (int u = 0; u < LONG_U; ++u)
+      if (c0 + u * step < D) take(raw[u], c0 + u * step, D - (c0 + u * step));
+  }
+}
+template <typename T, typename F>
+__device__ __forceinline__ void walk_two(const T* x, const T* dy, int D, F take) {
+  constexpr int V = Lane<T>::V, step = LONG_NT * V;
+  for (int c0 = threadIdx.x * V; c0 < D; c0 += LONG_U * step) {
+    typename Lane<T>::vec rx[LONG_U], rd[LONG_U];
+#pragma unroll
+    for (int u = 0; u < LONG_U; ++u)
+      if (c0 + u * step < D) {
+        rx[u] = Lane<T>::load(x + c0 + u * step, D - (c0 + u * step));
+        rd[u] = Lane<T>::load(dy + c0 + u * step, D - (c0 + u * step));
+      }
+#pragma unroll
+    for (int u = 0; u < LONG_U; ++u)
+      if (c0 + u * step < D) take(rx[u], rd[u], c0 + u * step, D - (c0 + u * step));
+  }
+}
+
 template <typename T>
-__global__ __launch_bounds__(NT) void ln_fwd_long_kernel(const FwdArgs a) {
-  __shared__ double sm[NT / 64];
+__global__ __launch_bounds__(LONG_NT) void ln_fwd_long_kernel(const FwdArgs a) {
+  constexpr int V = Lane<T>::V;
+  typedef typename Lane<T>::vec vec;
+  __shared__ double sm[LONG_NT / 64];
   const double inv = 1.0 / (double)a.D;
   for (long r = blockIdx.x; r < a.n_rows; r += gridDim.x) {
     const T* x = (const T*)a.x + r * a.ldx;
     T* y = (T*)a.y + r * a.ldy;
     double s = 0.0;
-    for (int j = threadIdx.x; j < a.D; j += NT) s += (double)(float)x[j];
-    const float mu = (float)(block_sum64<NT>(s, sm) * inv);
+    walk<T>(x, a.D, [&](const vec v, int, int left) __attribute__((always_inline)) {
+      float p = 0.f;
+#pragma unroll
+      for (int e = 0; e < V; ++e) p += e < left ? (float)v[e] : 0.f;
+      s += (double)p;
+    });
+    const float mu = (float)(block_sum64<LONG_NT>(s, sm) * inv);
     s = 0.0;
-    for (int j = threadIdx.x; j < a.D; j += NT) {
-      const float c = (float)x[j] - mu;
-      s = fma((double)c, (double)c, s);
-    }
-    const float rs = (float)(1.0 / sqrt(fma(block_sum64<NT>(s, sm), inv, (double)a.eps)));
-    for (int j = threadIdx.x; j < a.D; j += NT)
-      y[j] = (T)fmaf(((float)x[j] - mu) * rs, a.gamma ? a.gamma[j] : 1.f, a.beta ? a.beta[j] : 0.f);
+    walk<T>(x, a.D, [&](const vec v, int, int left) __attribute__((always_inline)) {
+      float p = 0.f;
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const float c = (float)v[e] - mu;
+        p = e < left ? fmaf(c, c, p) : p;
+      }
+      s += (double)p;
+    });
+    const float rs = (float)(1.0 / sqrt(fma(block_sum64<LONG_NT>(s, sm), inv, (double)a.eps)));
+    walk<T>(x, a.D, [&](const vec v, int col, int left) __attribute__((always_inline)) {
+      float ga[V], be[V];
+      load_weights<V>(a.gamma, 1.f, col, a.D, ga);
+      load_weights<V>(a.beta, 0.f, col, a.D, be);
+      vec o;
+#pragma unroll
+      for (int e = 0; e < V; ++e) o[e] = (T)fmaf(((float)v[e] - mu) * rs, ga[e], be[e]);
+      Lane<T>::store(y + col, o, left);
+    });
     if (threadIdx.x == 0) {
       if (a.mean) a.mean[r] = mu;
       if (a.rstd) a.rstd[r] = rs;
@@ -327,8 +378,10 @@ __global__ __launch_bounds__(NT) void ln_fwd_long_kernel(const FwdArgs a) {
 }
 
 template <typename T>
-__global__ __launch_bounds__(NT) void ln_bwd_long_kernel(const BwdArgs a) {
-  __shared__ double sm[NT / 64];
+__global__ __launch_bounds__(LONG_NT) void ln_bwd_long_kernel(const BwdArgs a) {
+  constexpr int V = Lane<T>::V;
+  typedef typename Lane<T>::vec vec;
+  __shared__ double sm[LONG_NT / 64];
   const double inv = 1.0 / (double)a.D;
   for (long r = blockIdx.x; r < a.n_rows; r += gridDim.x) {
     const T* x = (const T*)a.x + r * a.ldx;
@@ -336,16 +389,30 @@ __global__ __launch_bounds__(NT) void ln_bwd_long_kernel(const BwdArgs a) {
     T* dx = (T*)a.dx + r * a.ld_dx;
     const float mu = a.mean[r], rs = a.rstd[r];
     double s64 = 0.0, q64 = 0.0;
-    for (int j = threadIdx.x; j < a.D; j += NT) {
-      const float t = (float)dy[j] * (a.gamma ? a.gamma[j] : 1.f);
-      s64 += (double)t;
-      q64 = fma((double)t, (double)(((float)x[j] - mu) * rs), q64);
-    }
-    const float s = (float)(block_sum64<NT>(s64, sm) * inv), q = (float)(block_sum64<NT>(q64, sm) * inv);
-    for (int j = threadIdx.x; j < a.D; j += NT) {
-      const float t = (float)dy[j] * (a.gamma ? a.gamma[j] : 1.f), h = ((float)x[j] - mu) * rs;
-      dx[j] = (T)(rs * (t - fmaf(h, q, s)));
-    }
+    walk_two<T>(x, dy, a.D, [&](const vec v, const vec d, int col, int left) __attribute__((always_inline)) {
+      float ga[V], p = 0.f, q = 0.f;
+      load_weights<V>(a.gamma, 1.f, col, a.D, ga);
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const float t = e < left ? (float)d[e] * ga[e] : 0.f, h = e < left ? ((float)v[e] - mu) * rs : 0.f;
+        p += t;
+        q = fmaf(t, h, q);
+      }
+      s64 += (double)p;
+      q64 += (double)q;
+    });
+    const float s = (float)(block_sum64<LONG_NT>(s64, sm) * inv), q = (float)(block_sum64<LONG_NT>(q64, sm) * inv);
+    walk_two<T>(x, dy, a.D, [&](const vec v, const vec d, int col, int left) __attribute__((always_inline)) {
+      float ga[V];
+      load_weights<V>(a.gamma, 1.f, col, a.D, ga);
+      vec o;
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const float h = ((float)v[e] - mu) * rs;
+        o[e] = (T)(rs * ((float)d[e] * ga[e] - fmaf(h, q, s)));
+      }
+      Lane<T>::store(dx + col, o, left);
+    });
   }
 }
 
@@ -453,7 +520,7 @@ int launch_fwd(const char* who, const FwdArgs& a, hipStream_t st) {
   if (nv <= 1024) return start_fwd<T, 256, 4, 1>(who, a, st);
   if (nv <= 2048) return start_fwd<T, 1024, 2, 1>(who, a, st);
   if (nv <= 4096) return start_fwd<T, 1024, 4, 1>(who, a, st);
-  hipLaunchKernelGGL(ln_fwd_long_kernel<T>, dim3((unsigned)std::min<long>(a.n_rows, 1 << 20)), dim3(NT), 0, st, a);
+  hipLaunchKernelGGL(ln_fwd_long_kernel<T>, dim3((unsigned)std::min<long>(a.n_rows, 1 << 20)), dim3(LONG_NT), 0, st, a);
   return check_launch(who);
 }
 template <typename T, int TPR, int NV>
@@ -533,7 +600,7 @@ int emx_layernorm_bwd(const void* dy, int64_t ld_dy, const void* x, int64_t ldx,
         if (r) return r;
       }
       if (dx) {
-        hipLaunchKernelGGL(ln_bwd_long_kernel<T>, dim3((unsigned)std::min<int64_t>(n_rows, 1 << 20)), dim3(NT), 0, st, a);
+        hipLaunchKernelGGL(ln_bwd_long_kernel<T>, dim3((unsigned)std::min<int64_t>(n_rows, 1 << 20)), dim3(LONG_NT), 0, st, a);
         return check_launch(who);
       }
       return (int)EMX_OK;

@@ -581,7 +581,7 @@ int emx_mlp_wgrad_adam_local(const emx_mlp_desc* desc, float* params, int64_t n_
  *   y may be x, dx may be dy or x (same pointer, same stride); any other overlap of their address ranges is refused.  mean and rstd,
  *   dgamma and dbeta are two vectors each.
  *   A row with an infinity or a NaN gives NaN in its own results (and in dgamma / dbeta); eps = 0 gives NaN for a constant row.  Sums are
- *   float32 (64 bits for rows of more than 64 KB, dx: 32 KB): a row that leaves its mean by more than 1e19 overflows its sum of squares
+ *   float32 at least: a row that leaves its mean by more than 1e19 overflows its sum of squares
  *   (rstd = 0), one whose sum passes float32's range gives infinities and NaN.
  *   ws: emx_layernorm_ws_floats(n_rows, D) floats of scratch (may be NULL where dgamma and dbeta are); its contents mean nothing
  *   between calls, calls that may run at the same time need one each.
