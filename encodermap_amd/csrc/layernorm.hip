@@ -117,7 +117,8 @@ __device__ __forceinline__ void load_weights(const float* w, float other, int co
 }
 
 // ---- rows that fit into registers: TPR threads hold a row, thread t its vectors t, t + TPR, ... (NV of them); each thread works on U
-// rows at a time, whose loads are all requested before the first is used
+// rows at a time, whose loads are all requested before the first is used.  Bound by HBM: 1e6 x 128 f32 181 us = 5.7 TB/s (a workgroup per
+// row with its sums through LDS: 969); 10007 x 1001 bf16 11.9 us = 3.7 TB/s, the start and end of so short a launch; 256 x 128 3.7 us, a launch.
 template <typename T, int TPR, int NV, int U>
 __global__ __launch_bounds__(TPR > NT ? TPR : NT) void ln_fwd_kernel(const FwdArgs a) {
   constexpr int V = Lane<T>::V, G = (TPR > NT ? TPR : NT) / TPR;
@@ -194,6 +195,8 @@ __global__ __launch_bounds__(TPR > NT ? TPR : NT) void ln_fwd_kernel(const FwdAr
 
 // ---- backward, rows that fit into registers: workgroup p walks the rows of part p, G at a time, TPR threads to a row; a thread keeps the
 // sums of ITS columns over the part's rows, the G groups' are added through LDS at the end.  The next rows' loads travel under this row's sums.
+// Bound by HBM: 65536 x 1024 bf16 87 us = 4.6 TB/s, 2047 x 2850 f32 18.3 us = 3.8 TB/s -- where twice and half the threads, vectors or parts are
+// all within 5 %; 4096 x 128 f32 3.8 us.
 template <typename T, int TPR, int NV>
 __global__ __launch_bounds__(TPR > NT ? TPR : NT) void ln_bwd_kernel(const BwdArgs a) {
   constexpr int V = Lane<T>::V, NB = TPR > NT ? TPR : NT, G = NB / TPR;
@@ -301,7 +304,8 @@ __global__ __launch_bounds__(TPR > NT ? TPR : NT) void ln_bwd_kernel(const BwdAr
 
 // ---- rows of any length: one workgroup per row walks it once per sum, four vectors of each thread on their way at a time.  A vector's values are
 // added in 32 bits, the vectors of a thread -- up to 2^16 of them -- in 64 (in 32 the roundings of equal terms all go one way: 2^20 times
-// 1.1 comes out 1 % off).
+// 1.1 comes out 1 % off).  4096 x 20000 f32 forward 169 us = 3.9 TB/s of what has to move (the second and third walk find the row in the caches),
+// backward 400; two rows of 2^24 3.4 ms, what one CU each can fetch.  Eight loads in flight: within 4 % either way.
 constexpr int LONG_NT = 1024, LONG_U = 4;
 template <typename T, typename F>
 __device__ __forceinline__ void walk(const T* x, int D, F take /* (vector, its first column, elements of the row from there on) */) {
@@ -433,7 +437,8 @@ __global__ __launch_bounds__(NT) void ln_part_kernel(const BwdArgs a) {
   p[a.D + j] = db;
 }
 
-// out[e] = sum over the parts of column e, for the 2 D columns (dgamma | dbeta): 32 columns and 32 shares of the parts per workgroup
+// out[e] = sum over the parts of column e, for the 2 D columns (dgamma | dbeta): 32 columns and 32 shares of the parts per workgroup.
+// 1024 parts of 1024 columns (8 MB): 4.2 us; 512 of 128: 2.2, a launch.
 constexpr int SUM_NT = 1024;
 __global__ __launch_bounds__(SUM_NT) void ln_sum_kernel(const float* __restrict__ part, int n_parts, int D, float* __restrict__ dgamma,
                                                         float* __restrict__ dbeta) {
@@ -458,6 +463,20 @@ __global__ __launch_bounds__(SUM_NT) void ln_sum_kernel(const float* __restrict_
     }
     if (e0 + (long)gridDim.x * 32 < E) __syncthreads();
   }
+}
+
+// ... a column per thread, for at most 32 parts of many columns (one part of 2^24 columns: 72 us against 2260, 32 of 200000: 10.5 against 41; 32 of
+// 5000 columns the other way round: 3.3 against 2.6)
+constexpr int FEW_PARTS = 32, MANY_COLUMNS = 16384;
+__global__ __launch_bounds__(NT) void ln_sum_few_kernel(const float* __restrict__ part, int n_parts, int D, float* __restrict__ dgamma,
+                                                        float* __restrict__ dbeta) {
+  const long E = 2l * D, e = (long)blockIdx.x * NT + threadIdx.x;
+  float* const out = e < D ? dgamma : dbeta;
+  if (e >= E || out == nullptr) return;
+  double s = 0.0;
+#pragma unroll 8
+  for (int p = 0; p < n_parts; ++p) s += (double)part[(long)p * E + e];
+  out[e < D ? e : e - D] = (float)s;
 }
 
 // The parts of a backward pass: consecutive rows each, at most 512 of them while a launch's second dimension (65535) allows it -- a thread adds
@@ -608,7 +627,8 @@ int emx_layernorm_bwd(const void* dy, int64_t ld_dy, const void* x, int64_t ldx,
     if (rc) return rc;
   }
   if (!sums) return EMX_OK;
-  hipLaunchKernelGGL(ln_sum_kernel, dim3((unsigned)std::min((2l * D + 31) / 32, 1l << 20)), dim3(SUM_NT), 0, st, ws, parts, D, dgamma, dbeta);
+  if (parts <= FEW_PARTS && D >= MANY_COLUMNS) hipLaunchKernelGGL(ln_sum_few_kernel, dim3((unsigned)((2l * D + NT - 1) / NT)), dim3(NT), 0, st, ws, parts, D, dgamma, dbeta);
+  else hipLaunchKernelGGL(ln_sum_kernel, dim3((unsigned)std::min((2l * D + 31) / 32, 1l << 20)), dim3(SUM_NT), 0, st, ws, parts, D, dgamma, dbeta);
   return check_launch(who);
 }
 
