@@ -125,7 +125,8 @@ __device__ __forceinline__ int find(const Mat* m, int n, int launch, int block, 
 }
 
 // ---- 1: the sum of squares in shares; the optimizer step also forms its update's direction u here.  Four consecutive elements per
-// thread at a time where the rows allow it (their length is a multiple of 4), the parts of a gradient eight at a time.
+// thread at a time where the rows allow it (their length is a multiple of 4), the parts of a gradient eight at a time.  Bound by HBM: 4096 x
+// 4096 f32 14.6 us = 4.6 TB/s; the optimizer step's of 21 M weights in one part 50 us, 340 MB read and written = 6.7 TB/s.
 template <typename T, bool MUON, int E>
 __device__ __forceinline__ double norm_share(const Mat& m, const StepArgs& a, float* u_out, unsigned e0, unsigned e1) {
   typedef T vec __attribute__((ext_vector_type(E), aligned(sizeof(T))));
@@ -229,7 +230,7 @@ __device__ __forceinline__ void split_unit(const float (&v)[8], char* hi, char* 
   *reinterpret_cast<uint4v*>(lo) = uint4v{y[0], y[1], y[2], y[3]};
 }
 
-// ---- 2: X_0 and its transpose as operands: a workgroup per 64 x 64 of X
+// ---- 2: X_0 and its transpose as operands: a workgroup per 64 x 64 of X.  4096 x 4096 f32 35 us for 67 MB read and 134 written = 5.7 TB/s.
 template <typename T, bool MUON>
 __global__ __launch_bounds__(NT) void ns_split_kernel(char* ws, const int n) {
   __shared__ float tile[64][65];
@@ -1203,7 +1204,8 @@ int tile_size(F tiles, int launch) {
 
 // The last tiles of a launch that has a whole round of them for the 256 CUs and at most half a round more: cut along k into as many parts as fill
 // the round (16 at most, four blocks of k to each): the upper half of 4096 x 4096, 528 tiles, 255 us -> 193 + 8 in ns_whole_kernel; six 1000 x 1500, 576
-// tiles, 72 -> 61 + 6.  Below 1024 k a tile is done in the time that ns_whole_kernel takes.
+// tiles, 72 -> 61 + 6.  Below 1024 k a tile is done in the time that ns_whole_kernel takes.  (Less than a round of tiles -- a CU with one runs at
+// 93 % of its rate with two -- cut in two: five steps of six 1000 x 1500 742 -> 839 us.)
 constexpr long CUS = 256;
 int cuts_of(int size, long count, int blocks_of_k) {
   const long rest = count % CUS;
