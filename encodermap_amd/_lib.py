@@ -916,7 +916,8 @@ class MatrixPlan:
     """The matrices of flat buffers that ``orthogonalize`` / ``muon_step`` work on, and the launches' scratch.
 
     ``mats``: (offset, rows, cols, row stride, scale of the update) per matrix, offsets in elements.  One plan serves one call at a time
-    (calls on different streams that may overlap need a plan each)."""
+    (calls on different streams that may overlap need a plan each), and has to live until its calls are done: the scratch belongs to the stream that
+    was current when the plan was made."""
 
     def __init__(self, mats, device="cuda"):
         self.n = len(mats)
