@@ -456,21 +456,28 @@ def launches_per_step(eng):
     return int(n1 - n0)
 
 
+_PORT_STORE, _PORTS_AGREED = None, 0   # (rank 0 may be the one that serves the store: kept until the process ends)
+
+
 def agree_on_port(world: int, rank: int) -> int:
-    """a free port for the probe children's rendezvous, the SAME on every rank: rank 0 asks the kernel for one and the ranks learn it
-    over a short-lived gloo group (CPU only: nothing here touches a GPU; the launcher's MASTER_PORT carries that group, the RCCL
-    group is initialised later on the same store).  One rank: no exchange."""
+    """a free port for the probe children's rendezvous, the SAME on every rank: rank 0 asks the kernel for one and leaves it in the
+    launcher's store (nothing here touches a GPU).  No process group of its own: two default groups one after the other have the
+    same name and so the same keys in that store, and a rank that comes to the second one first takes the other's address in the first
+    for the present one and waits for good.  One rank: no exchange."""
+    global _PORT_STORE, _PORTS_AGREED
     if world <= 1:
         return _free_port()
-    import torch.distributed as dist
+    if _PORT_STORE is None:
+        import torch.distributed as dist
+        from torch.distributed.rendezvous import rendezvous
 
-    dist.init_process_group("gloo", rank=rank, world_size=world)
-    try:
-        box = [_free_port() if rank == 0 else None]
-        dist.broadcast_object_list(box, src=0)
-    finally:
-        dist.destroy_process_group()
-    return int(box[0])
+        store, _, _ = next(rendezvous("env://", rank=rank, world_size=world))
+        _PORT_STORE = dist.PrefixStore("bench_probe_port", store)
+    _PORTS_AGREED += 1
+    key = f"port{_PORTS_AGREED}"       # (every call's own: another one's port may still be there)
+    if rank == 0:
+        _PORT_STORE.set(key, str(_free_port()))
+    return int(_PORT_STORE.get(key))
 
 
 def start_watchdog(seconds: float, what: str):
@@ -592,7 +599,7 @@ def launch_check(args) -> int:
     forced_eager = os.environ.get("EMX_DP_GRAPH_ALLREDUCE") == "0"
     if os.environ.get("EMX_BENCH_FAIL_CAPTURED") == "1" and not forced_eager:
         return 3
-    # as main() does it: the probe's port over a short-lived gloo group, then the run's own group on the same store
+    # as main() does it: the probe's port through the launcher's store, then the run's own group on the same store
     port = agree_on_port(world, rank)
     call_off = start_watchdog(float(os.environ.get("EMX_BENCH_WATCHDOG", "900")), f"the {world}-rank launch check")
     if os.environ.get("EMX_BENCH_HANG") == "1":            # (test hook: a rank that never comes back -- the watchdog's case)
