@@ -130,6 +130,16 @@ __device__ __forceinline__ void split_f16_pair(const float v0, const float v1, u
 #endif
 }
 
+// The registers of a matrix instruction's operand that inline assembly (split_f16_pair) has written.  A vector instruction's result may be
+// read by a matrix instruction two wait states later at the earliest, and the hardware does not hold the second one back: the compiler
+// puts the wait behind its own instructions, but does not see those of an assembly block (one state was left in ns_whole_kernel and in
+// some of the inference kernels).  In the operand's own registers, so that it stands between the two wherever they are scheduled.
+template <typename V>
+__device__ __forceinline__ V matrix_operand(V v) {
+  asm("s_nop 1" : "+v"(v));
+  return v;
+}
+
 // sin and cos of an angle of moderate size (|x| up to a few thousand: data angles are within a few periods): three-term
 // Cody-Waite reduction by pi/2 and the classic degree-7 / degree-8 minimax polynomials on [-pi/4, pi/4], ~1.5 ulp.  The
 // library sincosf carries a Payne-Hanek path for huge arguments that costs ~3 KB of scratch per lane in every kernel that

@@ -111,6 +111,7 @@ __device__ __forceinline__ void in2_split2(const float v0, const float v1, half8
   split_f16_pair(v0, v1, ph, pl);   // (three instructions a pair: emx_common.h)
   const half2v vh = __builtin_bit_cast(half2v, ph), vl = __builtin_bit_cast(half2v, pl);
   oh[i] = vh[0], oh[i + 1] = vh[1], ol[i] = vl[0], ol[i + 1] = vl[1];
+  if (i == 6) oh = matrix_operand(oh), ol = matrix_operand(ol);   // (pairs come in ascending order: the operand is complete)
 }
 
 // One layer of class (S, T) on the wave's 16 rows, products AND epilogue with every bound a compile-time constant: run-time tile

@@ -404,7 +404,8 @@ __device__ __forceinline__ void put_turned(char* block, const Planes& x, const h
     for (int e = 0; e < 16; ++e) d[e] = 0.f;
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks)
-      d = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8, uint4v{v[4 * ks], v[4 * ks + 1], v[4 * ks + 2], v[4 * ks + 3]}), one[ks], d, 0, 0, 0);
+      d = __builtin_amdgcn_mfma_f32_32x32x16_f16(
+          __builtin_bit_cast(half8, matrix_operand(uint4v{v[4 * ks], v[4 * ks + 1], v[4 * ks + 2], v[4 * ks + 3]})), one[ks], d, 0, 0, 0);
 #pragma unroll
     for (int q = 0; q < 4; ++q)
       *reinterpret_cast<uint2*>(block + (q >> 1) * 2048 + ((q & 1) * 32 + lr) * 16 + h * 8 + plane * 1024) =

@@ -1,0 +1,86 @@
+"""The wait states in front of matrix instructions, in the library as it is built: a vector instruction's result may be read by a matrix instruction two wait
+states later at the earliest.  The compiler sees to that between its own instructions, but not where one of them is inline assembly."""
+import os
+import re
+import shutil
+import struct
+import subprocess
+
+import pytest
+
+from encodermap_amd import _lib
+
+OBJDUMP = shutil.which("llvm-objdump") or "/opt/rocm/llvm/bin/llvm-objdump"
+NEEDED = 2
+MAGIC = b"__CLANG_OFFLOAD_BUNDLE__"
+REGISTERS = re.compile(r"\b([va])(?:\[(\d+):(\d+)\]|(\d+)\b)")
+
+
+def registers(text):
+    out = set()
+    for kind, first, last, one in REGISTERS.findall(text):
+        out.update((kind, i) for i in (range(int(first), int(last) + 1) if first else (int(one),)))
+    return out
+
+
+def code_objects(library):
+    """the gfx950 code objects that the shared library's offload bundles hold"""
+    at = library.find(MAGIC)
+    while at >= 0:
+        (count,) = struct.unpack_from("<Q", library, at + len(MAGIC))
+        entry = at + len(MAGIC) + 8
+        for _ in range(count):
+            offset, size, length = struct.unpack_from("<QQQ", library, entry)
+            name = library[entry + 24:entry + 24 + length]
+            entry += 24 + length
+            if b"gfx950" in name and size:
+                yield library[at + offset:at + offset + size]
+        at = library.find(MAGIC, at + len(MAGIC))
+
+
+def early_reads(lines):
+    """(function, instruction, states) of every matrix instruction that reads what a vector instruction has written too few states before"""
+    function, recent, found = "", [], []       # recent: (states since, registers) of the last vector results
+    for line in lines:
+        if line.endswith(">:\n"):
+            function, recent = line[line.find("<") + 1:-3], []
+            continue
+        text = line.split("//")[0].strip()
+        if not text or ":" in text.split()[0]:
+            continue
+        op, _, rest = text.partition(" ")
+        operands = rest.split(",")
+        if op.startswith("v_mfma"):
+            read = registers(",".join(operands[1:4]))
+            found += [(function, text, states) for states, written in recent if written & read]
+        states = int(operands[0], 0) + 1 if op == "s_nop" else 1
+        recent = [(since + states, written) for since, written in recent if since + states < NEEDED]
+        if op.startswith("v_") and not op.startswith("v_mfma"):
+            recent.append((0, registers(operands[0])))
+    return found
+
+
+def test_the_reader_finds_an_early_read():
+    listing = ["0000000000001000 <kernel>:\n", "\tv_cvt_pk_f16_f32 v9, v15, v14   // 0: 0\n", "\tv_mul_f32_e32 v26, 0x38800000, v13\n"]
+    use = "\tv_mfma_f32_32x32x16_f16 a[0:15], v[6:9], v[2:5], 0\n"
+    assert [f[2] for f in early_reads(listing + [use])] == [1]
+    assert early_reads(listing + ["\ts_nop 0\n", use]) == []
+    assert [f[2] for f in early_reads(listing[:2] + [use])] == [0]
+    assert early_reads(listing[:2] + ["\ts_nop 1\n", use]) == []
+
+
+@pytest.mark.skipif(not os.path.exists(OBJDUMP), reason="no llvm-objdump")
+def test_no_matrix_instruction_reads_a_result_early(tmp_path):
+    _lib.load()
+    with open(_lib.LIB_PATH, "rb") as f:
+        objects = list(code_objects(f.read()))
+    assert objects
+    matrix, found = 0, []
+    for i, data in enumerate(objects):
+        path = tmp_path / f"{i}.hsaco"
+        path.write_bytes(data)
+        text = subprocess.run([OBJDUMP, "-d", "--no-show-raw-insn", str(path)], capture_output=True, text=True, check=True).stdout
+        matrix += text.count("v_mfma")
+        found += early_reads(text.splitlines(keepends=True))
+    assert matrix > 1000
+    assert not found, f"{len(found)} of {matrix}: {found[:5]}"
