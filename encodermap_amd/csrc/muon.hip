@@ -9,8 +9,10 @@
 // obeys, whatever G is: |X| <= 1.21, |A| <= 1.45, |P| <= 2.81.
 //
 // Arithmetic: as the dense layers', every float32 product is THREE f16 matrix instructions on operands split into two f16 planes (hi = f16(v),
-// lo = f16(v - hi): 22 bits), accumulated in float32.  The bounds above make ONE fixed scale of 2^14 enough for X, A and P (|P| 2^14 <= 46.1e3
-// < 65504; what is lost below is 2^-24 2^-14 of the matrix' norm).  The norm is summed in 64 bits: an error of its scale is the one that
+// lo = f16(v - hi): 22 bits), accumulated in float32.  The bounds above make a scale of 2^14 enough for X, A and P (|P| 2^14 <= 46.1e3
+// < 65504; what is lost below is 2^-24 2^-14 of the matrix' norm).  Where |G|_F is small beside eps, |X_0|_F = |G|_F / (|G|_F + eps) is too, and
+// X is held another 2^q times as large (X~ = 2^q X), so that |X~| <= 1/2:  A~ = X~ X~^T = 4^q A,  P~ = b A~ + 4^-q c A~^2 = 4^q P (|P~| <= 1.2),
+// and a X~ + 4^-q P~ X~ = 2^q X_k+1.  q shrinks from step to step by what |X| may have grown (shift_at).  The norm is summed in 64 bits: an error of its scale is the one that
 // the iteration turns into an error of every singular value.  a X joins P X behind its sum, not as a diagonal of P: the sum then rounds at the
 // size of P X alone (4096 x 4096: 4.4e-6 off with it inside).
 //
@@ -72,13 +74,15 @@ struct alignas(16) Table {
 constexpr long TABLE_BYTES = 4096;
 static_assert(sizeof(Table) <= 4032 && sizeof(Table) % 16 == 0, "the first launch's arguments");
 
-// The scratch of one matrix: the shares of its sum of squares, X^T twice (read and written by a step; the second also holds the optimizer step's
+// The scratch of one matrix: the shares of its sum of squares and its shift, X^T twice (read and written by a step; the second also holds the optimizer step's
 // direction u at the begin) and, M > 128: X, A and P; M <= 128: the shares of A twice, 16 blocks from each workgroup.
 constexpr int LOW = 4;                        // blocks: matrices of at most 128 rows stay in the LDS of a workgroup (ns_low_kernel)
 constexpr int LOW_WGS = 32;                   // ... 128 columns each, or more where there are more than 32 x 128
+constexpr int HEAD = MAX_PARTS * 8 + 128;     // bytes in front of the operands
 struct Scratch {
   int M, N, Mb, Nb;
   bool turned;
+  int* shift;          // q of X_0
   char *t0, *t1, *x, *a, *p, *parts;
   double* part;
   __host__ __device__ Scratch(int rows, int cols, char* base) {
@@ -87,7 +91,8 @@ struct Scratch {
     Mb = (M + 31) / 32, Nb = (N + 31) / 32;
     const long xn = (long)Mb * Nb * BLK, an = low() ? (long)low_wgs() * 16 * BLK : (long)Mb * Mb * BLK;
     part = reinterpret_cast<double*>(base);
-    t0 = base + MAX_PARTS * 8, t1 = t0 + xn;
+    shift = reinterpret_cast<int*>(base + MAX_PARTS * 8);
+    t0 = base + HEAD, t1 = t0 + xn;
     x = t1 + xn;
     a = low() ? x : x + xn;
     p = a + an;
@@ -106,7 +111,7 @@ struct Scratch {
     const Scratch s(rows, cols, nullptr);
     const size_t xn = (size_t)s.Mb * s.Nb;
     const size_t an = (size_t)s.Mb * s.Mb;
-    return MAX_PARTS * 8 + (s.low() ? 2 * xn + 2 * (size_t)s.low_wgs() * 16 : 3 * xn + (2 + (s.gram_parts() > 1 ? s.gram_parts() : 0)) * an) * BLK;
+    return HEAD + (s.low() ? 2 * xn + 2 * (size_t)s.low_wgs() * 16 : 3 * xn + (2 + (s.gram_parts() > 1 ? s.gram_parts() : 0)) * an) * BLK;
   }
 };
 // (1024 elements and more to a share: the optimizer step reads up to 32 gradient parts of each)
@@ -206,9 +211,19 @@ __global__ __launch_bounds__(NT) void ns_norm_kernel(char* ws, const Table tab) 
   __syncthreads();
   if (threadIdx.x == 0) s.part[part] = (sm[0] + sm[1]) + (sm[2] + sm[3]);
 }
-// 2^14 / (|u|_F + eps), in every thread of a workgroup of N threads
+// How X_0 is held: 2^q u / (|u|_F + eps), |X~_0|_F in 1/8 .. 1/2 (q = 0: as it is; 96 at most, |u|_F = 1e-29 eps)
+struct Start {
+  double inv;          // 1 / (|u|_F + eps)
+  int q;
+  __device__ __forceinline__ double scale() const { return ldexp(inv, 14 + q); }
+};
+constexpr int MAX_SHIFT = 96;
+// q of X_k: a step multiplies |X| by 3.4445 = 2^1.7843 at most, and 457 / 256 = 1.7852
+__device__ __forceinline__ int shift_at(int q0, int k) { return max(q0 - (457 * k + 255) / 256, 0); }
+__device__ __forceinline__ float pow2(int e) { return ldexpf(1.f, e); }
+// in every thread of a workgroup of N threads
 template <int N>
-__device__ __forceinline__ double scale_of(const Mat& m, const Scratch& s, float eps, double* sm /* N / 64 */) {
+__device__ __forceinline__ Start start_of(const Mat& m, const Scratch& s, float eps, double* sm /* N / 64 */) {
   const int parts = parts_of((long)m.rows * m.cols);
   double sum = 0.0;
   for (int i = threadIdx.x; i < parts; i += N) sum += s.part[i];
@@ -218,7 +233,14 @@ __device__ __forceinline__ double scale_of(const Mat& m, const Scratch& s, float
   sum = 0.0;
 #pragma unroll
   for (int i = 0; i < N / 64; ++i) sum += sm[i];
-  return (double)SC / (sqrt(sum) + (double)eps);
+  const double norm = sqrt(sum), all = norm + (double)eps;
+  const auto exponent = [](double v) { return (int)((__double_as_longlong(v) >> 52) & 0x7ff); };   // (of zero: 0)
+  return {1.0 / all, min(max(exponent(all) - exponent(norm) - 2, 0), MAX_SHIFT)};
+}
+// the matrix' shift as an earlier launch has left it: a scalar load, asked for long before its use
+__device__ __forceinline__ int shift_of(const Scratch& s) {
+  typedef const __attribute__((address_space(4))) int* Uniform;
+  return *(Uniform)(uintptr_t)s.shift;
 }
 
 // eight values of a row as the hi and lo units of an operand
@@ -242,7 +264,9 @@ __global__ __launch_bounds__(NT) void ns_split_kernel(char* ws, const int n) {
   const Scratch s(m.rows, m.cols, ws + m.ws);
   const int tid = threadIdx.x;
   const int tn = (s.Nb + 1) / 2, ti = inside / tn, tj = inside - ti * tn;
-  const double f = scale_of<NT>(m, s, a.eps, sm);
+  const Start start = start_of<NT>(m, s, a.eps, sm);
+  if (inside == 0 && tid == 0) *s.shift = start.q;
+  const double f = start.scale();
   const float* const u_in = reinterpret_cast<const float*>(s.t1);
   // the tile as it is stored: rows (r0 ..), columns (c0 ..) of G
   const int r0 = 64 * (s.turned ? tj : ti), c0 = 64 * (s.turned ? ti : tj);
@@ -270,11 +294,13 @@ __global__ __launch_bounds__(NT) void ns_split_kernel(char* ws, const int n) {
 
 // ---- 3: the products.  KIND 0: A = X X^T; 1: P = a I + b A + c A A^T; 2: X <- P X; 3: the last step's X, written out
 enum { GRAM = 0, POLY = 1, NEXT = 2, LAST = 3 };
-// A 32 x 32 block of the last X into the caller's tensors (x: row 32 ib + 8 q + 4 h + r, column 32 jb + lr, scaled by 2^28): the update of w, or
-// the result.  All of a block's reads stand in front of its writes.  A turned matrix has four consecutive elements per lane.
+// A 32 x 32 block of the last X into the caller's tensors (x: row 32 ib + 8 q + 4 h + r, column 32 jb + lr, scaled by 2^28 2^shift): the update of
+// w, or the result.  All of a block's reads stand in front of its writes.  A turned matrix has four consecutive elements per lane.
 template <typename T, bool MUON>
-__device__ __forceinline__ void write_block(const Mat& m, const StepArgs& a, const Scratch& s, const f32x16& x, int ib, int jb, int lr, int h) {
-  const float keep = a.keep, f = MUON ? -(a.lr * m.scale) * (RSC * RSC) : RSC * RSC;
+__device__ __forceinline__ void write_block(const Mat& m, const StepArgs& a, const Scratch& s, f32x16 x, int shift, int ib, int jb, int lr, int h) {
+  const float keep = a.keep, f = MUON ? -(a.lr * m.scale) : 1.f, unscale = RSC * RSC * pow2(-shift);
+#pragma unroll
+  for (int e = 0; e < 16; ++e) x[e] *= unscale;
   const int row0 = 32 * ib + 4 * h, col = 32 * jb + lr;
   typedef typename std::conditional<MUON, float, T>::type O;
   O* const base = (MUON ? (O*)a.w : (O*)a.out) + m.off;
@@ -425,6 +451,14 @@ __device__ __forceinline__ void add_planes(f32x16& x, const char* block, float f
   }
 }
 
+// x 4^-shift; the same shift in all lanes, and most matrices' is zero
+__device__ __forceinline__ void shift_down(f32x16& x, int shift) {
+  if (shift == 0) return;
+  const float f = pow2(-2 * shift);
+#pragma unroll
+  for (int e = 0; e < 16; ++e) x[e] *= f;
+}
+
 __device__ __forceinline__ float4* part_of(const Scratch& s, int part, int ib, int jb, int q, int lane) {
   return reinterpret_cast<float4*>(s.parts + (((long)part * s.Mb + ib) * s.Mb + jb) * BLK + q * 1024 + lane * 16);
 }
@@ -432,7 +466,7 @@ __device__ __forceinline__ float4* part_of(const Scratch& s, int part, int ib, i
 // A block of a product where it belongs (x: element 4 q + r = row 32 ib + 8 q + 4 h + r of column 32 jb + lr, scaled by 2^28)
 template <int KIND, typename T, bool MUON>
 __device__ __forceinline__ void store_block(const Mat& m, const StepArgs& a, const Scratch& s, f32x16 x, int ib, int jb, int part /* of the sum; -1: all of it */,
-                                            const char* t_in, char* t_out, int lr, int h) {
+                                            const char* t_in, char* t_out, int k /* the step */, int q0, int lr, int h) {
   if (ib >= s.Mb || jb >= (KIND <= POLY ? s.Mb : s.Nb) || (KIND <= POLY && ib > jb)) return;   // (A and P: the upper half, stored twice)
   if constexpr (KIND == GRAM) {
     if (part >= 0) {
@@ -441,15 +475,18 @@ __device__ __forceinline__ void store_block(const Mat& m, const StepArgs& a, con
       return;
     }
   }
+  const int shift = shift_at(q0, k);
+  if constexpr (KIND != GRAM) shift_down(x, shift);
   if constexpr (KIND >= NEXT) add_planes(x, t_in + ((long)jb * s.Mb + ib) * BLK, CA * SC, lr, h);
   if constexpr (KIND == LAST) {
-    write_block<T, MUON>(m, a, s, x, ib, jb, lr, h);
+    write_block<T, MUON>(m, a, s, x, shift, ib, jb, lr, h);
   } else {
     half8 one[2];
     identity(one, lr, h);
     char* const O = KIND == GRAM ? s.a : KIND == POLY ? s.p : t_out;
+    const float f = KIND == NEXT ? RSC * pow2(shift_at(q0, k + 1) - shift) : RSC;
 #pragma unroll
-    for (int e = 0; e < 16; ++e) x[e] *= RSC;
+    for (int e = 0; e < 16; ++e) x[e] *= f;
     if constexpr (KIND == POLY) {
 #pragma unroll
       for (int e = 0; e < 16; ++e) x[e] *= CC;
@@ -485,7 +522,7 @@ __device__ __forceinline__ float4* cut_of(char* ws, int rb, int unit, int cuts, 
 }
 
 template <int KIND, typename T, bool MUON, int RB>
-__global__ __launch_bounds__(NT, 2) void ns_big_kernel(char* ws, const int n, const int odd, const int whole, const int run, const int first_cut,
+__global__ __launch_bounds__(NT, 2) void ns_big_kernel(char* ws, const int n, const int step, const int whole, const int run, const int first_cut,
                                                        const int cuts) {
   __shared__ __align__(16) char lds[2][BT_C * BLK];
   // runs of consecutive tiles to each XCD: they share operands in its L2
@@ -503,7 +540,7 @@ __global__ __launch_bounds__(NT, 2) void ns_big_kernel(char* ws, const int n, co
   const Scratch& s = unit.s;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lr = lane & 31, h = lane >> 5;
-  char *const t_in = odd ? s.t1 : s.t0, *const t_out = odd ? s.t0 : s.t1;
+  char *const t_in = (step & 1) ? s.t1 : s.t0, *const t_out = (step & 1) ? s.t0 : s.t1;
   const int Jb = KIND <= POLY ? s.Mb : s.Nb, Ks = unit.Ks, parts = unit.parts, part = unit.part;
   int K0 = unit.K0, Kb = unit.Kb;                          // this workgroup's blocks of k
   if (cut >= 0) {
@@ -511,6 +548,7 @@ __global__ __launch_bounds__(NT, 2) void ns_big_kernel(char* ws, const int n, co
     Kb = (cut + 1) * unit.Kb / cuts - cut * unit.Kb / cuts;
   }
   const int ib0 = RB * (4 * unit.ti + wave), jb0 = BT_C * unit.tj;   // this wave's first blocks
+  const int q0 = KIND == GRAM ? 0 : shift_of(s);
   const char* const Ub = KIND == GRAM ? s.x : KIND == POLY ? s.a : s.p;
   const char* const Vb = KIND == GRAM ? s.x : KIND == POLY ? s.a : t_in;
   // (blocks beyond the matrix are read from its last one and not stored)
@@ -630,15 +668,16 @@ __global__ __launch_bounds__(NT, 2) void ns_big_kernel(char* ws, const int n, co
 #pragma unroll
   for (int i = 0; i < RB; ++i)
 #pragma unroll
-    for (int j = 0; j < BT_C; ++j) store_block<KIND, T, MUON>(m, a, s, acc[i][j], ib0 + i, jb0 + j, parts > 1 ? part : -1, t_in, t_out, lr, h);
+    for (int j = 0; j < BT_C; ++j) store_block<KIND, T, MUON>(m, a, s, acc[i][j], ib0 + i, jb0 + j, parts > 1 ? part : -1, t_in, t_out, step, q0, lr, h);
 }
 
 // The tiles that were cut, from their shares in the shares' order: a workgroup per column of blocks
 template <int KIND, typename T, bool MUON, int RB>
-__global__ __launch_bounds__(NT) void ns_whole_kernel(char* ws, const int n, const int odd, const int whole, const int cuts) {
+__global__ __launch_bounds__(NT) void ns_whole_kernel(char* ws, const int n, const int step, const int whole, const int cuts) {
   const int u = (int)blockIdx.x / BT_C, j = (int)blockIdx.x % BT_C;
   const Unit<KIND, RB> unit(ws, n, whole + u);
   const Scratch& s = unit.s;
+  const int q0 = KIND == GRAM ? 0 : shift_of(s);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 #pragma unroll
   for (int i = 0; i < RB; ++i) {
@@ -653,7 +692,7 @@ __global__ __launch_bounds__(NT) void ns_whole_kernel(char* ws, const int n, con
         x[4 * q] += v.x, x[4 * q + 1] += v.y, x[4 * q + 2] += v.z, x[4 * q + 3] += v.w;
       }
     store_block<KIND, T, MUON>(unit.m, reinterpret_cast<const Table*>(ws)->a, s, x, RB * (4 * unit.ti + wave) + i, BT_C * unit.tj + j,
-                               unit.parts > 1 ? unit.part : -1, odd ? s.t1 : s.t0, odd ? s.t0 : s.t1, lane & 31, lane >> 5);
+                               unit.parts > 1 ? unit.part : -1, (step & 1) ? s.t1 : s.t0, (step & 1) ? s.t0 : s.t1, step, q0, lane & 31, lane >> 5);
   }
 }
 
@@ -678,14 +717,14 @@ __global__ __launch_bounds__(NT) void ns_join_kernel(char* ws, const int n) {
       const float4 v = *part_of(s, p, ib, jb, q, lane);
       x[4 * q] += v.x, x[4 * q + 1] += v.y, x[4 * q + 2] += v.z, x[4 * q + 3] += v.w;
     }
-  store_block<GRAM, float, false>(m, tab.a, s, x, ib, jb, -1, nullptr, nullptr, lane & 31, lane >> 5);
+  store_block<GRAM, float, false>(m, tab.a, s, x, ib, jb, -1, nullptr, nullptr, 0, 0, lane & 31, lane >> 5);
 }
 
 // ---- the products in tiles of 64 x 64, for matrices that would leave most of the machine idle in larger ones: the four waves of a
 // workgroup take a quarter of k each, straight from global memory (four K-steps of operands in registers: three travel under the products of
 // one), and add up through LDS, a block to each wave.
 template <int KIND, typename T, bool MUON>
-__global__ __launch_bounds__(NT, 2) void ns_mid_kernel(char* ws, const int n, const int odd, const int total, const int run, int, int) {
+__global__ __launch_bounds__(NT, 2) void ns_mid_kernel(char* ws, const int n, const int step, const int total, const int run, int, int) {
   __shared__ __align__(16) float4 fold[4][3][4][64];   // [block][wave but its own][q][lane]
   const int turn = (int)(blockIdx.x >> 3), at = ((turn / run) * 8 + (int)(blockIdx.x & 7)) * run + turn % run;
   if (at >= total) return;
@@ -696,14 +735,14 @@ __global__ __launch_bounds__(NT, 2) void ns_mid_kernel(char* ws, const int n, co
   const Scratch s(m.rows, m.cols, ws + m.ws);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lr = lane & 31, h = lane >> 5;
-  char *const t_in = odd ? s.t1 : s.t0, *const t_out = odd ? s.t0 : s.t1;
+  char *const t_in = (step & 1) ? s.t1 : s.t0, *const t_out = (step & 1) ? s.t0 : s.t1;
   const int Jb = KIND <= POLY ? s.Mb : s.Nb, Ks = KIND == GRAM ? s.Nb : s.Mb;
   const int parts = KIND == GRAM ? s.gram_parts() : 1, part = inside % parts;
   const int K0 = part * Ks / parts, Kb = (part + 1) * Ks / parts - K0;
   inside /= parts;
   int ti, tj;
   tile_of(inside, (s.Mb + 1) / 2, (Jb + 1) / 2, 1, KIND <= POLY, ti, tj);
-  const int ib0 = 2 * ti, jb0 = 2 * tj;
+  const int ib0 = 2 * ti, jb0 = 2 * tj, q0 = KIND == GRAM ? 0 : shift_of(s);
   const char* const Ub = KIND == GRAM ? s.x : KIND == POLY ? s.a : s.p;
   const char* const Vb = KIND == GRAM ? s.x : KIND == POLY ? s.a : t_in;
   // (blocks beyond the matrix are read from its last one and not stored)
@@ -779,7 +818,7 @@ __global__ __launch_bounds__(NT, 2) void ns_mid_kernel(char* ws, const int n, co
     x[4 * q + 2] = (s0.z + s1.z) + (s2.z + s3.z);
     x[4 * q + 3] = (s0.w + s1.w) + (s2.w + s3.w);
   }
-  store_block<KIND, T, MUON>(m, a, s, x, ib0 + (wave >> 1), jb0 + (wave & 1), parts > 1 ? part : -1, t_in, t_out, lr, h);
+  store_block<KIND, T, MUON>(m, a, s, x, ib0 + (wave >> 1), jb0 + (wave & 1), parts > 1 ? part : -1, t_in, t_out, step, q0, lr, h);
 }
 
 // ---- matrices of at most 128 rows: a workgroup of sixteen waves holds 128 columns of X in registers, a wave one block.  The operands of the
@@ -904,7 +943,7 @@ __device__ void thin_matrix(Thin& l, double* sm, const Mat& m, const Scratch& s,
   };
   double y[2], sum = 0.0;
   if (step == 0) {
-    const double f = scale_of<LOW_NT>(m, s, a.eps, sm) * (double)RSC;
+    const double f = start_of<LOW_NT>(m, s, a.eps, sm).inv;
     for (int st = wg; st < s.strips(); st += wgs) {
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
@@ -990,7 +1029,8 @@ __global__ __launch_bounds__(LOW_NT) void ns_low_kernel(char* ws, const int n, c
     put_direct(area + (jb * 4 + ib) * BLK, y, lr, h);
     if (ib != jb) put_turned(area + (ib * 4 + jb) * BLK, y, one, lr, h);
   };
-  auto form_poly = [&]() __attribute__((always_inline)) {   // av: A, area2: A (complete).  Leaves P in area2 (complete)
+  auto form_poly = [&](int shift) __attribute__((always_inline)) {   // av: A, area2: A (complete).  Leaves P in area2 (complete)
+    const float c = CC * RSC * pow2(-2 * shift);
     f32x16 sq;
     clear(sq);
     if (square) low_product(sq, u2, v2, Mb);
@@ -998,7 +1038,7 @@ __global__ __launch_bounds__(LOW_NT) void ns_low_kernel(char* ws, const int n, c
     if (square) {
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
-        av[e] = fmaf(CC * RSC, sq[e], CB * av[e]);
+        av[e] = fmaf(c, sq[e], CB * av[e]);
       }
       keep_symmetric(area2, av);
     }
@@ -1013,6 +1053,7 @@ __global__ __launch_bounds__(LOW_NT) void ns_low_kernel(char* ws, const int n, c
   };
 
   if (step == 0) {
+    Start start{};
     double f = 0.0;
     f32x16 gram;
     clear(gram);
@@ -1028,7 +1069,7 @@ __global__ __launch_bounds__(LOW_NT) void ns_low_kernel(char* ws, const int n, c
           }
         }
       }
-      if (st == wg) f = scale_of<LOW_NT>(m, s, a.eps, sm);   // (behind the first loads)
+      if (st == wg) start = start_of<LOW_NT>(m, s, a.eps, sm), f = start.scale();   // (behind the first loads)
 #pragma unroll
       for (int e = 0; e < 16; ++e) x[e] = (float)((double)x[e] * f);
       if (!a.low_steps) break;                  // (one strip)
@@ -1043,9 +1084,12 @@ __global__ __launch_bounds__(LOW_NT) void ns_low_kernel(char* ws, const int n, c
     }
     if (a.low_steps) {
       if (square) leave_share(s.a, gram);
+      if (wg == 0 && threadIdx.x == 0) *s.shift = start.q;
       return;
     }
+    const int q0 = __builtin_amdgcn_readfirstlane(start.q);
     for (int k = 0; k < steps; ++k) {
+      const int shift = shift_at(q0, k);
       const Planes y(x);
       if (rows) put_turned(area1 + (ib * 4 + jb) * BLK, y, one, lr, h);
       __syncthreads();
@@ -1057,18 +1101,19 @@ __global__ __launch_bounds__(LOW_NT) void ns_low_kernel(char* ws, const int n, c
       }
       __syncthreads();
       if (rows) put_direct(area1 + (jb * 4 + ib) * BLK, y, lr, h);
-      form_poly();
+      form_poly(shift);
       clear(x);
       if (rows && jb < s.Nb) {
         low_product(x, u2, v1, Mb);
+        shift_down(x, shift);
         add_planes(x, area1 + (jb * 4 + ib) * BLK, CA * SC, lr, h);
       }
       if (k + 1 < steps) {
-        times(x, RSC);
+        times(x, RSC * pow2(shift_at(q0, k + 1) - shift));
         __syncthreads();
       }
     }
-    if (rows && jb < s.Nb) write_block<T, MUON>(m, a, s, x, ib, jb, lr, h);
+    if (rows && jb < s.Nb) write_block<T, MUON>(m, a, s, x, shift_at(q0, steps - 1), ib, jb, lr, h);
     return;
   }
 
@@ -1085,6 +1130,7 @@ __global__ __launch_bounds__(LOW_NT) void ns_low_kernel(char* ws, const int n, c
     for (int q = 0; q < 4; ++q) *reinterpret_cast<half8*>(area1 + (ib * 4 + jb) * BLK + q * 1024 + lane * 16) = t[q];
   };
   request_t(wg);
+  const int q0 = shift_of(s), shift = shift_at(q0, step - 1), shift_out = shift_at(q0, step);
   clear(av);
   if (square) {
 #pragma unroll 4
@@ -1099,7 +1145,7 @@ __global__ __launch_bounds__(LOW_NT) void ns_low_kernel(char* ws, const int n, c
   }
   keep_t();
   __syncthreads();
-  form_poly();
+  form_poly(shift);
   f32x16 gram;
   clear(gram);
   for (int st = wg; st < s.strips(); st += wgs) {
@@ -1112,13 +1158,14 @@ __global__ __launch_bounds__(LOW_NT) void ns_low_kernel(char* ws, const int n, c
     clear(x);
     if (rows) {
       low_product(x, u2, v1, Mb);
+      shift_down(x, shift);
       add_planes(x, area1 + (jb * 4 + ib) * BLK, CA * SC, lr, h);
     }
     if (step == steps) {
-      if (rows && 4 * st + jb < s.Nb) write_block<T, MUON>(m, a, s, x, ib, 4 * st + jb, lr, h);
+      if (rows && 4 * st + jb < s.Nb) write_block<T, MUON>(m, a, s, x, shift, ib, 4 * st + jb, lr, h);
       continue;
     }
-    times(x, RSC);
+    times(x, RSC * pow2(shift_out - shift));
     __syncthreads();
     if (rows) {
       const Planes y(x);
@@ -1298,11 +1345,11 @@ int run(const char* who, const emx_matrix* mats, int n, const StepArgs& a, char*
       // consecutive tiles to an XCD: an eighth of them all, or -- where their lengths differ -- a few in turn, so that each gets long ones
       const long run = p.uneven ? 8 : (whole + 7) / 8, blocks = (whole + 8 * run - 1) / (8 * run) * 8 * run;
       const auto kernel = size == 0 ? ns_mid_kernel<KIND, T, MUON> : size == 1 ? ns_big_kernel<KIND, T, MUON, 1> : ns_big_kernel<KIND, T, MUON, 2>;
-      hipLaunchKernelGGL(kernel, dim3((unsigned)(blocks + rest * cuts)), dim3(NT), 0, st, ws, t.n, k & 1, (int)whole, (int)run, (int)blocks, cuts);
+      hipLaunchKernelGGL(kernel, dim3((unsigned)(blocks + rest * cuts)), dim3(NT), 0, st, ws, t.n, k, (int)whole, (int)run, (int)blocks, cuts);
       const int rc = check_launch(who);
       if (rc || rest == 0) return rc;
       hipLaunchKernelGGL((size == 1 ? ns_whole_kernel<KIND, T, MUON, 1> : ns_whole_kernel<KIND, T, MUON, 2>), dim3((unsigned)(rest * BT_C)), dim3(NT), 0, st, ws,
-                         t.n, k & 1, (int)whole, cuts);
+                         t.n, k, (int)whole, cuts);
       return check_launch(who);
     };
     if ((rc = low(0))) return rc;
