@@ -151,20 +151,29 @@ __device__ __forceinline__ double norm_share(const Mat& m, const StepArgs& a, fl
       const float* g = (const float*)a.g + at;
       fvec mo = *reinterpret_cast<const fvec*>(a.mom + at);
       fvec v = *reinterpret_cast<const fvec*>(g);
+      // (pairs of pairs inside the eight: 32 parts one after the other are 9e-8 off, these 6e-8, as a tree over all of them)
       int k = 1;
-      for (; k + 8 <= a.n_slices; k += 8) {
-        fvec p[8];
+      if (a.n_slices >= 8) {
+        for (k = 0; k + 8 <= a.n_slices; k += 8) {
+          fvec p[8];
 #pragma unroll
-        for (int q = 0; q < 8; ++q) p[q] = *reinterpret_cast<const fvec*>(g + (k + q) * a.slice_stride);
+          for (int q = 0; q < 8; ++q) p[q] = k + q ? *reinterpret_cast<const fvec*>(g + (k + q) * a.slice_stride) : v;
 #pragma unroll
-        for (int q = 0; q < 8; ++q)
-#pragma unroll
-          for (int i = 0; i < E; ++i) v[i] += p[q][i];
+          for (int i = 0; i < E; ++i) {
+            const float eight = ((p[0][i] + p[1][i]) + (p[2][i] + p[3][i])) + ((p[4][i] + p[5][i]) + (p[6][i] + p[7][i]));
+            v[i] = k ? v[i] + eight : eight;
+          }
+        }
       }
-      for (; k < a.n_slices; ++k) {
-        const fvec p = *reinterpret_cast<const fvec*>(g + k * a.slice_stride);
+      if (k < a.n_slices) {                     // the last seven at most (or all of them)
+        fvec r = *reinterpret_cast<const fvec*>(g + k * a.slice_stride);
+        for (++k; k < a.n_slices; ++k) {
+          const fvec p = *reinterpret_cast<const fvec*>(g + k * a.slice_stride);
 #pragma unroll
-        for (int i = 0; i < E; ++i) v[i] += p[i];
+          for (int i = 0; i < E; ++i) r[i] += p[i];
+        }
+#pragma unroll
+        for (int i = 0; i < E; ++i) v[i] += r[i];
       }
       fvec o;
 #pragma unroll

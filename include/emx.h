@@ -604,7 +604,7 @@ int emx_layernorm_bwd(const void* dy, int64_t ld_dy, const void* x, int64_t ldx,
  *     the factor of its update in emx_muon_step.  Matrices of a call may not share elements; rows or cols may be 0 (nothing is done).
  *   emx_orthogonalize: out <- orth(g) for every matrix; g and out (EMX_F32 / EMX_F16 / EMX_BF16, the same offsets in both) may be the same
  *     buffer (any other overlap is refused, as is any between w, g and momentum below).  What lies between the matrices is neither read nor written.
- *   emx_muon_step, float32:  G = sum over n_slices of g[s * slice_stride + .] in order (the weight-gradient partials of emx_mlp_wgrad, or one
+ *   emx_muon_step, float32:  G = sum over n_slices of g[s * slice_stride + .] in a fixed order (the weight-gradient partials of emx_mlp_wgrad, or one
  *     gradient);  momentum <- beta momentum + G;  U = nesterov ? G + beta momentum : momentum;  w <- w (1 - lr weight_decay) - lr scale orth(U).
  *     0 <= beta < 1.  The operand store of the dense-layer launches is NOT rewritten: emx_mlp_mirror afterwards.
  *   Products run on operands of 22 bits with float32 accumulation (of at most 16 rows: in 64 bits); the bits are those of X_k's own size, also where
