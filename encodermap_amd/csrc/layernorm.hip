@@ -50,8 +50,8 @@ __device__ __forceinline__ float lanes_sum(float v) {
   return v;
 }
 
-// the sum over the TPR threads that share a row, in each of them.  More than a wave: one slot per wave in `area`, which the caller
-// gives each sum of a row anew (three in turn), so that one barrier is enough
+// the sum over the TPR threads that share a row, in each of them.  More than a wave: one slot per wave in `area`, behind ONE barrier -- the
+// same area may be written again only once another barrier has been passed since it was read, so the caller has two at least and takes them in turn
 template <int TPR>
 __device__ __forceinline__ float row_sum(float v, float* area) {
   if constexpr (TPR <= 64) return lanes_sum<TPR>(v);
@@ -122,7 +122,8 @@ __device__ __forceinline__ void load_weights(const float* w, float other, int co
 template <typename T, int TPR, int NV, int U>
 __global__ __launch_bounds__(TPR > NT ? TPR : NT) void ln_fwd_kernel(const FwdArgs a) {
   constexpr int V = Lane<T>::V, G = (TPR > NT ? TPR : NT) / TPR;
-  __shared__ float sm[3][TPR > 64 ? TPR / 64 : 1];
+  static_assert(TPR <= 64 || U == 1, "each of the two areas is used once: rows in turn would need them in turn");
+  __shared__ float sm[2][TPR > 64 ? TPR / 64 : 1];
   const int t = threadIdx.x % TPR, g = threadIdx.x / TPR;
   const float inv = 1.f / (float)a.D;
   const int step = TPR * V, first = t * V;
