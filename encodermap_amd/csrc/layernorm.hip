@@ -495,12 +495,16 @@ size_t size_of(int dtype) { return dtype == EMX_F32 ? 4 : 2; }
 bool fits(int64_t n, int64_t ld) { return ld >= 0 && n <= ((int64_t)1 << 58) / std::max<int64_t>(ld, 1); }
 bool aligned(const void* p, size_t es) { return (uintptr_t)p % es == 0; }
 
-// Is [a, a + n rows) clear of [b, ...), or the very same rows (the in-place form)?
+// Is [a, a + n rows) clear of [b, ...), or the very same rows (the in-place form)?  Clear are also different columns of rows of one stride
+// (blocks of one wider buffer), whichever rows: their places modulo the stride differ.
 bool disjoint_or_same(const void* a, long lda, const void* b, long ldb, long n, int D, size_t es) {
   if (a == b && lda == ldb) return true;
   const char *a0 = (const char*)a, *b0 = (const char*)b;
   const char *a1 = a0 + ((n - 1) * lda + D) * es, *b1 = b0 + ((n - 1) * ldb + D) * es;
-  return a1 <= b0 || b1 <= a0;
+  if (a1 <= b0 || b1 <= a0) return true;
+  if (lda != ldb || lda <= 0) return false;
+  const long stride = lda * (long)es, width = D * (long)es, ahead = (b0 - a0) % stride, shift = ahead < 0 ? ahead + stride : ahead;
+  return shift >= width && shift + width <= stride;
 }
 
 template <typename F>
