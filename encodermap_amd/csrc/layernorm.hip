@@ -10,6 +10,7 @@
 // over the parts.
 #include <algorithm>
 #include <cstdint>
+#include <initializer_list>
 
 #include "emx_common.h"
 
@@ -507,6 +508,22 @@ bool disjoint_or_same(const void* a, long lda, const void* b, long ldb, long n, 
   return shift >= width && shift + width <= stride;
 }
 
+// The memory of an operand, from its first element to its last (rows) or of n floats; none: null
+struct Span {
+  const char *lo, *hi;
+};
+Span rows_of(const void* p, long ld, long n, int D, size_t es) {
+  const char* lo = (const char*)p;
+  return {lo, p ? lo + ((n - 1) * ld + D) * es : lo};
+}
+Span vector_of(const float* p, size_t n) { return {(const char*)p, (const char*)(p ? p + n : p)}; }
+// does what is written share memory with any of the others?
+bool meets(Span out, std::initializer_list<Span> others) {
+  for (const Span& o : others)
+    if (out.lo && o.lo && out.lo < o.hi && o.lo < out.hi) return true;
+  return false;
+}
+
 template <typename F>
 int by_type(int dtype, F f) {
   if (dtype == EMX_F16) return f((_Float16)0);
@@ -579,11 +596,15 @@ int emx_layernorm_fwd(const void* x, int dtype, int64_t n_rows, int D, int64_t l
   EMX_REQUIRE(n_rows >= 0 && D >= 1 && D <= EMX_LAYERNORM_MAX_D, "%s: n_rows %lld, D %d", who, (long long)n_rows, D);
   EMX_REQUIRE(eps >= 0.f, "%s: eps %g", who, (double)eps);   // (refuses NaN)
   if (n_rows == 0) return EMX_OK;
+  EMX_REQUIRE(aligned(gamma, 4) && aligned(beta, 4) && aligned(mean, 4) && aligned(rstd, 4), "%s: gamma, beta, mean and rstd on float boundaries", who);
   EMX_REQUIRE(!mean || mean != rstd, "%s: mean and rstd are the same vector", who);
   EMX_REQUIRE(x && y && aligned(x, size_of(dtype)) && aligned(y, size_of(dtype)), "%s: x and y are needed, on element boundaries", who);
   EMX_REQUIRE(n_rows == 1 || (fits(n_rows, ldx) && fits(n_rows, ldy) && ldy >= D), "%s: row strides %lld, %lld of %d columns", who, (long long)ldx, (long long)ldy, D);
   if (n_rows == 1) ldx = ldy = D;
   EMX_REQUIRE(disjoint_or_same(x, ldx, y, ldy, n_rows, D, size_of(dtype)), "%s: x and y overlap without being the same rows", who);
+  const Span rx = rows_of(x, ldx, n_rows, D, size_of(dtype)), ry = rows_of(y, ldy, n_rows, D, size_of(dtype));
+  const Span vg = vector_of(gamma, D), vb = vector_of(beta, D), vm = vector_of(mean, n_rows), vr = vector_of(rstd, n_rows);
+  EMX_REQUIRE(!meets(ry, {vg, vb}) && !meets(vm, {rx, ry, vg, vb, vr}) && !meets(vr, {rx, ry, vg, vb}), "%s: what is written shares memory with another operand", who);
   const FwdArgs a{x, y, gamma, beta, mean, rstd, n_rows, ldx, ldy, D, eps};
   return by_type(dtype, [&](auto t) {
     return launch_fwd<decltype(t)>(who, a, (hipStream_t)stream);
@@ -600,6 +621,8 @@ int emx_layernorm_bwd(const void* dy, int64_t ld_dy, const void* x, int64_t ldx,
   EMX_REQUIRE(n_rows >= 0 && D >= 1 && D <= EMX_LAYERNORM_MAX_D, "%s: n_rows %lld, D %d", who, (long long)n_rows, D);
   const bool sums = dgamma || dbeta;
   const size_t es = size_of(dtype);
+  EMX_REQUIRE(aligned(gamma, 4) && aligned(mean, 4) && aligned(rstd, 4) && aligned(dgamma, 4) && aligned(dbeta, 4) && aligned(ws, 4),
+              "%s: vectors and workspace on float boundaries", who);
   if (n_rows > 0) {
     EMX_REQUIRE(dy && x && mean && rstd && aligned(dy, es) && aligned(x, es) && aligned(dx, es), "%s: dy, x, mean and rstd are needed, on element boundaries", who);
     EMX_REQUIRE(n_rows == 1 || (fits(n_rows, ld_dy) && fits(n_rows, ldx) && (!dx || (fits(n_rows, ld_dx) && ld_dx >= D))), "%s: row strides %lld, %lld, %lld of %d columns", who,
@@ -612,6 +635,14 @@ int emx_layernorm_bwd(const void* dy, int64_t ld_dy, const void* x, int64_t ldx,
   if (sums && parts > 0 && (!ws || ws_floats < emx_layernorm_ws_floats(n_rows, D)))
     return fail(EMX_EWORKSPACE, "%s: workspace of %zu floats, %zu needed", who, ws ? ws_floats : (size_t)0, emx_layernorm_ws_floats(n_rows, D));
   EMX_REQUIRE(!dgamma || dgamma != dbeta, "%s: dgamma and dbeta are the same vector", who);
+  if (n_rows > 0) {
+    // (dgamma and dbeta are written when everything but the parts has been read)
+    const Span rdy = rows_of(dy, ld_dy, n_rows, D, es), rx = rows_of(x, ldx, n_rows, D, es), rdx = rows_of(dx, ld_dx, n_rows, D, es);
+    const Span vg = vector_of(gamma, D), vm = vector_of(mean, n_rows), vr = vector_of(rstd, n_rows), part = vector_of(sums ? ws : nullptr, emx_layernorm_ws_floats(n_rows, D));
+    EMX_REQUIRE(!meets(rdx, {vg, vm, vr}) && !meets(part, {rdy, rx, rdx, vg, vm, vr}), "%s: what is written shares memory with another operand", who);
+    EMX_REQUIRE(!meets(vector_of(dgamma, D), {rdx, part}) && !meets(vector_of(dbeta, D), {rdx, part}), "%s: what is written shares memory with another operand", who);
+  }
+  EMX_REQUIRE(!meets(vector_of(dgamma, D), {vector_of(dbeta, D)}), "%s: dgamma and dbeta share memory", who);
   hipStream_t st = (hipStream_t)stream;
   if (n_rows > 0) {
     const BwdArgs a{dy, x, dx, gamma, mean, rstd, sums ? ws : nullptr, n_rows, ld_dy, ldx, ld_dx, (n_rows + parts - 1) / parts, D, parts};

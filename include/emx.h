@@ -579,7 +579,8 @@ int emx_mlp_wgrad_adam_local(const emx_mlp_desc* desc, float* params, int64_t n_
  *   gamma, beta, mean, rstd, dgamma, dbeta: float32.  gamma / beta NULL: ones / zeros.  mean / rstd NULL (forward): not kept.
  *   dx, dgamma, dbeta NULL: not wanted.  dgamma and dbeta are overwritten, not added to; without rows they are zero.
  *   y may be x, dx may be dy or x (same pointer, same stride), and they may be different columns of a buffer's rows (same stride); any other overlap
- *   of their address ranges is refused.  mean and rstd, dgamma and dbeta are two vectors each.
+ *   of their address ranges is refused.  What is written (y, mean, rstd; dx, dgamma, dbeta, ws) otherwise shares no memory with any other operand
+ *   (refused too; dgamma and dbeta may lie where dy, x, gamma, mean or rstd do: they are written last).
  *   A row with an infinity or a NaN gives NaN in its own results (and in dgamma / dbeta); eps = 0 gives NaN for a constant row.  Sums are
  *   float32 at least: a row that leaves its mean by more than 1e19 overflows its sum of squares
  *   (rstd = 0), one whose sum passes float32's range gives infinities and NaN.
