@@ -581,7 +581,8 @@ int emx_mlp_wgrad_adam_local(const emx_mlp_desc* desc, float* params, int64_t n_
  *   y may be x, dx may be dy or x (same pointer, same stride), and they may be different columns of a buffer's rows (same stride); any other overlap
  *   of their address ranges is refused.  What is written (y, mean, rstd; dx, dgamma, dbeta, ws) otherwise shares no memory with any other operand
  *   (refused too; dgamma and dbeta may lie where dy, x, gamma, mean or rstd do: they are written last).
- *   A row with an infinity or a NaN gives NaN in its own results (and in dgamma / dbeta); eps = 0 gives NaN for a constant row.  Sums are
+ *   A row with an infinity or a NaN gives NaN in its own results (and in dgamma / dbeta).  eps = 0: the results of a constant row mean nothing (what
+ *   the rounding of its mean leaves of zero is divided by its own size: NaN, an infinity or values of about one); other rows need no eps.  Sums are
  *   float32 at least: a row that leaves its mean by more than 1e19 overflows its sum of squares
  *   (rstd = 0), one whose sum passes float32's range gives infinities and NaN.
  *   ws: emx_layernorm_ws_floats(n_rows, D) floats of scratch (may be NULL where dgamma and dbeta are); its contents mean nothing
