@@ -8,7 +8,7 @@
 // multiplies the small ones by up to 3.4, so after five steps those above ~1e-2 lie around one.  Hence the bounds every stored value
 // obeys, whatever G is: |X| <= 1.21, |A| <= 1.45, |P| <= 2.81.
 //
-// Arithmetic: as the dense layers', every float32 product is THREE f16 matrix instructions on operands split into two f16 planes (hi = f16(v),
+// Arithmetic (matrices of at most 48 rows: float32 or 64 bits, ns_low_kernel): as the dense layers', every float32 product is THREE f16 matrix instructions on operands split into two f16 planes (hi = f16(v),
 // lo = f16(v - hi): 22 bits), accumulated in float32.  The bounds above make a scale of 2^14 enough for X, A and P (|P| 2^14 <= 46.1e3
 // < 65504; what is lost below is 2^-24 2^-14 of the matrix' norm).  Where |G|_F is small beside eps, |X_0|_F = |G|_F / (|G|_F + eps) is too, and
 // X is held another 2^q times as large (X~ = 2^q X), so that |X~| <= 1/2:  A~ = X~ X~^T = 4^q A,  P~ = b A~ + 4^-q c A~^2 = 4^q P (|P~| <= 1.2),
@@ -1008,6 +1008,169 @@ __device__ void thin_matrix(Thin& l, double* sm, const Mat& m, const Scratch& s,
   if (step < steps && mine) reinterpret_cast<double*>(shares_out + (long)wg * 16 * BLK)[entry] = sum;
 }
 
+// ---- ... and of 17 to 48 rows, on float32 operands: split ones are rounded twice, and in matrices of so few rows whose singular values lie close together
+// (gradients that are mostly noise) that made 1.3 times float32's error on average, 2.1 at worst; these make 0.7 times it.  Five steps of 32 x 128 take 17.7 us
+// (19.9 on split operands), of 48 x 128 25.3 (25.4), of 20 x 9000 73 (79); 64 x 128 35.6 (25.7): there the float32 instructions bound it, and split operands are
+// as exact as float32 again.  Tiles of v_mfma_f32_16x16x4_f32 -- lane l: row l % 16 of either
+// operand, k = l / 16; results: rows 4 (l / 16) + i, column l % 16.  A lane takes four consecutive k of a row at a time, one to each of four such instructions: both
+// operands of a product have their k in that order.  Wave w holds the blocks (w / 8, w % 8) and (w / 8 + 2, w % 8) of the strip's 3 x 8 in registers.
+constexpr int SMALL = 48;
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+struct Small {
+  float x[SMALL][132], a[SMALL][68];   // (a row is four banks behind the one above it: neither rows nor columns of 16 meet)
+};
+static_assert(sizeof(Small) <= 2 * LOW_AREA, "the low kernel's LDS");
+
+template <typename T, bool MUON>
+__device__ void small_matrix(Small& l, double* sm, const Mat& m, const Scratch& s, const StepArgs& a, const int wg, const int step) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lr = lane & 15, h = lane >> 4, M = s.M, nb = (M + 15) / 16, wgs = s.low_wgs(), steps = a.steps;
+  const long pitch = 32l * s.Nb;
+  int ib = 0, jb = wave;                                               // this wave's block of the upper half of A and P
+  for (; ib < nb && jb >= nb; ++ib) jb -= nb - ib - 1;
+  const bool square = ib < nb;
+  const int cb = wave & 7, rb = 16 * cb < s.N ? wave >> 3 : nb;        // its blocks of X: rows rb, rb + 2 (none behind the matrix' last column)
+  f32x4 y[2];                                                          // ... their values
+  auto each = [&](auto take) __attribute__((always_inline)) {          // take(value, row, column of the strip)
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+      if (rb + 2 * j < nb)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float v = y[j][i];
+          take(v, 16 * (rb + 2 * j) + 4 * h + i, 16 * cb + lr);
+          y[j][i] = v;
+        }
+  };
+  auto product = [&](const float* u, const float* v, int k16) __attribute__((always_inline)) {   // rows u times rows v, 16 k16 long
+    f32x4 even{}, odd{};
+    for (int k = 0; k < k16; ++k) {
+      const f32x4 fu = *reinterpret_cast<const f32x4*>(u + 16 * k), fv = *reinterpret_cast<const f32x4*>(v + 16 * k);
+      even = __builtin_amdgcn_mfma_f32_16x16x4f32(fu[0], fv[0], even, 0, 0, 0);
+      odd = __builtin_amdgcn_mfma_f32_16x16x4f32(fu[1], fv[1], odd, 0, 0, 0);
+      even = __builtin_amdgcn_mfma_f32_16x16x4f32(fu[2], fv[2], even, 0, 0, 0);
+      odd = __builtin_amdgcn_mfma_f32_16x16x4f32(fu[3], fv[3], odd, 0, 0, 0);
+    }
+    return even + odd;
+  };
+  auto put = [&]() __attribute__((always_inline)) {
+    each([&](float& v, int r, int c) { l.x[r][c] = v; });
+    __syncthreads();
+  };
+  auto gram = [&](int st) __attribute__((always_inline)) {             // of the strip in l.x
+    f32x4 v{};
+    if (square) v = product(&l.x[16 * ib + lr][4 * h], &l.x[16 * jb + lr][4 * h], (min(s.N - 128 * st, 128) + 15) / 16);
+    return v;
+  };
+  auto keep = [&](const f32x4 v) __attribute__((always_inline)) {      // a block of A or P, and its mirror image
+    if (square) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) l.a[16 * ib + 4 * h + i][16 * jb + lr] = v[i];
+      if (ib != jb) *reinterpret_cast<f32x4*>(&l.a[16 * jb + lr][16 * ib + 4 * h]) = v;
+    }
+    __syncthreads();
+  };
+  auto poly = [&](f32x4 v) __attribute__((always_inline)) {            // v: A.  Leaves P in l.a
+    keep(v);
+    f32x4 sq{};
+    if (square) sq = product(&l.a[16 * ib + lr][4 * h], &l.a[16 * jb + lr][4 * h], nb);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = fmaf(CC, sq[i], CB * v[i]);
+    __syncthreads();
+    keep(v);
+  };
+  auto next = [&]() __attribute__((always_inline)) {                   // y <- a X + P X
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+      if (rb + 2 * j < nb) {
+        f32x4 even{}, odd{};
+        for (int k = 0; k < nb; ++k) {
+          const f32x4 p = *reinterpret_cast<const f32x4*>(&l.a[16 * (rb + 2 * j) + lr][16 * k + 4 * h]);
+          const float* const x = &l.x[16 * k + 4 * h][16 * cb + lr];
+          even = __builtin_amdgcn_mfma_f32_16x16x4f32(p[0], x[0], even, 0, 0, 0);
+          odd = __builtin_amdgcn_mfma_f32_16x16x4f32(p[1], x[132], odd, 0, 0, 0);
+          even = __builtin_amdgcn_mfma_f32_16x16x4f32(p[2], x[264], even, 0, 0, 0);
+          odd = __builtin_amdgcn_mfma_f32_16x16x4f32(p[3], x[396], odd, 0, 0, 0);
+        }
+        y[j] = even + odd;
+      }
+    each([&](float& v, int r, int c) { v = fmaf(CA, l.x[r][c], v); });
+    __syncthreads();
+  };
+  auto share = [&](char* shares, int g) { return reinterpret_cast<f32x4*>(shares + (long)g * 16 * BLK + (ib * 4 + jb) * 1024 + lane * 16); };
+  auto travel = [&](char* t, int st) __attribute__((always_inline)) {  // X from step to step: float32 rows
+    each([&](float& v, int r, int c) {
+      if (r < M && 128 * st + c < pitch) reinterpret_cast<float*>(t)[r * pitch + 128 * st + c] = v;
+    });
+  };
+  auto write = [&](int st) __attribute__((always_inline)) {
+    each([&](float& v, int r, int c) {
+      const int j = 128 * st + c;
+      if (r < M && j < s.N) {
+        const long at = m.off + (s.turned ? j * m.ld + r : r * m.ld + j);
+        if constexpr (MUON) a.w[at] = fmaf(a.w[at], a.keep, -(a.lr * m.scale) * v);
+        else ((T*)a.out)[at] = (T)v;
+      }
+    });
+  };
+  f32x4 sum{};
+  if (step == 0) {
+    const double f = start_of<LOW_NT>(m, s, a.eps, sm).inv;
+    for (int st = wg; st < s.strips(); st += wgs) {
+      if (st != wg) __syncthreads();                                   // (l.x may still be read for the strip before)
+      each([&](float& v, int r, int c) {
+        const int j = 128 * st + c;
+        v = 0.f;
+        if (r < M && j < s.N) {
+          const long gr = s.turned ? j : r, gc = s.turned ? r : j;
+          v = (float)(f * (double)(MUON ? reinterpret_cast<const float*>(s.t1)[gr * m.cols + gc] : (float)((const T*)a.g)[m.off + gr * m.ld + gc]));
+        }
+      });
+      if (a.low_steps) travel(s.t0, st);
+      put();
+      sum += gram(st);
+    }
+    if (a.low_steps) {
+      if (square) *share(s.a, wg) = sum;
+      return;
+    }
+    for (int k = 0; k < steps; ++k) {
+      poly(k == 0 ? sum : gram(0));
+      next();
+      if (k + 1 < steps) put();
+    }
+    write(0);
+    return;
+  }
+  char *const shares_in = (step & 1) ? s.a : s.p, *const shares_out = (step & 1) ? s.p : s.a;
+  char *const t_in = (step & 1) ? s.t0 : s.t1, *const t_out = (step & 1) ? s.t1 : s.t0;
+  auto request = [&](int st) __attribute__((always_inline)) {
+    each([&](float& v, int r, int c) { v = r < M && 128 * st + c < pitch ? reinterpret_cast<const float*>(t_in)[r * pitch + 128 * st + c] : 0.f; });
+  };
+  request(wg);                                                         // (on its way while the shares are added up)
+  if (square)
+#pragma unroll 8
+    for (int g = 0; g < wgs; ++g) sum += *share(shares_in, g);
+  poly(sum);
+  sum = f32x4{};
+  for (int st = wg; st < s.strips(); st += wgs) {
+    if (st != wg) {
+      __syncthreads();
+      request(st);
+    }
+    put();
+    next();
+    if (step == steps) {
+      write(st);
+      continue;
+    }
+    travel(t_out, st);
+    put();
+    sum += gram(st);
+  }
+  if (step < steps && square) *share(shares_out, wg) = sum;
+}
+
 template <typename T, bool MUON>
 __global__ __launch_bounds__(LOW_NT) void ns_low_kernel(char* ws, const int n, const int step /* 0: X_0 and its A (or everything) */) {
   extern __shared__ __align__(16) char lds[];
@@ -1024,6 +1187,10 @@ __global__ __launch_bounds__(LOW_NT) void ns_low_kernel(char* ws, const int n, c
   const int wgs = s.low_wgs(), Mb = s.Mb;
   if (s.M <= THIN) {
     thin_matrix<T, MUON>(*reinterpret_cast<Thin*>(lds), sm, m, s, a, wg, step);
+    return;
+  }
+  if (s.M <= SMALL) {
+    small_matrix<T, MUON>(*reinterpret_cast<Small*>(lds), sm, m, s, a, wg, step);
     return;
   }
   const bool rows = ib < Mb, square = ib <= jb && jb < Mb;   // this wave has a block of X; of the upper half of A and P

@@ -609,7 +609,7 @@ int emx_layernorm_bwd(const void* dy, int64_t ld_dy, const void* x, int64_t ldx,
  *   emx_muon_step, float32:  G = sum over n_slices of g[s * slice_stride + .] in a fixed order (the weight-gradient partials of emx_mlp_wgrad, or one
  *     gradient);  momentum <- beta momentum + G;  U = nesterov ? G + beta momentum : momentum;  w <- w (1 - lr weight_decay) - lr scale orth(U).
  *     0 <= beta < 1.  The operand store of the dense-layer launches is NOT rewritten: emx_mlp_mirror afterwards.
- *   Products run on operands of 22 bits with float32 accumulation (of at most 16 rows: in 64 bits); the bits are those of X_k's own size, also where
+ *   Products run on operands of 22 bits with float32 accumulation (17 to 48 rows: of float32; at most 16: in 64 bits); the bits are those of X_k's own size, also where
  *   |G|_F is far below eps and the result small with it (down to |G|_F = 1e-29 eps).  An infinity or a NaN in a matrix makes its result NaN, a matrix of
  *   zeros stays zero.  1 <= steps <= EMX_ORTHOGONALIZE_MAX_STEPS, sides up to EMX_MATRIX_MAX_SIDE (more: EMX_EUNSUPPORTED), eps > 0.
  *   ws: emx_orthogonalize_ws_bytes(mats, n_mats) bytes of scratch on a 16-byte boundary (0 from that function: the matrices are refused); its
