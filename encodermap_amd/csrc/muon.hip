@@ -1403,6 +1403,12 @@ bool share(const void* a, const void* b, int64_t lo, int64_t hi, int64_t more, s
   return a0 < b1 && b0 < a1;
 }
 
+// ... elements [lo, hi) of a buffer and a workspace?
+bool covers(const void* ws, size_t bytes, const void* a, int64_t lo, int64_t hi, size_t es) {
+  const uintptr_t w0 = (uintptr_t)ws, a0 = (uintptr_t)a + lo * es, a1 = (uintptr_t)a + hi * es;
+  return a0 < w0 + bytes && w0 < a1;
+}
+
 // hands out the workgroups (or tiles) of a launch
 template <typename F>
 long number(Table& t, int launch, F blocks) {
@@ -1555,8 +1561,8 @@ size_t ws_bytes_of(const emx_matrix* mats, int n) {   // (groups run one after t
   return most;
 }
 
-int check_workspace(const char* who, const emx_matrix* mats, int n, const void* ws, size_t ws_bytes) {
-  const size_t need = ws_bytes_of(mats, n);
+int check_workspace(const char* who, const emx_matrix* mats, int n, const void* ws, size_t ws_bytes, size_t& need) {
+  need = ws_bytes_of(mats, n);
   if (!ws || ws_bytes < need || ((uintptr_t)ws & 15))
     return fail(EMX_EWORKSPACE, "%s: workspace of %zu bytes at %p, %zu needed on a 16-byte boundary", who, ws_bytes, ws, need);
   return EMX_OK;
@@ -1584,7 +1590,9 @@ int emx_orthogonalize(const emx_matrix* mats, int n_mats, const void* g, void* o
   int64_t lo, hi;
   extent(mats, n_mats, lo, hi);
   EMX_REQUIRE(g == out || !share(g, out, lo, hi, 0, es), "%s: g and out overlap without being the same buffer", who);
-  if ((rc = check_workspace(who, mats, n_mats, ws, ws_bytes))) return rc;
+  size_t need;
+  if ((rc = check_workspace(who, mats, n_mats, ws, ws_bytes, need))) return rc;
+  EMX_REQUIRE(!covers(ws, need, g, lo, hi, es) && !covers(ws, need, out, lo, hi, es), "%s: the workspace lies in the matrices' memory", who);
   StepArgs a{};
   a.g = g, a.out = out, a.n_slices = 1, a.steps = steps, a.eps = eps;
   hipStream_t st = (hipStream_t)stream;
@@ -1611,7 +1619,10 @@ int emx_muon_step(const emx_matrix* mats, int n_mats, float* w, const float* g, 
   const int64_t more = n_slices > 1 ? (n_slices - 1) * slice_stride : 0;
   EMX_REQUIRE(!share(w, momentum, lo, hi, 0, 4) && !share(w, g, lo, hi, more, 4) && !share(momentum, g, lo, hi, more, 4),
               "%s: w, g and momentum have to be three buffers", who);
-  if ((rc = check_workspace(who, mats, n_mats, ws, ws_bytes))) return rc;
+  size_t need;
+  if ((rc = check_workspace(who, mats, n_mats, ws, ws_bytes, need))) return rc;
+  EMX_REQUIRE(!covers(ws, need, w, lo, hi, 4) && !covers(ws, need, momentum, lo, hi, 4) && !covers(ws, need, g, lo, hi + more, 4),
+              "%s: the workspace lies in the matrices' memory", who);
   StepArgs a{};
   a.g = g, a.w = w, a.mom = momentum, a.slice_stride = slice_stride, a.n_slices = n_slices, a.nesterov = nesterov != 0, a.steps = steps;
   a.beta = beta, a.keep = (float)(1.0 - (double)lr * weight_decay), a.lr = lr, a.eps = eps;

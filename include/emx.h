@@ -613,7 +613,8 @@ int emx_layernorm_bwd(const void* dy, int64_t ld_dy, const void* x, int64_t ldx,
  *   |G|_F is far below eps and the result small with it (down to |G|_F = 1e-29 eps).  An infinity or a NaN in a matrix makes its result NaN, a matrix of
  *   zeros stays zero.  1 <= steps <= EMX_ORTHOGONALIZE_MAX_STEPS, sides up to EMX_MATRIX_MAX_SIDE (more: EMX_EUNSUPPORTED), eps > 0.
  *   ws: emx_orthogonalize_ws_bytes(mats, n_mats) bytes of scratch on a 16-byte boundary (0 from that function: the matrices are refused); its
- *   contents mean nothing between calls, calls that may run at the same time need one each.  `mats` is host memory, read during the call.
+ *   contents mean nothing between calls, calls that may run at the same time need one each; refused where it lies between the first and the last element of
+ *   a buffer's matrices.  `mats` is host memory, read during the call.
  * ------------------------------------------------------------------------------------------------ */
 #define EMX_MATRIX_MAX_SIDE 32768
 #define EMX_ORTHOGONALIZE_MAX_STEPS 64
