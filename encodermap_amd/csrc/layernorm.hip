@@ -119,7 +119,8 @@ __device__ __forceinline__ void load_weights(const float* w, float other, int co
 
 // ---- rows that fit into registers: TPR threads hold a row, thread t its vectors t, t + TPR, ... (NV of them); each thread works on U
 // rows at a time, whose loads are all requested before the first is used.  Bound by HBM: 1e6 x 128 f32 181 us = 5.7 TB/s (a workgroup per
-// row with its sums through LDS: 969); 10007 x 1001 bf16 11.9 us = 3.7 TB/s, the start and end of so short a launch; 256 x 128 3.7 us, a launch.
+// row with its sums through LDS: 969); 10007 x 1001 bf16, whose 40 MB stay in the last-level cache from call to call, 11.5 us = 3.5 TB/s, the start
+// and end of so short a launch (15.5 with buffers in turn that do not); 256 x 128 3.7 us, a launch.
 template <typename T, int TPR, int NV, int U>
 __global__ __launch_bounds__(TPR > NT ? TPR : NT) void ln_fwd_kernel(const FwdArgs a) {
   constexpr int V = Lane<T>::V, G = (TPR > NT ? TPR : NT) / TPR;
@@ -197,8 +198,10 @@ __global__ __launch_bounds__(TPR > NT ? TPR : NT) void ln_fwd_kernel(const FwdAr
 
 // ---- backward, rows that fit into registers: workgroup p walks the rows of part p, G at a time, TPR threads to a row; a thread keeps the
 // sums of ITS columns over the part's rows, the G groups' are added through LDS at the end.  The next rows' loads travel under this row's sums.
-// Bound by HBM: 65536 x 1024 bf16 87 us = 4.6 TB/s, 2047 x 2850 f32 18.3 us = 3.8 TB/s -- where twice and half the threads, vectors or parts are
-// all within 5 %; 4096 x 128 f32 3.8 us.
+// Bound by HBM: 65536 x 1024 bf16 87 us = 4.6 TB/s; 2047 x 2850 f32, whose 70 MB stay in the last-level cache, 18.3 us (with the sum of the parts 20.8,
+// and 25.3 with buffers in turn that do not) -- where twice and half the threads, vectors or parts are all within 5 %; 4096 x 128 f32 3.8 us.
+// 16-bit rows of more than 8192 values spill fifteen registers a thread (4096 x 12288 bf16 154 us, 16384 131); with gamma read again for each row
+// instead of kept the compiler spills others, and the times are the same.
 template <typename T, int TPR, int NV>
 __global__ __launch_bounds__(TPR > NT ? TPR : NT) void ln_bwd_kernel(const BwdArgs a) {
   constexpr int V = Lane<T>::V, NB = TPR > NT ? TPR : NT, G = NB / TPR;
@@ -306,8 +309,9 @@ __global__ __launch_bounds__(TPR > NT ? TPR : NT) void ln_bwd_kernel(const BwdAr
 
 // ---- rows of any length: one workgroup per row walks it once per sum, four vectors of each thread on their way at a time.  A vector's values are
 // added in 32 bits, the vectors of a thread -- up to 2^16 of them -- in 64 (in 32 the roundings of equal terms all go one way: 2^20 times
-// 1.1 comes out 1 % off).  4096 x 20000 f32 forward 169 us = 3.9 TB/s of what has to move (the second and third walk find the row in the caches),
-// backward 400; two rows of 2^24 3.4 ms, what one CU each can fetch.  Eight loads in flight: within 4 % either way.
+// 1.1 comes out 1 % off).  4096 x 20000 f32 forward 169-184 us = 3.6-3.9 TB/s of what has to move (the second and third walk find the row in the caches),
+// backward 400-415, three walks and the sums over rows; 4096 x 12288 f32 backward 250, 16384 341; two rows of 2^24 3.4 and 6.0 ms, one CU each: fewer rows
+// than CUs leave the others idle.  Eight loads in flight: within 4 % either way.
 constexpr int LONG_NT = 1024, LONG_U = 4;
 template <typename T, typename F>
 __device__ __forceinline__ void walk(const T* x, int D, F take /* (vector, its first column, elements of the row from there on) */) {

@@ -3,16 +3,18 @@
 //
 //   X_0 = G / (|G|_F + eps)    (G transposed where it has more rows than columns, so that X is M x N with M <= N)
 //   A = X X^T,  P = b A + c A^2,  X <- a X + P X       `steps` times; (a, b, c) = (3.4445, -4.7750, 2.0315)
+// (K. Jordan et al., "Muon: An optimizer for hidden layers in neural networks", 2024.)
 //
 // A singular value s of X goes to s (a + b s^2 + c s^4): that polynomial maps [0, 1] into [0, 1.2024] and [0, 1.2024] into itself, and
 // multiplies the small ones by up to 3.4, so after five steps those above ~1e-2 lie around one.  Hence the bounds every stored value
 // obeys, whatever G is: |X| <= 1.21, |A| <= 1.45, |P| <= 2.81.
 //
-// Arithmetic (matrices of at most 48 rows: float32 or 64 bits, ns_low_kernel): as the dense layers', every float32 product is THREE f16 matrix instructions on operands split into two f16 planes (hi = f16(v),
-// lo = f16(v - hi): 22 bits), accumulated in float32.  The bounds above make a scale of 2^14 enough for X, A and P (|P| 2^14 <= 46.1e3
-// < 65504; what is lost below is 2^-24 2^-14 of the matrix' norm).  Where |G|_F is small beside eps, |X_0|_F = |G|_F / (|G|_F + eps) is too, and
-// X is held another 2^q times as large (X~ = 2^q X), so that |X~| <= 1/2:  A~ = X~ X~^T = 4^q A,  P~ = b A~ + 4^-q c A~^2 = 4^q P (|P~| <= 1.2),
-// and a X~ + 4^-q P~ X~ = 2^q X_k+1.  q shrinks from step to step by what |X| may have grown (shift_at).  The norm is summed in 64 bits: an error of its scale is the one that
+// Arithmetic (of matrices of more than 48 rows; of smaller ones: float32 and 64 bits, ns_low_kernel): as the dense layers', every float32
+// product is THREE f16 matrix instructions on operands split into two f16 planes (hi = f16(v), lo = f16(v - hi): 22 bits), accumulated in
+// float32.  The bounds above make a scale of 2^14 enough for X, A and P (|P| 2^14 <= 46.1e3 < 65504; what is lost below is 2^-24 2^-14 of the
+// matrix' norm).  Where |G|_F is small beside eps, |X_0|_F = |G|_F / (|G|_F + eps) is too, and X is held another 2^q times as large
+// (X~ = 2^q X), so that |X~| <= 1/2:  A~ = X~ X~^T = 4^q A,  P~ = b A~ + 4^-q c A~^2 = 4^q P (|P~| <= 1.2), and a X~ + 4^-q P~ X~ = 2^q X_k+1.
+// q shrinks from step to step by what |X| may have grown (shift_at).  The norm is summed in 64 bits: an error of its scale is the one that
 // the iteration turns into an error of every singular value.  a X joins P X behind its sum, not as a diagonal of P: the sum then rounds at the
 // size of P X alone (4096 x 4096: 4.4e-6 off with it inside).
 //

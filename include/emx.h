@@ -599,7 +599,8 @@ int emx_layernorm_bwd(const void* dy, int64_t ld_dy, const void* x, int64_t ldx,
 
 /* ------------------------------------------------------------------------------------------------ *
  * Orthogonalised matrix updates (csrc/muon.hip): an optimizer for the KERNELS of a network beside emx_adam_step* above (which stays the one
- * for biases, norms' weights and whatever is no matrix).  The reference's only optimizer is Adam (autoencoder.py:741-743).
+ * for biases, norms' weights and whatever is no matrix).  The reference's only optimizer is Adam (autoencoder.py:741-743).  The iteration, its coefficients and the
+ * five steps are those of K. Jordan et al., "Muon: An optimizer for hidden layers in neural networks" (2024).
  *   orth(G): X = G / (|G|_F + eps); `steps` times  A = X X^T, X <- a X + (b A + c A A) X  with (a, b, c) = (3.4445, -4.7750, 2.0315)
  *   (X^T in X's place where G has more rows than columns).  All singular values of G above ~1e-2 of its norm come out around 1 (0.68 .. 1.2).
  *   emx_matrix: a matrix of the flat buffers the call is given: rows x cols elements from `offset` on, row stride `ld` >= cols; `scale` is
@@ -608,7 +609,8 @@ int emx_layernorm_bwd(const void* dy, int64_t ld_dy, const void* x, int64_t ldx,
  *     buffer (any other overlap is refused, as is any between w, g and momentum below).  What lies between the matrices is neither read nor written.
  *   emx_muon_step, float32:  G = sum over n_slices of g[s * slice_stride + .] in a fixed order (the weight-gradient partials of emx_mlp_wgrad, or one
  *     gradient);  momentum <- beta momentum + G;  U = nesterov ? G + beta momentum : momentum;  w <- w (1 - lr weight_decay) - lr scale orth(U).
- *     0 <= beta < 1.  The operand store of the dense-layer launches is NOT rewritten: emx_mlp_mirror afterwards.
+ *     0 <= beta < 1.  Nothing else that emx_adam_step_slices does is done here: no L2 term (its l2 w belongs into G), no clipping, no regulariser cost, no next batch,
+ *     and the operand store of the dense-layer launches is NOT rewritten: emx_mlp_mirror afterwards.
  *   Products run on operands of 22 bits with float32 accumulation (17 to 48 rows: of float32; at most 16: in 64 bits); the bits are those of X_k's own size, also where
  *   |G|_F is far below eps and the result small with it (down to |G|_F = 1e-29 eps).  An infinity or a NaN in a matrix makes its result NaN, a matrix of
  *   zeros stays zero.  1 <= steps <= EMX_ORTHOGONALIZE_MAX_STEPS, sides up to EMX_MATRIX_MAX_SIDE (more: EMX_EUNSUPPORTED), eps > 0.
