@@ -298,8 +298,8 @@ def _counters_file(name):
     """(blob, path, reason): the newest per-launch counters of the configuration (rocprofv3 PMC passes over this script,
     tools/run_pmc_step.sh) IF they were taken on these kernel sources -- a file whose ``source_hash`` is not this build's is refused
     (None, path, why): numbers of another build are not quoted beside this one's timings."""
-    for rnd in ("r06", "r05", "r04", "r03", "r02"):
-        path = os.path.join("profiles", f"{rnd}_step_counters.json" if name == "C2" else f"{rnd}_{name.lower()}_counters.json")
+    for prefix in ("", "r06_", "r05_", "r04_", "r03_", "r02_"):     # (the newest has none)
+        path = os.path.join("profiles", f"{prefix}step_counters.json" if name == "C2" else f"{prefix}{name.lower()}_counters.json")
         try:
             blob = json.load(open(os.path.join(ROOT, path)))
         except Exception:
