@@ -1010,12 +1010,13 @@ __device__ void thin_matrix(Thin& l, double* sm, const Mat& m, const Scratch& s,
   if (step < steps && mine) reinterpret_cast<double*>(shares_out + (long)wg * 16 * BLK)[entry] = sum;
 }
 
-// ---- ... and of 17 to 48 rows, on float32 operands: split ones are rounded twice, and in matrices of so few rows whose singular values lie close together
-// (gradients that are mostly noise) that made 1.3 times float32's error on average, 2.1 at worst; these make 0.7 times it.  Five steps of 32 x 128 take 17.7 us
-// (19.9 on split operands), of 48 x 128 25.3 (25.4), of 20 x 9000 73 (79); 64 x 128 35.6 (25.7): there the float32 instructions bound it, and split operands are
-// as exact as float32 again.  Tiles of v_mfma_f32_16x16x4_f32 -- lane l: row l % 16 of either
-// operand, k = l / 16; results: rows 4 (l / 16) + i, column l % 16.  A lane takes four consecutive k of a row at a time, one to each of four such instructions: both
-// operands of a product have their k in that order.  Wave w holds the blocks (w / 8, w % 8) and (w / 8 + 2, w % 8) of the strip's 3 x 8 in registers.
+// ---- ... and of 17 to 48 rows, on float32 operands: split ones are rounded twice, and in matrices of so few rows whose singular values lie
+// close together (gradients that are mostly noise) that made 1.3 times float32's error on average, 2.1 at worst; these make 0.7 times it.
+// Five steps of 32 x 128 take 17.4 us (19.9 on split operands), of 48 x 128 24.4 (25.4), of 20 x 9000 73 (79), of 48 x 300 48.7 (42.6), of
+// 32000 x 40 217 (197): from 33 rows on the float32 instructions bound it.  64 x 128 35.6 (25.7), and there split operands are as exact as
+// float32 again.  Tiles of v_mfma_f32_16x16x4_f32 -- lane l: row l % 16 of either operand, k = l / 16; results: rows 4 (l / 16) + i, column
+// l % 16.  A lane takes four consecutive k of a row at a time, one to each of four such instructions: both operands of a product have their k
+// in that order.  Wave w holds the blocks (w / 8, w % 8) and (w / 8 + 2, w % 8) of the strip's 3 x 8 in registers.
 constexpr int SMALL = 48;
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 struct Small {
@@ -1105,38 +1106,69 @@ __device__ void small_matrix(Small& l, double* sm, const Mat& m, const Scratch& 
       if (r < M && 128 * st + c < pitch) reinterpret_cast<float*>(t)[r * pitch + 128 * st + c] = v;
     });
   };
-  auto write = [&](int st) __attribute__((always_inline)) {
-    each([&](float& v, int r, int c) {
-      const int j = 128 * st + c;
-      if (r < M && j < s.N) {
-        const long at = m.off + (s.turned ? j * m.ld + r : r * m.ld + j);
-        if constexpr (MUON) a.w[at] = fmaf(a.w[at], a.keep, -(a.lr * m.scale) * v);
-        else ((T*)a.out)[at] = (T)v;
+  // a strip of the caller's matrix: a lane's four values of a block lie side by side where the matrix is turned
+  typedef typename std::conditional<MUON, float, T>::type O;
+  typedef O quad __attribute__((ext_vector_type(4), aligned(sizeof(O))));
+  auto read = [&](const O* from, long ld, int st) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int r = 16 * (rb + 2 * j) + 4 * h, c = 128 * st + 16 * cb + lr;
+      y[j] = f32x4{};
+      if (rb + 2 * j >= nb || c >= s.N) continue;
+      if (s.turned && r + 4 <= M) {
+        const quad v = *reinterpret_cast<const quad*>(from + c * ld + r);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y[j][i] = (float)v[i];
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (r + i < M) y[j][i] = (float)from[s.turned ? c * ld + r + i : (r + i) * ld + c];
       }
-    });
+    }
+  };
+  auto write = [&](int st) __attribute__((always_inline)) {
+    O* const to = (MUON ? (O*)a.w : (O*)a.out) + m.off;
+    const float f = MUON ? -(a.lr * m.scale) : 1.f, keep = a.keep;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int r = 16 * (rb + 2 * j) + 4 * h, c = 128 * st + 16 * cb + lr;
+      if (rb + 2 * j >= nb || c >= s.N) continue;
+      if (s.turned && r + 4 <= M) {
+        quad* const at = reinterpret_cast<quad*>(to + c * m.ld + r);
+        quad o{};
+        if constexpr (MUON) o = *at;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[i] = MUON ? (O)fmaf((float)o[i], keep, f * y[j][i]) : (O)y[j][i];
+        *at = o;
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (r + i < M) {
+            O* const at = to + (s.turned ? c * m.ld + r + i : (r + i) * m.ld + c);
+            *at = MUON ? (O)fmaf((float)*at, keep, f * y[j][i]) : (O)y[j][i];
+          }
+      }
+    }
   };
   f32x4 sum{};
   if (step == 0) {
     const double f = start_of<LOW_NT>(m, s, a.eps, sm).inv;
+    const O* const from = MUON ? reinterpret_cast<const O*>(s.t1) : (const O*)a.g + m.off;
+    const long ld = MUON ? m.cols : m.ld;
+    read(from, ld, wg);
     for (int st = wg; st < s.strips(); st += wgs) {
       if (st != wg) __syncthreads();                                   // (l.x may still be read for the strip before)
-      each([&](float& v, int r, int c) {
-        const int j = 128 * st + c;
-        v = 0.f;
-        if (r < M && j < s.N) {
-          const long gr = s.turned ? j : r, gc = s.turned ? r : j;
-          v = (float)(f * (double)(MUON ? reinterpret_cast<const float*>(s.t1)[gr * m.cols + gc] : (float)((const T*)a.g)[m.off + gr * m.ld + gc]));
-        }
-      });
+      each([&](float& v, int, int) { v = (float)(f * (double)v); });
       if (a.low_steps) travel(s.t0, st);
       put();
+      if (st + wgs < s.strips()) read(from, ld, st + wgs);             // (on its way during the products)
       sum += gram(st);
     }
     if (a.low_steps) {
       if (square) *share(s.a, wg) = sum;
       return;
     }
-    for (int k = 0; k < steps; ++k) {
+    for (int k = 0; k < steps; ++k) {                                  // (one strip: y is its values still)
       poly(k == 0 ? sum : gram(0));
       next();
       if (k + 1 < steps) put();
@@ -1156,19 +1188,17 @@ __device__ void small_matrix(Small& l, double* sm, const Mat& m, const Scratch& 
   poly(sum);
   sum = f32x4{};
   for (int st = wg; st < s.strips(); st += wgs) {
-    if (st != wg) {
-      __syncthreads();
-      request(st);
-    }
+    if (st != wg) __syncthreads();
     put();
     next();
     if (step == steps) {
       write(st);
-      continue;
+    } else {
+      travel(t_out, st);
+      put();
     }
-    travel(t_out, st);
-    put();
-    sum += gram(st);
+    if (st + wgs < s.strips()) request(st + wgs);
+    if (step < steps) sum += gram(st);
   }
   if (step < steps && square) *share(shares_out, wg) = sum;
 }
